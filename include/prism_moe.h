@@ -69,6 +69,42 @@ int prism_moe_route_topk(const void* logits, int dtype, int64_t num_tokens, int3
                          int32_t top_k, int32_t renorm, int64_t* topk_ids, void* topk_weights,
                          int32_t* expert_counts, void* stream);
 
+/* Scored routing (prism_moe_route_scored). */
+#define PRISM_MOE_SCORE_SOFTMAX 0
+#define PRISM_MOE_SCORE_SIGMOID 1
+#define PRISM_MOE_GROUP_MAX 0    /* a group's score: its largest selection key               */
+#define PRISM_MOE_GROUP_TOP2 1   /* the sum of its two largest (of its one, if it has one)     */
+
+typedef struct prism_moe_router {
+  int32_t scoring;         /* PRISM_MOE_SCORE_*                                              */
+  const float* bias;       /* [E] added to the scores for the choice only, or NULL           */
+  int32_t num_groups;      /* groups of E / num_groups consecutive experts                   */
+  int32_t topk_groups;     /* groups that stay                                               */
+  int32_t group_score;     /* PRISM_MOE_GROUP_*                                              */
+  int32_t renorm;          /* divide the k weights by their sum + 1e-20                      */
+  float scale;             /* factor of the weights, after renorm                            */
+} prism_moe_router;
+
+/*
+ * Routing by scores, for blocks whose router is not plain softmax / top-k:
+ *   s     = softmax(logits) or sigmoid(logits), over the experts of one token
+ *   key   = s + bias; only experts of the topk_groups best groups can be chosen
+ *   ids   = the k experts with the largest keys, in descending order; equal keys (and equal group
+ *           scores) go to the lowest index
+ *   w     = s[ids] (without the bias), / (their sum + 1e-20) with renorm, * scale
+ * Keys, scores and weights are those of 64-bit arithmetic; weights are rounded once. NaN keys rank
+ * above all numbers, as torch.topk ranks them (a NaN logit makes its token's weights NaN); experts
+ * of groups that do not stay are never chosen, whatever the others hold.
+ *   logits [T, E] dtype; topk_ids [T, k] int64 out; topk_weights [T, k] weights_dtype out;
+ *   expert_counts [E] int32 out, or NULL.
+ * Limits: 1 <= E <= 1024, 1 <= k <= 32, num_groups <= 32 divides E, k <= topk_groups * E / num_groups.
+ * No counterpart in the reference, whose router is prism_moe_route_topk's.
+ */
+int prism_moe_route_scored(const void* logits, int dtype, int64_t num_tokens, int32_t num_experts,
+                           int32_t top_k, const prism_moe_router* router, int64_t* topk_ids,
+                           void* topk_weights, int weights_dtype, int32_t* expert_counts,
+                           void* stream);
+
 /* Bytes of scratch prism_moe_build_dispatch_plan needs. */
 size_t prism_moe_dispatch_workspace_size(int64_t num_tokens, int32_t top_k, int32_t num_experts,
                                          int32_t ep_size);
@@ -161,6 +197,54 @@ int prism_moe_expert_swiglu(const void* x_sorted, int dtype, int64_t rows_capaci
                             void* stream);
 
 /*
+ * 4-bit weights with group scales: W[n, k] = (code[n, k] - zero) * scale, one scale (and zero
+ * point) per row and group of group_size (32, 64 or 128) consecutive inputs; K must be a multiple of
+ * group_size. Held in tiles of 16 rows by 128 inputs (N padded to 16, K to 128; the padding's codes
+ * may be anything, its scales must be finite):
+ *   qweight [N/16][ceil(K/128)][16][64] bytes: a row's 64 bytes are 16 little-endian words of 8
+ *           codes, the word at 4 t + j (t, j < 4) holding inputs 32 j + 8 t .. + 7, nibbles from the
+ *           low end in the order 0 2 4 6 1 3 5 7 of the eight
+ *   scales  [N/16][ceil(K/128)][16][128 / group_size] bf16
+ *   zeros   the same shape, uint8 in 0..15; NULL: 8 everywhere
+ * A stack of E matrices holds them one after the other. gate_up matrices [2I, K] hold 8 gate rows
+ * and 8 up rows by turns: row 16 i + r is gate row 8 i + r (r < 8) or up row 8 i + r - 8.
+ * 16-byte aligned. prism_infer_b200/quant.py lays weights out.
+ */
+typedef struct prism_moe_w4 {
+  const void* qweight;
+  const void* scales;
+  const void* zeros;
+  int32_t group_size;
+} prism_moe_w4;
+
+/*
+ * y = x W^T for 4-bit weights: x [rows, in_features] and y [rows, out_features] bf16, row-major,
+ * 16-byte aligned, out_features % 8 == 0; any number of rows, one (a matrix-vector product)
+ * included. Sums are fp32, scales are applied to fp32 group sums, y is rounded once.
+ * Replaces F.linear of prism_infer/layers/linear.py:77,181 on quantised weights.
+ */
+int prism_moe_linear_w4(const void* x, int64_t rows, int64_t in_features, int64_t out_features,
+                        const prism_moe_w4* weight, void* y, void* stream);
+
+/* Bytes of scratch prism_moe_expert_swiglu_w4 needs. */
+size_t prism_moe_expert_w4_workspace_size(int64_t rows_capacity, int64_t inter);
+
+/*
+ * prism_moe_expert_swiglu on 4-bit weights (bf16 activations): w_gate_up stacks num_local_experts
+ * matrices [2I, H] (gate and up rows by turns, as above), w_down as many [H, I]. hidden and inter
+ * must be multiples of their matrix's group size. The gate and up sums stay in fp32; their product
+ * silu(g) * u is rounded to bf16, the operand type of the second product. Rows of no segment are
+ * left as they are; a segment whose seg_expert lies outside [0, num_local_experts) is skipped and
+ * records PRISM_MOE_ERR_ARG in ``device_error``.
+ */
+int prism_moe_expert_swiglu_w4(const void* x_sorted, int64_t rows_capacity, int64_t hidden,
+                               int64_t inter, const int32_t* seg_offsets,
+                               const int32_t* seg_expert, int32_t num_segments,
+                               int32_t num_local_experts, const prism_moe_w4* w_gate_up,
+                               const prism_moe_w4* w_down, void* y, void* workspace,
+                               size_t workspace_bytes, int* device_error, void* stream);
+
+/*
  * Weighted combine: out[t] = sum_j w[t, j] * expert_out[row(t*k + j)], row = entry_row[f]
  * (identity when entry_row is NULL). Each product is rounded to dtype and the k products are
  * summed in fp32 in slot order, then rounded once: the numerics of the reference's
@@ -233,6 +317,22 @@ int prism_moe_block_forward_norm(const void* x, const void* router_logits, int d
                                  int64_t* topk_ids, void* topk_weights, void* workspace,
                                  size_t workspace_bytes, void* stream,
                                  const prism_moe_norm_epilogue* epilogue);
+
+/*
+ * The block after its router, for a choice the caller made (prism_moe_route_topk,
+ * prism_moe_route_scored or its own): plan, gather, grouped SwiGLU experts, weighted combine, with
+ * the optional norm epilogue. Experts are ``w_gate_up`` / ``w_down`` in dtype, or, where those are
+ * NULL, the 4-bit ``q_gate_up`` / ``q_down`` (bf16 activations). Workspace: that of
+ * prism_moe_block_forward. Ids outside [0, E) add nothing to ``out`` and record PRISM_MOE_ERR_ARG in
+ * the workspace's first word.
+ */
+int prism_moe_block_forward_routed(const void* x, const int64_t* topk_ids,
+                                   const void* topk_weights, int dtype, int64_t num_tokens,
+                                   int64_t hidden, int64_t inter, int32_t num_experts,
+                                   int32_t top_k, const void* w_gate_up, const void* w_down,
+                                   const prism_moe_w4* q_gate_up, const prism_moe_w4* q_down,
+                                   void* out, void* workspace, size_t workspace_bytes,
+                                   void* stream, const prism_moe_norm_epilogue* epilogue);
 
 /* ---------------------------------------------------------------------------------------------
  * Expert parallelism over NVLink peer memory (one process per GPU).

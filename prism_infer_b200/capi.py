@@ -10,6 +10,7 @@ layers/moe.py:69-100).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import threading
 from pathlib import Path
@@ -33,12 +34,39 @@ class NormEpilogue(ctypes.Structure):
                 ("eps", ctypes.c_float), ("residual_out", ctypes.c_void_p)]
 
 
+class Router(ctypes.Structure):
+    """``prism_moe_router``: how prism_moe_route_scored scores, groups and weighs."""
+    _fields_ = [("scoring", ctypes.c_int32), ("bias", ctypes.c_void_p),
+                ("num_groups", ctypes.c_int32), ("topk_groups", ctypes.c_int32),
+                ("group_score", ctypes.c_int32), ("renorm", ctypes.c_int32),
+                ("scale", ctypes.c_float)]
+
+
+class W4(ctypes.Structure):
+    """``prism_moe_w4``: a 4-bit matrix or stack of matrices."""
+    _fields_ = [("qweight", ctypes.c_void_p), ("scales", ctypes.c_void_p),
+                ("zeros", ctypes.c_void_p), ("group_size", ctypes.c_int32)]
+
+
 _ep = ctypes.POINTER(NormEpilogue)
+_w4p = ctypes.POINTER(W4)
+SCORINGS = {"softmax": 0, "sigmoid": 1}
+GROUP_SCORES = {"max": 0, "top2": 1}
 _SIGNATURES = {
     "prism_moe_version": (ctypes.c_int, []),
     "prism_moe_last_error": (ctypes.c_char_p, []),
     "prism_moe_route_topk": (ctypes.c_int, [_vp, ctypes.c_int, _i64, _i32, _i32, _i32, _vp, _vp,
                                             _vp, _vp]),
+    "prism_moe_route_scored": (ctypes.c_int, [_vp, ctypes.c_int, _i64, _i32, _i32,
+                                              ctypes.POINTER(Router), _vp, _vp, ctypes.c_int,
+                                              _vp, _vp]),
+    "prism_moe_linear_w4": (ctypes.c_int, [_vp, _i64, _i64, _i64, _w4p, _vp, _vp]),
+    "prism_moe_expert_w4_workspace_size": (_sz, [_i64, _i64]),
+    "prism_moe_expert_swiglu_w4": (ctypes.c_int, [_vp, _i64, _i64, _i64, _vp, _vp, _i32, _i32,
+                                                  _w4p, _w4p, _vp, _vp, _sz, _vp, _vp]),
+    "prism_moe_block_forward_routed": (ctypes.c_int, [_vp, _vp, _vp, ctypes.c_int, _i64, _i64,
+                                                      _i64, _i32, _i32, _vp, _vp, _w4p, _w4p, _vp,
+                                                      _vp, _sz, _vp, _ep]),
     "prism_moe_dispatch_workspace_size": (_sz, [_i64, _i32, _i32, _i32]),
     "prism_moe_build_dispatch_plan": (ctypes.c_int, [_vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp,
                                                      _vp, _vp, _vp, _vp, _sz, _vp]),
@@ -165,6 +193,57 @@ def route_topk(logits, top_k: int, renorm: bool, with_counts: bool = False):
     return ids, w, counts
 
 
+def _one_device(*ts):
+    """The device all given CUDA tensors are on (contiguous, one device, or RuntimeError)."""
+    _need_cuda(*ts)
+    devs = {t.device for t in ts if t is not None}
+    if len(devs) != 1:
+        raise RuntimeError(f"tensors are on different devices: {sorted(map(str, devs))}")
+    return devs.pop()
+
+
+def _on(device):
+    """Context that makes ``device`` current (kernels launch on the current device)."""
+    torch = _torch()
+    if device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def route_scored(logits, top_k: int, *, scoring: str = "softmax", bias=None, num_groups: int = 1,
+                 topk_groups: int = 1, group_score: str = "max", renorm: bool = True,
+                 scale: float = 1.0, out_dtype=None, with_counts: bool = False):
+    """Routing by ``scoring`` ("softmax" or "sigmoid") scores of ``logits`` [T, E]: the ``top_k``
+    largest scores + ``bias`` (fp32 [E], for the choice only) among the ``topk_groups`` best of
+    ``num_groups`` groups (by ``group_score`` "max" or "top2"), equal keys to the lowest index; the
+    weights are the chosen scores, divided by their sum with ``renorm``, times ``scale``
+    (prism_moe_route_scored). Returns (topk_ids int64 [T,k], topk_weights [T,k] in ``out_dtype``,
+    by default the logits' dtype, expert_counts int32 [E] or None)."""
+    torch = _torch()
+    if scoring not in SCORINGS:
+        raise RuntimeError(f"unknown scoring {scoring!r}; one of {sorted(SCORINGS)}")
+    if group_score not in GROUP_SCORES:
+        raise RuntimeError(f"unknown group_score {group_score!r}; one of {sorted(GROUP_SCORES)}")
+    if logits.dim() != 2:
+        raise RuntimeError("route_scored: logits must be [T, E]")
+    dev = _one_device(logits, bias)
+    T, E = logits.shape
+    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (E,)):
+        raise RuntimeError(f"route_scored: bias must be float32 [{E}]")
+    out_dtype = logits.dtype if out_dtype is None else out_dtype
+    dt, wdt = dtype_code(logits.dtype), dtype_code(out_dtype)
+    ids = torch.empty(T, max(int(top_k), 0), dtype=torch.int64, device=dev)
+    w = torch.empty(T, max(int(top_k), 0), dtype=out_dtype, device=dev)
+    counts = torch.empty(E, dtype=torch.int32, device=dev) if with_counts else None
+    router = Router(SCORINGS[scoring], ptr(bias), num_groups, topk_groups,
+                    GROUP_SCORES[group_score], int(bool(renorm)), float(scale))
+    with _on(dev):
+        check(load().prism_moe_route_scored(ptr(logits), dt, T, E, top_k, ctypes.byref(router),
+                                            ptr(ids), ptr(w), wdt, ptr(counts), stream_of(dev)),
+              "prism_moe_route_scored")
+    return ids, w, counts
+
+
 def dispatch_plan(topk_ids, num_experts: int, ep_size: int, want_perm: bool = True):
     """Kernel 2 (plan) on ``topk_ids`` [T, k] int64. Returns a dict of int tensors: perm,
     input_splits, sorted_local_eid (int64, reference layout) and expert_counts,
@@ -229,6 +308,85 @@ def expert_swiglu(x_sorted, seg_offsets, w_gate_up, w_down, seg_expert=None, y=N
                                       ptr(seg_expert), nseg, El, ptr(w_gate_up), ptr(w_down),
                                       ptr(y), ptr(ws), ws_bytes, ptr(device_error),
                                       stream_of(x_sorted.device)), "prism_moe_expert_swiglu")
+    return y
+
+
+def _w4(weight) -> W4:
+    return W4(ptr(weight.qweight), ptr(weight.scales), ptr(weight.zeros), weight.group_size)
+
+
+def _need_bf16(x, what: str) -> None:
+    if x.dtype != _torch().bfloat16:
+        raise RuntimeError(f"{what}: 4-bit weights take bfloat16 activations, got {x.dtype}")
+
+
+def linear_w4(x, weight, out=None):
+    """y = x W^T for a 4-bit ``weight`` (``quant.W4Weight``, a single matrix): ``x`` [M, K] bf16, any
+    M from 0; returns [M, N] bf16 (prism_moe_linear_w4)."""
+    torch = _torch()
+    _need_bf16(x, "linear_w4")
+    if weight.stack is not None or weight.gate_up:
+        raise RuntimeError("linear_w4: takes a single matrix, no stack and no gate_up rows")
+    if x.dim() != 2 or x.shape[1] != weight.in_features:
+        raise RuntimeError(f"linear_w4: x {tuple(x.shape)} does not match {weight.in_features} "
+                           "inputs")
+    dev = _one_device(x, weight.qweight, out)
+    M, N = x.shape[0], weight.out_features
+    if out is None:
+        out = torch.empty(M, N, dtype=x.dtype, device=dev)
+    elif tuple(out.shape) != (M, N) or out.dtype != x.dtype:
+        raise RuntimeError("linear_w4: out must be [M, N] in x's dtype")
+    with _on(dev):
+        check(load().prism_moe_linear_w4(ptr(x), M, weight.in_features, N,
+                                         ctypes.byref(_w4(weight)), ptr(out), stream_of(dev)),
+              "prism_moe_linear_w4")
+    return out
+
+
+def _expert_shapes(what: str, H: int, w_gate_up, w_down):
+    """(experts, inter) of a pair of 4-bit expert stacks for hidden size ``H``."""
+    El, I = w_gate_up.stack, w_gate_up.out_features // 2
+    if El is None or not w_gate_up.gate_up or w_down.gate_up or w_down.stack != El or \
+            w_gate_up.in_features != H or \
+            (w_down.out_features, w_down.in_features) != (H, I):
+        raise RuntimeError(f"{what}: 4-bit expert weights do not match each other or hidden {H}")
+    return El, I
+
+
+def expert_swiglu_w4(x_sorted, seg_offsets, w_gate_up, w_down, seg_expert=None, y=None,
+                     device_error=None):
+    """Grouped SwiGLU experts on 4-bit weights (``quant.W4Weight`` stacks) over the segment table:
+    ``expert_swiglu`` with ``w_gate_up`` [El, 2I, H] and ``w_down`` [El, H, I] in 4 bits and bf16
+    activations (prism_moe_expert_swiglu_w4)."""
+    torch = _torch()
+    _need_bf16(x_sorted, "expert_swiglu_w4")
+    if x_sorted.dim() != 2:
+        raise RuntimeError("expert_swiglu_w4: x_sorted must be [R, H]")
+    R, H = x_sorted.shape
+    El, I = _expert_shapes("expert_swiglu_w4", H, w_gate_up, w_down)
+    dev = _one_device(x_sorted, seg_offsets, seg_expert, w_gate_up.qweight, w_down.qweight, y,
+                      device_error)
+    nseg = seg_offsets.numel() - 1
+    for name, t in (("seg_offsets", seg_offsets), ("seg_expert", seg_expert),
+                    ("device_error", device_error)):
+        if t is not None and t.dtype != torch.int32:
+            raise RuntimeError(f"expert_swiglu_w4: {name} must be int32")
+    if seg_expert is None and nseg != El:
+        raise RuntimeError(f"expert_swiglu_w4: {nseg} segments for {El} experts need seg_expert")
+    if seg_expert is not None and seg_expert.numel() != nseg:
+        raise RuntimeError("expert_swiglu_w4: seg_expert must name one expert per segment")
+    if y is None:
+        y = torch.empty_like(x_sorted)
+    elif y.shape != x_sorted.shape or y.dtype != x_sorted.dtype:
+        raise RuntimeError("expert_swiglu_w4: y must look like x_sorted")
+    lib = load()
+    ws_bytes = lib.prism_moe_expert_w4_workspace_size(R, I)
+    ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=dev)
+    with _on(dev):
+        check(lib.prism_moe_expert_swiglu_w4(
+            ptr(x_sorted), R, H, I, ptr(seg_offsets), ptr(seg_expert), nseg, El,
+            ctypes.byref(_w4(w_gate_up)), ctypes.byref(_w4(w_down)), ptr(y), ptr(ws), ws_bytes,
+            ptr(device_error), stream_of(dev)), "prism_moe_expert_swiglu_w4")
     return y
 
 
@@ -329,6 +487,65 @@ def block_forward(x, router_logits, w_gate_up, w_down, top_k: int, renorm: bool,
         ptr(w_down), ptr(out), None, None, ptr(ws), ws.numel(), stream_of(x.device),
         ctypes.byref(epilogue) if epilogue is not None else None),
         "prism_moe_block_forward")
+    return out
+
+
+def _routed_workspace(device, nbytes: int):
+    """The block's scratch: the (device, stream) workspace, or, while a CUDA graph is captured,
+    memory of that graph's own (two graphs never share it; its error word starts zero at every
+    replay and is not the one ``block_error_word`` returns)."""
+    torch = _torch()
+    if torch.cuda.is_current_stream_capturing():
+        ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
+        ws[:256].zero_()
+        return ws
+    return block_workspace(device, nbytes)
+
+
+def block_forward_routed(x, topk_ids, topk_weights, w_gate_up, w_down, out=None, epilogue=None):
+    """The block after its router for a given choice: ``topk_ids`` [T,k] int64 and ``topk_weights``
+    [T,k] in x's dtype; plan, gather, experts, combine (prism_moe_block_forward_routed). The experts
+    are tensors [E,2I,H] and [E,H,I], or two 4-bit stacks (``quant.W4Weight``)."""
+    torch = _torch()
+    from prism_infer_b200.quant import W4Weight
+    T, H = x.shape
+    k = topk_ids.shape[-1]
+    w4 = isinstance(w_gate_up, W4Weight)
+    if w4 != isinstance(w_down, W4Weight):
+        raise RuntimeError("block_forward_routed: give either dense or 4-bit expert weights")
+    if w4:
+        _need_bf16(x, "block_forward_routed")
+        E, I = _expert_shapes("block_forward_routed", H, w_gate_up, w_down)
+        held = (w_gate_up.qweight, w_down.qweight)
+    else:
+        E, twoI, H2 = w_gate_up.shape
+        I = twoI // 2
+        if H2 != H or tuple(w_down.shape) != (E, H, I):
+            raise RuntimeError("block_forward_routed: inconsistent shapes")
+        if w_gate_up.dtype != x.dtype or w_down.dtype != x.dtype:
+            raise RuntimeError("block_forward_routed: weights must have the hidden dtype")
+        held = (w_gate_up, w_down)
+    dev = _one_device(x, topk_ids, topk_weights, out, *held)
+    if topk_ids.dtype != torch.int64 or topk_weights.dtype != x.dtype or \
+            tuple(topk_ids.shape) != (T, k) or tuple(topk_weights.shape) != (T, k):
+        raise RuntimeError("block_forward_routed: topk_ids must be int64 [T, k], topk_weights "
+                           "[T, k] in the hidden dtype")
+    if out is None:
+        out = torch.empty_like(x)
+    if T == 0:
+        return out
+    lib = load()
+    dt = dtype_code(x.dtype)
+    dense = (None, None) if w4 else (ptr(w_gate_up), ptr(w_down))
+    quant = (ctypes.byref(_w4(w_gate_up)), ctypes.byref(_w4(w_down))) if w4 else (None, None)
+    with _on(dev):
+        nbytes = lib.prism_moe_block_workspace_size(T, H, I, E, k, dt)
+        ws = _routed_workspace(dev, nbytes)
+        check(lib.prism_moe_block_forward_routed(
+            ptr(x), ptr(topk_ids), ptr(topk_weights), dt, T, H, I, E, k, *dense, *quant, ptr(out),
+            ptr(ws), ws.numel(), stream_of(dev),
+            ctypes.byref(epilogue) if epilogue is not None else None),
+            "prism_moe_block_forward_routed")
     return out
 
 

@@ -113,6 +113,100 @@ BlockLayout block_layout(int64_t T, int64_t H, int64_t I, int E, int k, int dtyp
   return L;
 }
 
+// 4-bit weights [n, k] of one matrix (or a stack): what the kernels need of them.
+int check_w4(const char* what, const prism_moe_w4* w, int64_t k, int64_t n) {
+  PRISM_CHECK_ARG(w && w->qweight && w->scales, "%s: null 4-bit weight", what);
+  PRISM_CHECK_ARG(w->group_size == 32 || w->group_size == 64 || w->group_size == 128,
+                  "%s: group_size %d is not 32, 64 or 128", what, w->group_size);
+  PRISM_CHECK_ARG(k % w->group_size == 0, "%s: %lld inputs are not a multiple of group_size %d",
+                  what, static_cast<long long>(k), w->group_size);
+  PRISM_CHECK_ARG(n % 8 == 0, "%s: %lld outputs are not a multiple of 8", what,
+                  static_cast<long long>(n));
+  PRISM_CHECK_ARG(k < (int64_t(1) << 30) && n < (int64_t(1) << 30), "%s: matrix too large", what);
+  PRISM_CHECK_ARG((reinterpret_cast<uintptr_t>(w->qweight) | reinterpret_cast<uintptr_t>(w->scales) |
+                   reinterpret_cast<uintptr_t>(w->zeros)) % 16 == 0,
+                  "%s: 4-bit weights must be 16-byte aligned", what);
+  return PRISM_MOE_OK;
+}
+
+size_t w4_scratch_bytes(int64_t rows, int64_t inter) {
+  return align_up(static_cast<size_t>(2 * rows * inter), 256);
+}
+
+// gate_up with SwiGLU into ``h`` (bf16: the next product's operand type), then down.
+int expert_swiglu_w4(const void* xs, int64_t rows, int64_t H, int64_t I,
+                     const int32_t* seg_offsets, const int32_t* seg_expert, int nseg, int El,
+                     const prism_moe_w4& gu, const prism_moe_w4& dn, void* y, void* h, int* err,
+                     cudaStream_t st) {
+  W4Problem p;
+  p.x = xs;
+  p.rows_cap = rows;
+  p.K = H;
+  p.n_out = I;
+  p.swiglu = true;
+  p.seg_offsets = seg_offsets;
+  p.seg_expert = seg_expert;
+  p.nseg = nseg;
+  p.num_mats = El;
+  p.w = gu;
+  p.out = h;
+  p.err = err;
+  record_stage(3, st);
+  if (int r = w4_product(p, st)) return r;
+  record_stage(4, st);
+  p.x = h;
+  p.K = I;
+  p.n_out = H;
+  p.swiglu = false;
+  p.w = dn;
+  p.out = y;
+  const int r = w4_product(p, st);
+  record_stage(5, st);
+  return r;
+}
+
+// Plan, gather, experts (dense, or 4-bit where ``q_gu`` is given) and combine for routed tokens.
+int block_after_router(const void* x, const int64_t* ids, const void* w, int dtype, int64_t T,
+                       int64_t H, int64_t I, int E, int k, const void* w_gate_up,
+                       const void* w_down, const prism_moe_w4* q_gu, const prism_moe_w4* q_dn,
+                       void* out, char* ws, const BlockLayout& L,
+                       const prism_moe_norm_epilogue* epilogue, cudaStream_t st) {
+  int* err = reinterpret_cast<int*>(ws + L.err);
+  int32_t* counts = reinterpret_cast<int32_t*>(ws + L.counts);
+  int32_t* offsets = reinterpret_cast<int32_t*>(ws + L.offsets);
+  int32_t* entry_row = reinterpret_cast<int32_t*>(ws + L.entry_row);
+  void* xs = ws + L.xs;
+  void* h = ws + L.h;
+  void* y = ws + L.y;
+  const int64_t N = T * k;
+  record_stage(1, st);
+  int r = build_plan(ids, T, k, E, 1, nullptr, nullptr, nullptr, counts, offsets, entry_row,
+                     nullptr, ws + L.plan, L.plan_bytes, st, err);
+  if (r) return r;
+  record_stage(2, st);
+  r = permute_rows(x, T, H * elem_size(dtype), k, entry_row, xs, st);
+  if (r) return r;
+  if (q_gu)
+    r = expert_swiglu_w4(xs, N, H, I, offsets, nullptr, E, E, *q_gu, *q_dn, y, h, err, st);
+  else if (dtype == PRISM_MOE_BF16)
+    r = expert_swiglu_bf16(xs, N, H, I, offsets, nullptr, E, E, w_gate_up, w_down, y, h, err, st);
+  else
+    r = expert_swiglu_f32(static_cast<const float*>(xs), N, H, I, offsets, nullptr, E, E,
+                          static_cast<const float*>(w_gate_up), static_cast<const float*>(w_down),
+                          static_cast<float*>(y), static_cast<float*>(h), st);
+  if (r) return r;
+  CombineSource src{};
+  if (epilogue) {
+    src.residual = epilogue->residual;
+    src.norm_weight = epilogue->norm_weight;
+    src.residual_out = epilogue->residual_out;
+    src.eps = epilogue->eps;
+  }
+  r = combine(y, dtype, entry_row, w, T, k, H, out, st, &src);
+  record_stage(6, st);
+  return r;
+}
+
 }  // namespace
 }  // namespace prism
 
@@ -138,6 +232,39 @@ int prism_moe_route_topk(const void* logits, int dtype, int64_t num_tokens, int3
   if (int r = check_device()) return r;
   return route_topk(logits, dtype, num_tokens, num_experts, top_k, renorm, topk_ids, topk_weights,
                     expert_counts, static_cast<cudaStream_t>(stream));
+}
+
+int prism_moe_route_scored(const void* logits, int dtype, int64_t num_tokens, int32_t num_experts,
+                           int32_t top_k, const prism_moe_router* router, int64_t* topk_ids,
+                           void* topk_weights, int weights_dtype, int32_t* expert_counts,
+                           void* stream) {
+  PRISM_CHECK_ARG(dtype_ok(dtype) && dtype_ok(weights_dtype), "route_scored: unknown dtype %d / %d",
+                  dtype, weights_dtype);
+  PRISM_CHECK_ARG(num_tokens >= 0, "route_scored: negative num_tokens");
+  PRISM_CHECK_ARG(router != nullptr, "route_scored: null router");
+  PRISM_CHECK_ARG(num_experts >= 1 && num_experts <= 1024,
+                  "route_scored: num_experts %d outside [1, 1024]", num_experts);
+  PRISM_CHECK_ARG(router->scoring == PRISM_MOE_SCORE_SOFTMAX ||
+                      router->scoring == PRISM_MOE_SCORE_SIGMOID,
+                  "route_scored: unknown scoring %d", router->scoring);
+  PRISM_CHECK_ARG(router->group_score == PRISM_MOE_GROUP_MAX ||
+                      router->group_score == PRISM_MOE_GROUP_TOP2,
+                  "route_scored: unknown group_score %d", router->group_score);
+  const int groups = router->num_groups, keep = router->topk_groups;
+  PRISM_CHECK_ARG(groups >= 1 && groups <= 32 && num_experts % groups == 0,
+                  "route_scored: num_groups %d outside [1, 32] or no divisor of %d experts", groups,
+                  num_experts);
+  PRISM_CHECK_ARG(keep >= 1 && keep <= groups, "route_scored: topk_groups %d outside [1, %d]", keep,
+                  groups);
+  PRISM_CHECK_ARG(top_k >= 1 && top_k <= 32 && top_k <= keep * (num_experts / groups),
+                  "route_scored: top_k %d outside [1, min(32, %d experts of %d groups)]", top_k,
+                  keep * (num_experts / groups), keep);
+  PRISM_CHECK_ARG(num_tokens == 0 || (logits && topk_ids && topk_weights),
+                  "route_scored: null pointer");
+  if (int r = check_device()) return r;
+  return route_scored(logits, dtype, num_tokens, num_experts, top_k, *router, topk_ids,
+                      topk_weights, weights_dtype, expert_counts,
+                      static_cast<cudaStream_t>(stream));
 }
 
 size_t prism_moe_dispatch_workspace_size(int64_t num_tokens, int32_t top_k, int32_t num_experts,
@@ -207,6 +334,58 @@ int prism_moe_expert_swiglu(const void* x_sorted, int dtype, int64_t rows_capaci
                            static_cast<float*>(y), static_cast<float*>(workspace), st);
 }
 
+int prism_moe_linear_w4(const void* x, int64_t rows, int64_t in_features, int64_t out_features,
+                        const prism_moe_w4* weight, void* y, void* stream) {
+  PRISM_CHECK_ARG(rows >= 0 && in_features >= 1 && out_features >= 1, "linear_w4: bad shape");
+  PRISM_CHECK_ARG(rows < (int64_t(1) << 31), "linear_w4: too many rows");
+  if (int r = check_w4("linear_w4", weight, in_features, out_features)) return r;
+  PRISM_CHECK_ARG(rows == 0 || (x && y), "linear_w4: null pointer");
+  PRISM_CHECK_ARG((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) % 16 == 0,
+                  "linear_w4: buffers must be 16-byte aligned");
+  if (int r = check_device()) return r;
+  if (rows == 0) return PRISM_MOE_OK;
+  W4Problem p;
+  p.x = x;
+  p.rows_cap = rows;
+  p.K = in_features;
+  p.n_out = out_features;
+  p.w = *weight;
+  p.out = y;
+  return w4_product(p, static_cast<cudaStream_t>(stream));
+}
+
+size_t prism_moe_expert_w4_workspace_size(int64_t rows_capacity, int64_t inter) {
+  if (rows_capacity < 0 || inter < 1) return 0;
+  return w4_scratch_bytes(rows_capacity, inter);
+}
+
+int prism_moe_expert_swiglu_w4(const void* x_sorted, int64_t rows_capacity, int64_t hidden,
+                               int64_t inter, const int32_t* seg_offsets,
+                               const int32_t* seg_expert, int32_t num_segments,
+                               int32_t num_local_experts, const prism_moe_w4* w_gate_up,
+                               const prism_moe_w4* w_down, void* y, void* workspace,
+                               size_t workspace_bytes, int* device_error, void* stream) {
+  PRISM_CHECK_ARG(rows_capacity >= 0 && hidden >= 1 && inter >= 1, "expert_swiglu_w4: bad shape");
+  PRISM_CHECK_ARG(rows_capacity < (int64_t(1) << 31), "expert_swiglu_w4: rows_capacity too large");
+  PRISM_CHECK_ARG(num_segments >= 1 && num_segments <= kMaxW4Segments,
+                  "expert_swiglu_w4: segments %d outside [1, %d]", num_segments, kMaxW4Segments);
+  PRISM_CHECK_ARG(num_local_experts >= 1, "expert_swiglu_w4: no experts");
+  if (int r = check_w4("expert_swiglu_w4", w_gate_up, hidden, 2 * inter)) return r;
+  if (int r = check_w4("expert_swiglu_w4", w_down, inter, hidden)) return r;
+  PRISM_CHECK_ARG(workspace_bytes >= w4_scratch_bytes(rows_capacity, inter),
+                  "expert_swiglu_w4: workspace too small");
+  PRISM_CHECK_ARG(rows_capacity == 0 || (x_sorted && seg_offsets && y && workspace),
+                  "expert_swiglu_w4: null pointer");
+  PRISM_CHECK_ARG((reinterpret_cast<uintptr_t>(x_sorted) | reinterpret_cast<uintptr_t>(y) |
+                   reinterpret_cast<uintptr_t>(workspace)) % 16 == 0,
+                  "expert_swiglu_w4: buffers must be 16-byte aligned");
+  if (int r = check_device()) return r;
+  if (rows_capacity == 0) return PRISM_MOE_OK;
+  return expert_swiglu_w4(x_sorted, rows_capacity, hidden, inter, seg_offsets, seg_expert,
+                          num_segments, num_local_experts, *w_gate_up, *w_down, y, workspace,
+                          device_error, static_cast<cudaStream_t>(stream));
+}
+
 int prism_moe_combine(const void* expert_out, int dtype, const int32_t* entry_row,
                       const void* topk_weights, int64_t num_tokens, int32_t top_k, int64_t hidden,
                       void* out, void* stream) {
@@ -252,45 +431,52 @@ int prism_moe_block_forward_norm(const void* x, const void* router_logits, int d
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (num_tokens == 0) return PRISM_MOE_OK;
   char* ws = static_cast<char*>(workspace);
-  int* err = reinterpret_cast<int*>(ws + L.err);
   int64_t* ids = topk_ids ? topk_ids : reinterpret_cast<int64_t*>(ws + L.ids);
   void* w = topk_weights ? topk_weights : static_cast<void*>(ws + L.w);
-  int32_t* counts = reinterpret_cast<int32_t*>(ws + L.counts);
-  int32_t* offsets = reinterpret_cast<int32_t*>(ws + L.offsets);
-  int32_t* entry_row = reinterpret_cast<int32_t*>(ws + L.entry_row);
-  void* xs = ws + L.xs;
-  void* h = ws + L.h;
-  void* y = ws + L.y;
-  const int64_t N = num_tokens * top_k;
   record_stage(0, st);
   int r = route_topk(router_logits, dtype, num_tokens, num_experts, top_k, renorm, ids, w, nullptr, st);
   if (r) return r;
-  record_stage(1, st);
-  r = build_plan(ids, num_tokens, top_k, num_experts, 1, nullptr, nullptr, nullptr, counts, offsets,
-                 entry_row, nullptr, ws + L.plan, L.plan_bytes, st, err);
-  if (r) return r;
-  record_stage(2, st);
-  r = permute_rows(x, num_tokens, hidden * elem_size(dtype), top_k, entry_row, xs, st);
-  if (r) return r;
-  if (dtype == PRISM_MOE_BF16)
-    r = expert_swiglu_bf16(xs, N, hidden, inter, offsets, nullptr, num_experts, num_experts,
-                           w_gate_up, w_down, y, h, err, st);
-  else
-    r = expert_swiglu_f32(static_cast<const float*>(xs), N, hidden, inter, offsets, nullptr,
-                          num_experts, num_experts, static_cast<const float*>(w_gate_up),
-                          static_cast<const float*>(w_down), static_cast<float*>(y),
-                          static_cast<float*>(h), st);
-  if (r) return r;
-  CombineSource src{};
-  if (epilogue) {
-    src.residual = epilogue->residual;
-    src.norm_weight = epilogue->norm_weight;
-    src.residual_out = epilogue->residual_out;
-    src.eps = epilogue->eps;
+  return block_after_router(x, ids, w, dtype, num_tokens, hidden, inter, num_experts, top_k,
+                            w_gate_up, w_down, nullptr, nullptr, out, ws, L, epilogue, st);
+}
+
+int prism_moe_block_forward_routed(const void* x, const int64_t* topk_ids,
+                                   const void* topk_weights, int dtype, int64_t num_tokens,
+                                   int64_t hidden, int64_t inter, int32_t num_experts,
+                                   int32_t top_k, const void* w_gate_up, const void* w_down,
+                                   const prism_moe_w4* q_gate_up, const prism_moe_w4* q_down,
+                                   void* out, void* workspace, size_t workspace_bytes,
+                                   void* stream, const prism_moe_norm_epilogue* epilogue) {
+  PRISM_CHECK_ARG(dtype_ok(dtype), "block_forward_routed: unknown dtype %d", dtype);
+  PRISM_CHECK_ARG(num_tokens >= 0 && hidden >= 1 && inter >= 1, "block_forward_routed: bad shape");
+  PRISM_CHECK_ARG(num_experts >= 1 && num_experts <= 1024,
+                  "block_forward_routed: num_experts %d outside [1, 1024]", num_experts);
+  PRISM_CHECK_ARG(top_k >= 1 && top_k <= 32 && top_k <= num_experts,
+                  "block_forward_routed: top_k %d outside [1, min(num_experts, 32)]", top_k);
+  const bool w4 = q_gate_up || q_down;
+  PRISM_CHECK_ARG(w4 ? (!w_gate_up && !w_down) : (w_gate_up && w_down),
+                  "block_forward_routed: give either dense or 4-bit expert weights");
+  if (w4) {
+    PRISM_CHECK_ARG(dtype == PRISM_MOE_BF16,
+                    "block_forward_routed: 4-bit experts take bf16 activations");
+    if (int r = check_w4("block_forward_routed", q_gate_up, hidden, 2 * inter)) return r;
+    if (int r = check_w4("block_forward_routed", q_down, inter, hidden)) return r;
   }
-  r = combine(y, dtype, entry_row, w, num_tokens, top_k, hidden, out, st, &src);
-  record_stage(6, st);
-  return r;
+  const BlockLayout L = block_layout(num_tokens, hidden, inter, num_experts, top_k, dtype);
+  PRISM_CHECK_ARG(workspace && workspace_bytes >= L.total,
+                  "block_forward_routed: workspace too small (%zu < %zu)", workspace_bytes, L.total);
+  PRISM_CHECK_ARG(num_tokens == 0 || (x && topk_ids && topk_weights && out),
+                  "block_forward_routed: null pointer");
+  PRISM_CHECK_ARG(!epilogue || (epilogue->residual && epilogue->norm_weight &&
+                                epilogue->residual_out && epilogue->eps >= 0.f),
+                  "block_forward_routed: incomplete norm epilogue");
+  if (int r = check_device()) return r;
+  if (num_tokens == 0) return PRISM_MOE_OK;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  record_stage(0, st);
+  return block_after_router(x, topk_ids, topk_weights, dtype, num_tokens, hidden, inter,
+                            num_experts, top_k, w_gate_up, w_down, q_gate_up, q_down, out,
+                            static_cast<char*>(workspace), L, epilogue, st);
 }
 
 int prism_moe_block_forward(const void* x, const void* router_logits, int dtype,

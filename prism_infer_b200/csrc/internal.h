@@ -6,6 +6,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "../../include/prism_moe.h"
+
 namespace prism {
 
 // State of one expert-parallel step, kept at a fixed offset (kEpStepOffset) of the EP workspace.
@@ -84,6 +86,29 @@ struct GemmDispatch {
 // route.cu
 int route_topk(const void* logits, int dtype, int64_t T, int E, int k, int renorm, int64_t* ids,
                void* w, int32_t* counts, cudaStream_t st);
+
+// route_scored.cu
+int route_scored(const void* logits, int dtype, int64_t T, int E, int k,
+                 const prism_moe_router& r, int64_t* ids, void* w, int w_dtype, int32_t* counts,
+                 cudaStream_t st);
+
+// w4_small.cu — out[r, n] = sum_k x[r, k] * W_e[n, k] over a segment table, W in 4 bits. With
+// ``swiglu`` the matrices are gate_up tiles of 2 * n_out rows and out = silu(gate) * up. Rows of no
+// segment are left as they are; a segment whose expert id lies outside [0, num_mats) is skipped and
+// recorded in ``err``. ``seg_offsets`` NULL: one segment of rows_cap rows.
+struct W4Problem {
+  const void* x = nullptr;        // [rows_cap, K] bf16
+  int64_t rows_cap = 0, K = 0, n_out = 0;
+  bool swiglu = false;
+  const int32_t* seg_offsets = nullptr;
+  const int32_t* seg_expert = nullptr;
+  int nseg = 1, num_mats = 1;
+  prism_moe_w4 w{};
+  void* out = nullptr;            // [rows_cap, n_out] bf16
+  int* err = nullptr;
+};
+constexpr int kMaxW4Segments = 2048;   // the kernels keep the segments' prefix in shared memory
+int w4_product(const W4Problem& pr, cudaStream_t st);
 
 // dispatch.cu — row_entry (row -> flat entry) is an internal output, NULL when not wanted.
 // Entries whose expert id lies outside [0, E) are left out of every output (entry_row = -1)

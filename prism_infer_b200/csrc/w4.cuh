@@ -1,0 +1,114 @@
+// 4-bit weights: the layout both product kernels read, and its decoding.
+//
+// A matrix [N, K] is held in tiles of 16 rows by 128 inputs, row tiles outermost:
+//   qweight [N/16][ceil(K/128)][16 rows][64 bytes]      scales, zeros [N/16][ceil(K/128)][16][128/G]
+// A row's 64 bytes are 16 words of 8 codes; the word at 4 t + j (t, j < 4) holds inputs
+// 32 j + 8 t .. + 7, nibbles from the low end: inputs 0 2 4 6 1 3 5 7 of the eight. So a 16-byte load
+// of quarter t gives, in word j, the 8 consecutive inputs that belong to group (32 j) / G, and
+// (word >> 4 i) & 0x000f000f is the pair of inputs (2 i, 2 i + 1) in the two halves of a register.
+// gate_up matrices alternate 8 gate rows and 8 up rows, so a tile holds both factors of 8 outputs.
+#pragma once
+#include "common.cuh"
+#include "segments.cuh"
+
+namespace prism {
+
+__device__ __forceinline__ uint4 load_stream(const uint8_t* p) {   // read once: not kept in L1
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int j) {
+  return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w;
+}
+
+// bf16 pair (code - zero) of inputs (2 i, 2 i + 1); ``zero`` holds 128 + zero twice. Both the value
+// 128 + code (128 .. 143, 7 fraction bits suffice) and the difference are exact.
+__device__ __forceinline__ uint32_t code_pair(uint32_t word, int i, uint32_t zero) {
+  const uint32_t c = ((word >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+  uint32_t d;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(c), "r"(zero));
+  return d;
+}
+
+// The PG scales of one row and chunk, widened to fp32 (exact).
+template <int PG>
+__device__ __forceinline__ void load_scales(const uint16_t* p, float (&s)[PG]) {
+  if constexpr (PG == 1) {
+    s[0] = bf16_bits_to_float(__ldg(p));
+  } else if constexpr (PG == 2) {
+    const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(p));
+    s[0] = __uint_as_float(v << 16);
+    s[1] = __uint_as_float(v & 0xffff0000u);
+  } else {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+    s[0] = __uint_as_float(v.x << 16);
+    s[1] = __uint_as_float(v.x & 0xffff0000u);
+    s[2] = __uint_as_float(v.y << 16);
+    s[3] = __uint_as_float(v.y & 0xffff0000u);
+  }
+}
+
+// 128 + zero as a bf16 pair for each of the PG groups; 8 without zero points.
+template <int PG, bool kZeros>
+__device__ __forceinline__ void load_zeros(const uint8_t* z, int64_t at, uint32_t (&out)[PG]) {
+  if constexpr (!kZeros) {
+#pragma unroll
+    for (int i = 0; i < PG; ++i) out[i] = 0x43084308u;
+  } else {
+    uint32_t v;
+    if constexpr (PG == 1)
+      v = __ldg(z + at);
+    else if constexpr (PG == 2)
+      v = __ldg(reinterpret_cast<const uint16_t*>(z + at));
+    else
+      v = __ldg(reinterpret_cast<const uint32_t*>(z + at));
+#pragma unroll
+    for (int i = 0; i < PG; ++i)
+      out[i] = (((v >> (8 * i)) & 0xfu) * 0x00010001u) | 0x43004300u;
+  }
+}
+
+// silu(g) * u in fp32.
+__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.f + expf(-g)) * u; }
+
+struct RowSpan {
+  int64_t begin, end;
+};
+
+// Rows of segment s, kept inside [0, rows_cap) (no table: one segment of every row).
+__device__ __forceinline__ RowSpan segment_rows(const int32_t* seg_offsets, int s,
+                                                int64_t rows_cap) {
+  if (!seg_offsets) return {0, rows_cap};
+  const int64_t b = max(seg_offsets[s], 0);
+  return {b, min(static_cast<int64_t>(seg_offsets[s + 1]), rows_cap)};
+}
+
+// Warp-cooperative: prefix[s] = row blocks (of ``bm`` rows) before segment s, prefix[nseg] = all.
+__device__ __forceinline__ void build_row_blocks(const int32_t* seg_offsets, int nseg,
+                                                 int64_t rows_cap, int bm, int32_t* prefix) {
+  const int lane = threadIdx.x & 31;
+  int32_t carry = 0;
+  for (int base = 0; base < nseg; base += 32) {
+    const int s = base + lane;
+    int32_t n = 0;
+    if (s < nseg) {
+      const RowSpan r = segment_rows(seg_offsets, s, rows_cap);
+      n = r.end > r.begin ? static_cast<int32_t>((r.end - r.begin + bm - 1) / bm) : 0;
+    }
+    int32_t incl = n;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int32_t y = __shfl_up_sync(0xffffffffu, incl, off);
+      if (lane >= off) incl += y;
+    }
+    if (s < nseg) prefix[s] = carry + incl - n;
+    carry += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  if (lane == 0) prefix[nseg] = carry;
+}
+
+}  // namespace prism

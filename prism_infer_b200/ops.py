@@ -28,6 +28,16 @@ Ops (shapes: T tokens, H hidden, E experts, k top-k, W expert-parallel ranks):
 * ``block_forward_norm`` / ``ep_forward_norm``: the two block ops with the decoder layer's next
   residual add + RMSNorm fused into the combine; extra arguments ``residual[T,H],
   norm_weight[H], eps``; they return ``(out, residual_out)``.
+* ``route_scored(logits[T,E], top_k, scoring, bias[E], num_groups, topk_groups, group_score, renorm,
+  scale, out_dtype) -> (topk_ids[T,k] int64, topk_weights[T,k])``: routing by softmax or sigmoid
+  scores with a selection bias and expert groups (no counterpart in the reference).
+* ``block_forward_routed(x, topk_ids, topk_weights, w_gate_up, w_down) -> out[T,H]``: the block after
+  a router of the caller's choice; ``block_forward_routed_norm`` with the norm fused.
+* 4-bit weights (``quant.W4Weight`` as its tensors ``q, scales, zeros`` and group size):
+  ``linear_w4(x[M,K], q, scales, zeros, out_features, group_size) -> y[M,N]``,
+  ``expert_swiglu_w4(x_sorted, seg_offsets, gate_up q/scales/zeros, down q/scales/zeros, inter,
+  gate_up group, down group, seg_expert) -> y``, ``block_forward_w4`` / ``block_forward_w4_norm``:
+  the routed block on such experts.
 """
 from __future__ import annotations
 
@@ -38,6 +48,7 @@ from torch import Tensor
 from torch.library import custom_op
 
 from prism_infer_b200 import capi
+from prism_infer_b200.quant import W4Weight
 
 _EP_BANKS: "weakref.WeakValueDictionary[int, object]" = weakref.WeakValueDictionary()
 
@@ -198,4 +209,122 @@ def ep_forward_norm(x: Tensor, router_logits: Tensor, w_gate_up: Tensor, w_down:
 
 @ep_forward_norm.register_fake
 def _(x, router_logits, w_gate_up, w_down, top_k, renorm, bank, residual, norm_weight, eps):
+    return torch.empty_like(x), torch.empty_like(x)
+
+
+# ---------------------------------------------------------------------------------- scored routing
+
+@custom_op("prism_moe::route_scored", mutates_args=())
+def route_scored(logits: Tensor, top_k: int, scoring: str, bias: Tensor | None, num_groups: int,
+                 topk_groups: int, group_score: str, renorm: bool, scale: float,
+                 out_dtype: torch.dtype | None) -> tuple[Tensor, Tensor]:
+    ids, w, _ = capi.route_scored(logits, top_k, scoring=scoring, bias=bias,
+                                  num_groups=num_groups, topk_groups=topk_groups,
+                                  group_score=group_score, renorm=renorm, scale=scale,
+                                  out_dtype=out_dtype)
+    return ids, w
+
+
+@route_scored.register_fake
+def _(logits, top_k, scoring, bias, num_groups, topk_groups, group_score, renorm, scale, out_dtype):
+    T = logits.shape[0]
+    return (logits.new_empty((T, top_k), dtype=torch.int64),
+            logits.new_empty((T, top_k), dtype=out_dtype or logits.dtype))
+
+
+@custom_op("prism_moe::block_forward_routed", mutates_args=())
+def block_forward_routed(x: Tensor, topk_ids: Tensor, topk_weights: Tensor, w_gate_up: Tensor,
+                         w_down: Tensor) -> Tensor:
+    return capi.block_forward_routed(x, topk_ids, topk_weights, w_gate_up, w_down)
+
+
+@block_forward_routed.register_fake
+def _(x, topk_ids, topk_weights, w_gate_up, w_down):
+    return torch.empty_like(x)
+
+
+@custom_op("prism_moe::block_forward_routed_norm", mutates_args=())
+def block_forward_routed_norm(x: Tensor, topk_ids: Tensor, topk_weights: Tensor,
+                              w_gate_up: Tensor, w_down: Tensor, residual: Tensor,
+                              norm_weight: Tensor, eps: float) -> tuple[Tensor, Tensor]:
+    return _routed_norm(x, topk_ids, topk_weights, w_gate_up, w_down, residual, norm_weight, eps)
+
+
+@block_forward_routed_norm.register_fake
+def _(x, topk_ids, topk_weights, w_gate_up, w_down, residual, norm_weight, eps):
+    return torch.empty_like(x), torch.empty_like(x)
+
+
+def _routed_norm(x, topk_ids, topk_weights, w_gate_up, w_down, residual, norm_weight, eps):
+    residual = residual.contiguous()
+    res_out = torch.empty_like(x)
+    epi = capi.norm_epilogue(residual, norm_weight, eps, res_out)
+    out = capi.block_forward_routed(x, topk_ids, topk_weights, w_gate_up, w_down, epilogue=epi)
+    return out, res_out
+
+
+# ---------------------------------------------------------------------------------- 4-bit weights
+
+def _experts_w4(hidden: int, inter: int, gu_q, gu_s, gu_z, gu_group, dn_q, dn_s, dn_z, dn_group):
+    return (W4Weight(gu_q, gu_s, gu_z, 2 * inter, hidden, gu_group, gate_up=True),
+            W4Weight(dn_q, dn_s, dn_z, hidden, inter, dn_group))
+
+
+@custom_op("prism_moe::linear_w4", mutates_args=())
+def linear_w4(x: Tensor, q: Tensor, scales: Tensor, zeros: Tensor | None, out_features: int,
+              group_size: int) -> Tensor:
+    return capi.linear_w4(x, W4Weight(q, scales, zeros, out_features, x.shape[1], group_size))
+
+
+@linear_w4.register_fake
+def _(x, q, scales, zeros, out_features, group_size):
+    return x.new_empty((x.shape[0], out_features))
+
+
+@custom_op("prism_moe::expert_swiglu_w4", mutates_args=())
+def expert_swiglu_w4(x_sorted: Tensor, seg_offsets: Tensor, gu_q: Tensor, gu_scales: Tensor,
+                     gu_zeros: Tensor | None, dn_q: Tensor, dn_scales: Tensor,
+                     dn_zeros: Tensor | None, inter: int, gu_group: int, dn_group: int,
+                     seg_expert: Tensor | None) -> Tensor:
+    gu, dn = _experts_w4(x_sorted.shape[1], inter, gu_q, gu_scales, gu_zeros, gu_group, dn_q,
+                         dn_scales, dn_zeros, dn_group)
+    return capi.expert_swiglu_w4(x_sorted, seg_offsets, gu, dn, seg_expert=seg_expert)
+
+
+@expert_swiglu_w4.register_fake
+def _(x_sorted, seg_offsets, gu_q, gu_scales, gu_zeros, dn_q, dn_scales, dn_zeros, inter, gu_group,
+      dn_group, seg_expert):
+    return torch.empty_like(x_sorted)
+
+
+@custom_op("prism_moe::block_forward_w4", mutates_args=())
+def block_forward_w4(x: Tensor, topk_ids: Tensor, topk_weights: Tensor, gu_q: Tensor,
+                     gu_scales: Tensor, gu_zeros: Tensor | None, dn_q: Tensor, dn_scales: Tensor,
+                     dn_zeros: Tensor | None, inter: int, gu_group: int,
+                     dn_group: int) -> Tensor:
+    gu, dn = _experts_w4(x.shape[1], inter, gu_q, gu_scales, gu_zeros, gu_group, dn_q, dn_scales,
+                         dn_zeros, dn_group)
+    return capi.block_forward_routed(x, topk_ids, topk_weights, gu, dn)
+
+
+@block_forward_w4.register_fake
+def _(x, topk_ids, topk_weights, gu_q, gu_scales, gu_zeros, dn_q, dn_scales, dn_zeros, inter,
+      gu_group, dn_group):
+    return torch.empty_like(x)
+
+
+@custom_op("prism_moe::block_forward_w4_norm", mutates_args=())
+def block_forward_w4_norm(x: Tensor, topk_ids: Tensor, topk_weights: Tensor, gu_q: Tensor,
+                          gu_scales: Tensor, gu_zeros: Tensor | None, dn_q: Tensor,
+                          dn_scales: Tensor, dn_zeros: Tensor | None, inter: int, gu_group: int,
+                          dn_group: int, residual: Tensor, norm_weight: Tensor,
+                          eps: float) -> tuple[Tensor, Tensor]:
+    gu, dn = _experts_w4(x.shape[1], inter, gu_q, gu_scales, gu_zeros, gu_group, dn_q, dn_scales,
+                         dn_zeros, dn_group)
+    return _routed_norm(x, topk_ids, topk_weights, gu, dn, residual, norm_weight, eps)
+
+
+@block_forward_w4_norm.register_fake
+def _(x, topk_ids, topk_weights, gu_q, gu_scales, gu_zeros, dn_q, dn_scales, dn_zeros, inter,
+      gu_group, dn_group, residual, norm_weight, eps):
     return torch.empty_like(x), torch.empty_like(x)
