@@ -109,6 +109,8 @@ struct W4Problem {
 };
 constexpr int kMaxW4Segments = 2048;   // the kernels keep the segments' prefix in shared memory
 int w4_product(const W4Problem& pr, cudaStream_t st);
+// w4_sm100.cu — the same for the segments of more than ``min_rows`` rows.
+int w4_product_large(const W4Problem& pr, int min_rows, cudaStream_t st);
 
 // dispatch.cu — row_entry (row -> flat entry) is an internal output, NULL when not wanted.
 // Entries whose expert id lies outside [0, E) are left out of every output (entry_row = -1)

@@ -88,8 +88,11 @@ __device__ __forceinline__ RowSpan segment_rows(const int32_t* seg_offsets, int 
 }
 
 // Warp-cooperative: prefix[s] = row blocks (of ``bm`` rows) before segment s, prefix[nseg] = all.
+// Only segments of more than ``min_rows`` and at most ``max_rows`` rows count.
 __device__ __forceinline__ void build_row_blocks(const int32_t* seg_offsets, int nseg,
-                                                 int64_t rows_cap, int bm, int32_t* prefix) {
+                                                 int64_t rows_cap, int bm, int32_t* prefix,
+                                                 int64_t min_rows = 0,
+                                                 int64_t max_rows = int64_t(1) << 31) {
   const int lane = threadIdx.x & 31;
   int32_t carry = 0;
   for (int base = 0; base < nseg; base += 32) {
@@ -97,7 +100,8 @@ __device__ __forceinline__ void build_row_blocks(const int32_t* seg_offsets, int
     int32_t n = 0;
     if (s < nseg) {
       const RowSpan r = segment_rows(seg_offsets, s, rows_cap);
-      n = r.end > r.begin ? static_cast<int32_t>((r.end - r.begin + bm - 1) / bm) : 0;
+      const int64_t len = r.end - r.begin;
+      n = len > min_rows && len <= max_rows ? static_cast<int32_t>((len + bm - 1) / bm) : 0;
     }
     int32_t incl = n;
 #pragma unroll

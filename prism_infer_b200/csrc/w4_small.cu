@@ -25,6 +25,7 @@ namespace prism {
 namespace {
 
 constexpr int kWarps = 8;
+constexpr int kSmallRows = 16;
 constexpr int kCh = 2;          // 128-input chunks a warp keeps in registers per pass
 constexpr int kColStride = 20;  // floats between the columns of a partial tile: no bank conflicts
 
@@ -43,6 +44,7 @@ struct SmallParams {
   const uint16_t* s;
   int kw, rw, rt, passes;    // input splits, row-tile splits, row tiles per item, input passes
   int blocks_n;              // ceil(tiles / rt)
+  int64_t max_rows;          // longer segments are the other kernel's
   int* err;
 };
 
@@ -67,7 +69,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) w4_small_kernel(const SmallPar
   const int nwarps = blockDim.x >> 5;
   const int tile_floats = 8 * NT * kColStride;
 
-  if (warp == 0) build_row_blocks(p.seg_offsets, p.nseg, p.rows_cap, 8 * NT, prefix);
+  if (warp == 0) build_row_blocks(p.seg_offsets, p.nseg, p.rows_cap, 8 * NT, prefix, 0, p.max_rows);
   __syncthreads();
   const int64_t total = static_cast<int64_t>(prefix[p.nseg]) * p.blocks_n;
 
@@ -254,7 +256,13 @@ int launch_zeros(const SmallParams& p, bool swiglu, int64_t u8, int64_t u16, cud
 }  // namespace
 
 int w4_product(const W4Problem& pr, cudaStream_t st) {
+  // Segments of at most kSmallRows rows run here, longer ones on the other kernel; the host does
+  // not know the segments' lengths, so a call whose rows could make both kinds launches both.
+  if (pr.rows_cap > kSmallRows)
+    if (int r = w4_product_large(pr, kSmallRows, st)) return r;
+  if (pr.nseg == 1 && pr.rows_cap > kSmallRows && !pr.seg_offsets) return PRISM_MOE_OK;
   SmallParams p{};
+  p.max_rows = kSmallRows;
   p.x = static_cast<const uint16_t*>(pr.x);
   p.ld_x = pr.K;
   p.K = static_cast<int>(pr.K);
@@ -273,7 +281,7 @@ int w4_product(const W4Problem& pr, cudaStream_t st) {
   p.err = pr.err;
   // most row blocks there can be, however the rows fall into segments
   const int64_t hit = std::min<int64_t>(pr.nseg, pr.rows_cap);
-  const int64_t u8 = hit + pr.rows_cap / 8, u16 = hit + pr.rows_cap / 16;
+  const int64_t u8 = std::min(hit + pr.rows_cap / 8, 2 * hit), u16 = hit;
   switch (pr.w.group_size) {
     case 32: return launch_zeros<32>(p, pr.swiglu, u8, u16, st);
     case 64: return launch_zeros<64>(p, pr.swiglu, u8, u16, st);
