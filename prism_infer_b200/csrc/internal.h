@@ -107,7 +107,7 @@ struct W4Problem {
   void* out = nullptr;            // [rows_cap, n_out] bf16
   int* err = nullptr;
 };
-constexpr int kMaxW4Segments = 2048;   // the kernels keep the segments' prefix in shared memory
+constexpr int kMaxW4Segments = 1024;   // the kernels keep the segments' prefix in shared memory
 int w4_product(const W4Problem& pr, cudaStream_t st);
 // w4_sm100.cu — the same for the segments of more than ``min_rows`` rows.
 int w4_product_large(const W4Problem& pr, int min_rows, cudaStream_t st);

@@ -34,17 +34,17 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t word, int i, uint32_t zer
   return d;
 }
 
-// The PG scales of one row and chunk, widened to fp32 (exact).
+// The PG scales of one row and chunk (global or shared memory), widened to fp32 (exact).
 template <int PG>
 __device__ __forceinline__ void load_scales(const uint16_t* p, float (&s)[PG]) {
   if constexpr (PG == 1) {
-    s[0] = bf16_bits_to_float(__ldg(p));
+    s[0] = bf16_bits_to_float(*p);
   } else if constexpr (PG == 2) {
-    const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(p));
+    const uint32_t v = *reinterpret_cast<const uint32_t*>(p);
     s[0] = __uint_as_float(v << 16);
     s[1] = __uint_as_float(v & 0xffff0000u);
   } else {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
     s[0] = __uint_as_float(v.x << 16);
     s[1] = __uint_as_float(v.x & 0xffff0000u);
     s[2] = __uint_as_float(v.y << 16);
@@ -61,11 +61,11 @@ __device__ __forceinline__ void load_zeros(const uint8_t* z, int64_t at, uint32_
   } else {
     uint32_t v;
     if constexpr (PG == 1)
-      v = __ldg(z + at);
+      v = z[at];
     else if constexpr (PG == 2)
-      v = __ldg(reinterpret_cast<const uint16_t*>(z + at));
+      v = *reinterpret_cast<const uint16_t*>(z + at);
     else
-      v = __ldg(reinterpret_cast<const uint32_t*>(z + at));
+      v = *reinterpret_cast<const uint32_t*>(z + at);
 #pragma unroll
     for (int i = 0; i < PG; ++i)
       out[i] = (((v >> (8 * i)) & 0xfu) * 0x00010001u) | 0x43004300u;

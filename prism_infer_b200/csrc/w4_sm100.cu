@@ -12,7 +12,10 @@
 // Warp roles (512 threads, one CTA per SM, persistent over a device-side tile list):
 //   warp 0        TMA of the activation rows (64 inputs x 64 rows per copy, 128-byte swizzle)
 //   warp 1        TMEM owner and MMA issuer
-//   warp 2        bulk copies of packed weights, 128 inputs of 8 row tiles (1 KB each) per stage
+//   warp 2        bulk copies of packed weights, 128 inputs of 8 row tiles (1 KB each) per slot, and
+//                 of their zero points
+//   warp 3        bulk copies of scales, 128 inputs of 8 row tiles per slot (their readers run up to
+//                 two chunks behind the decoders, so they have a ring of their own)
 //   warps 4-7     decode: 16 bytes (four words) per lane and row -> K-major, swizzled bf16 A tile
 //   warps 8-15    accumulate: two warps per TMEM lane quarter, each half of the columns; a lane owns
 //                 one weight row, so a group's scale is one register
@@ -40,9 +43,24 @@ constexpr int kNumStages = 4;
 constexpr int kPackStage = 8 * 1024;
 constexpr int kPackStages = 3;
 constexpr int kThreadsW4 = 512;
-constexpr size_t kBarOffset = static_cast<size_t>(kNumStages) * kStage + kPackStages * kPackStage;
-constexpr size_t kSmemW4 = 1024 + kBarOffset + 256 + kPrefixBytes;
-static_assert(kSmemW4 <= 232448, "shared memory budget");
+constexpr int kMaxScaleSlots = 8;
+constexpr size_t kPrefixW4 = ((kMaxW4Segments + 1) * 4 + 15) / 16 * 16;
+
+// Shared memory after the stages: packed slots, zero-point slots, scale slots, barriers, prefix.
+template <int G>
+struct Smem {
+  static constexpr int kPG = 128 / G;                 // groups per chunk
+  static constexpr int kZeroSlot = kRowsW * kPG;      // bytes
+  static constexpr int kScaleSlot = kRowsW * kPG * 2;
+  static constexpr int kScaleSlots = kPG == 4 ? 4 : kMaxScaleSlots;
+  static constexpr int kPacked = kNumStages * kStage;
+  static constexpr int kZeros = kPacked + kPackStages * kPackStage;
+  static constexpr int kScales = kZeros + kPackStages * kZeroSlot;
+  static constexpr int kBars = kScales + kScaleSlots * kScaleSlot;
+  static constexpr int kPrefix = kBars + 320;
+  static constexpr int kBytes = 1024 + kPrefix + static_cast<int>(kPrefixW4);
+  static_assert(kBytes <= 232448, "shared memory budget");
+};
 
 struct LargeParams {
   int num_kb, chunks, tiles, tiles_n;   // 64-input blocks, 128-input chunks, row tiles, M tiles
@@ -77,19 +95,29 @@ template <int N>
 __device__ __forceinline__ void reg_dealloc() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
-// tcgen05.wait::ld, naming the registers it makes readable.
-__device__ __forceinline__ void tmem_wait_ld16(uint32_t (&r)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
-                 "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]),
-                 "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
-}
 // (a0, a1) += s * (v0, v1)
 __device__ __forceinline__ void fma2(float2& a, uint32_t v0, uint32_t v1, uint64_t s2) {
   uint64_t v, c = *reinterpret_cast<uint64_t*>(&a);
   asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(v0), "r"(v1));
   asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(v), "l"(s2));
   a = *reinterpret_cast<float2*>(&c);
+}
+
+// acc[0 .. 32 kBatches) += s * (the accumulator's columns from ``taddr``), 32 columns per wait.
+template <int kBatches>
+__device__ __forceinline__ void add_scaled(float2 (&acc)[64], uint32_t taddr, float s) {
+  const float2 s2 = make_float2(s, s);
+  const uint64_t ss = *reinterpret_cast<const uint64_t*>(&s2);
+#pragma unroll
+  for (int b = 0; b < kBatches; ++b) {
+    uint32_t v[2][16];
+    tmem_ld16(taddr + b * 32, v[0]);
+    tmem_ld16(taddr + b * 32 + 16, v[1]);
+    tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      fma2(acc[b * 16 + i], v[i >> 3][2 * (i & 7)], v[i >> 3][2 * (i & 7) + 1], ss);
+  }
 }
 
 struct Tile {
@@ -118,21 +146,26 @@ __device__ __forceinline__ Tile tile_at(const LargeParams& p, const int32_t* pre
 template <int G, bool kZeros, bool kSwiGLU>
 __global__ void __launch_bounds__(kThreadsW4, 1)
     w4_large_kernel(const __grid_constant__ CUtensorMap tmap_x, const LargeParams p) {
-  constexpr int PG = 128 / G;
+  using S = Smem<G>;
+  constexpr int PG = S::kPG;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  uint8_t* packed = smem + kNumStages * kStage;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kBarOffset);
+  uint8_t* packed = smem + S::kPacked;
+  uint8_t* zeros = smem + S::kZeros;
+  uint8_t* scales = smem + S::kScales;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBars);
   uint64_t* empty = full + kNumStages;
   uint64_t* pk_full = empty + kNumStages;
   uint64_t* pk_empty = pk_full + kPackStages;
-  uint64_t* acc_full = pk_empty + kPackStages;
+  uint64_t* sc_full = pk_empty + kPackStages;
+  uint64_t* sc_empty = sc_full + kMaxScaleSlots;
+  uint64_t* acc_full = sc_empty + kMaxScaleSlots;
   uint64_t* acc_empty = acc_full + 2;
   uint64_t* drain = acc_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int32_t* prefix = reinterpret_cast<int32_t*>(smem + kBarOffset + 256);
+  int32_t* prefix = reinterpret_cast<int32_t*>(smem + S::kPrefix);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -143,6 +176,10 @@ __global__ void __launch_bounds__(kThreadsW4, 1)
     for (int s = 0; s < kPackStages; ++s) {
       mbar_init(&pk_full[s], 1);
       mbar_init(&pk_empty[s], 4);
+    }
+    for (int i = 0; i < S::kScaleSlots; ++i) {
+      mbar_init(&sc_full[i], 1);
+      mbar_init(&sc_empty[i], 8);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
@@ -260,18 +297,50 @@ __global__ void __launch_bounds__(kThreadsW4, 1)
           continue;
         }
         const int valid = min(8, p.tiles - t.mt * 8);
-        const uint8_t* src =
-            p.q + (static_cast<int64_t>(t.e) * p.tiles + t.mt * 8 + lane) * p.chunks * 1024;
+        const int64_t first = (static_cast<int64_t>(t.e) * p.tiles + t.mt * 8 + lane) * p.chunks;
         for (int c = 0; c < p.chunks; ++c) {
           ok = mbar_wait_bounded(&pk_empty[slot], phase ^ 1, abort, p.wait_ns);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(&pk_full[slot], valid * 1024);
+          constexpr int zb = kZeros ? 16 * PG : 0;   // zero points of one row tile
+          if (lane == 0) mbar_arrive_expect_tx(&pk_full[slot], valid * (1024 + zb));
+          __syncwarp();
+          if (lane < valid) {
+            bulk_load(packed + slot * kPackStage + lane * 1024, p.q + (first + c) * 1024, 1024,
+                      &pk_full[slot]);
+            if constexpr (kZeros)
+              bulk_load(zeros + slot * S::kZeroSlot + lane * zb, p.z + (first + c) * zb, zb,
+                        &pk_full[slot]);
+          }
+          if (++slot == kPackStages) {
+            slot = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      if (!ok && lane == 0) give_up();
+    } else if (warp == 3) {
+      // ---------------------------------------------------------------- scales
+      int slot = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      constexpr int bytes = 32 * PG;   // of one row tile and chunk
+      for (int64_t item = blockIdx.x; ok && item < total; item += gridDim.x) {
+        const Tile t = tile_at(p, prefix, item);
+        if (!usable(t)) continue;
+        const int valid = min(8, p.tiles - t.mt * 8);
+        const int64_t first = (static_cast<int64_t>(t.e) * p.tiles + t.mt * 8 + lane) * p.chunks;
+        for (int c = 0; c < p.chunks; ++c) {
+          ok = mbar_wait_bounded(&sc_empty[slot], phase ^ 1, abort, p.wait_ns);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(&sc_full[slot], valid * bytes);
           __syncwarp();
           if (lane < valid)
-            bulk_load(packed + slot * kPackStage + lane * 1024, src + static_cast<int64_t>(c) * 1024,
-                      1024, &pk_full[slot]);
-          if (++slot == kPackStages) {
+            bulk_load(scales + slot * S::kScaleSlot + lane * bytes,
+                      reinterpret_cast<const uint8_t*>(p.s) + (first + c) * bytes, bytes,
+                      &sc_full[slot]);
+          if (++slot == S::kScaleSlots) {
             slot = 0;
             phase ^= 1;
           }
@@ -290,19 +359,15 @@ __global__ void __launch_bounds__(kThreadsW4, 1)
     for (int64_t item = blockIdx.x; ok && item < total; item += gridDim.x) {
       const Tile t = tile_at(p, prefix, item);
       if (!usable(t)) continue;
-      const int64_t tile0 = static_cast<int64_t>(t.e) * p.tiles + t.mt * 8;
       for (int c = 0; ok && c < p.chunks; ++c) {
+        ok = mbar_wait_bounded(&pk_full[slot], pk_phase, abort, p.wait_ns);
+        if (!ok) break;
         // rows g and g + 8 of row tiles 2 w and 2 w + 1
         uint32_t zr[4][PG];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int rt = 2 * w + (r >> 1);
-          const bool there = t.mt * 8 + rt < p.tiles;
-          const int64_t at = (((tile0 + (there ? rt : 0)) * p.chunks + c) * 16 + g + 8 * (r & 1)) * PG;
-          load_zeros<PG, kZeros>(p.z, at, zr[r]);
-        }
-        ok = mbar_wait_bounded(&pk_full[slot], pk_phase, abort, p.wait_ns);
-        if (!ok) break;
+        for (int r = 0; r < 4; ++r)
+          load_zeros<PG, kZeros>(zeros + slot * S::kZeroSlot,
+                                 ((2 * w + (r >> 1)) * 16 + g + 8 * (r & 1)) * PG, zr[r]);
         uint4 v[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r)
@@ -357,56 +422,50 @@ __global__ void __launch_bounds__(kThreadsW4, 1)
     int buf = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
-    const int groups = G == 128 ? p.chunks : p.num_kb * (64 / (G == 128 ? 64 : G));
+    int slot = 0;
+    uint32_t sc_phase = 0;
+    const int groups = G == 128 ? p.chunks : p.num_kb * (G == 32 ? 2 : 1);
     for (int64_t item = blockIdx.x; ok && item < total; item += gridDim.x) {
       const Tile t = tile_at(p, prefix, item);
       if (!usable(t)) continue;
       const int left = (t.cols / 16 + 1) / 2 * 16;            // columns of side 0
       const int col0 = side ? left : 0, ncols = side ? t.cols - left : left;
       const int row = q * 32 + lane;                          // weight row in the tile
-      const int rt = t.mt * 8 + (row >> 4);
-      const bool there = rt < p.tiles;
-      const uint16_t* sp =
-          p.s + ((static_cast<int64_t>(t.e) * p.tiles + (there ? rt : 0)) * p.chunks * 16 + (row & 15)) * PG;
       float2 acc[64];
 #pragma unroll
       for (int i = 0; i < 64; ++i) acc[i] = make_float2(0.f, 0.f);
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + col0;
-      auto scale_of = [&](int gr) -> uint16_t {
-        return there && gr < groups ? __ldg(sp + static_cast<int64_t>(gr / PG) * 16 * PG + gr % PG) : 0;
-      };
-      uint16_t s0 = scale_of(0), s1 = scale_of(1), s2 = scale_of(2);
-      for (int gr = 0; gr < groups; ++gr) {
-        const float sc = bf16_bits_to_float(s0);
-        s0 = s1;
-        s1 = s2;
-        s2 = scale_of(gr + 3);
-        const float2 sc2 = make_float2(sc, sc);
-        const uint64_t ss = *reinterpret_cast<const uint64_t*>(&sc2);
-        if (!mbar_wait_bounded(&acc_full[buf], acc_phase, abort, p.wait_ns)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
+      for (int c = 0; ok && c < p.chunks; ++c) {
+        ok = mbar_wait_bounded(&sc_full[slot], sc_phase, abort, p.wait_ns);
+        if (!ok) break;
+        float sc[PG];
+        load_scales<PG>(reinterpret_cast<const uint16_t*>(scales + slot * S::kScaleSlot) + row * PG, sc);
         __syncwarp();
-        const uint32_t at = taddr + buf * kTok;
-        uint32_t v[2][16];
-        if (ncols > 0) tmem_ld16(at, v[0]);
-#pragma unroll
-        for (int piece = 0; piece < 8; ++piece) {
-          if (piece * 16 < ncols) {
-            tmem_wait_ld16(v[piece & 1]);
-            if (piece < 7 && piece * 16 + 16 < ncols) tmem_ld16(at + piece * 16 + 16, v[(piece + 1) & 1]);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              fma2(acc[piece * 8 + i], v[piece & 1][2 * i], v[piece & 1][2 * i + 1], ss);
-          }
+        if (lane == 0) mbar_arrive(&sc_empty[slot]);
+        if (++slot == S::kScaleSlots) {
+          slot = 0;
+          sc_phase ^= 1;
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_empty[buf]);
-        buf ^= 1;
-        acc_phase ^= buf == 0 ? 1u : 0u;
+#pragma unroll
+        for (int gr = 0; gr < PG; ++gr) {
+          if (c * PG + gr >= groups) break;
+          ok = mbar_wait_bounded(&acc_full[buf], acc_phase, abort, p.wait_ns);
+          if (!ok) break;
+          tc_fence_after();
+          __syncwarp();
+          const uint32_t at = taddr + buf * kTok;
+          // few columns, or all 128 of this side (those past ncols hold what an earlier tile left
+          // there and are never stored)
+          if (ncols > 32)
+            add_scaled<4>(acc, at, sc[gr]);
+          else if (ncols > 0)
+            add_scaled<1>(acc, at, sc[gr]);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acc_empty[buf]);
+          buf ^= 1;
+          acc_phase ^= buf == 0 ? 1u : 0u;
+        }
       }
       if (!ok) break;
       // ---- output: lanes are consecutive outputs of one activation row
@@ -459,9 +518,9 @@ __global__ void __launch_bounds__(kThreadsW4, 1)
 template <int G, bool kZeros, bool kSwiGLU>
 int launch_large(const CUtensorMap& map, const LargeParams& p, int grid, cudaStream_t st) {
   auto kern = w4_large_kernel<G, kZeros, kSwiGLU>;
-  if (int r = ensure_smem_attr(reinterpret_cast<const void*>(kern), static_cast<int>(kSmemW4)))
+  if (int r = ensure_smem_attr(reinterpret_cast<const void*>(kern), Smem<G>::kBytes))
     return r;
-  kern<<<grid, kThreadsW4, kSmemW4, st>>>(map, p);
+  kern<<<grid, kThreadsW4, Smem<G>::kBytes, st>>>(map, p);
   PRISM_LAUNCH_CHECK("w4_large_kernel launch");
   return PRISM_MOE_OK;
 }

@@ -224,7 +224,7 @@ int launch_small(SmallParams p, int64_t units, cudaStream_t st) {
   p.blocks_n = static_cast<int>(ceil_div(p.tiles, p.rt));
   const int bytes = static_cast<int>(sizeof(float)) *
                     ((p.nseg + 4) / 4 * 4 + p.kw * p.rt * 8 * NT * kColStride);
-  constexpr int kMaxBytes = 4 * ((kMaxSegments + 4) + 8 * 8 * 8 * NT * kColStride);
+  constexpr int kMaxBytes = 4 * ((kMaxW4Segments + 4) + 8 * 8 * 8 * NT * kColStride);
   if (int r = ensure_smem_attr(reinterpret_cast<const void*>(kern), kMaxBytes)) return r;
   const int64_t items = units * p.blocks_n;
   const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(items, 2 * sms)));
