@@ -10,7 +10,6 @@ layers/moe.py:69-100).
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import threading
 from pathlib import Path
@@ -145,9 +144,15 @@ def check(status: int, what: str) -> None:
 
 # ---------------------------------------------------------------------------------- torch glue
 
+_torch_module = None
+
+
 def _torch():
-    import torch
-    return torch
+    global _torch_module
+    if _torch_module is None:
+        import torch
+        _torch_module = torch
+    return _torch_module
 
 
 def dtype_code(dt) -> int:
@@ -193,21 +198,32 @@ def route_topk(logits, top_k: int, renorm: bool, with_counts: bool = False):
     return ids, w, counts
 
 
-def _one_device(*ts):
-    """The device all given CUDA tensors are on (contiguous, one device, or RuntimeError)."""
-    _need_cuda(*ts)
-    devs = {t.device for t in ts if t is not None}
-    if len(devs) != 1:
-        raise RuntimeError(f"tensors are on different devices: {sorted(map(str, devs))}")
-    return devs.pop()
+def _one_device(first, *others) -> int:
+    """Index of the device all given CUDA tensors are on (contiguous, or RuntimeError)."""
+    index = first.get_device()
+    for t in (first, *others):
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("prism MoE kernels run on CUDA tensors only (no CPU fallback)")
+        if not t.is_contiguous():
+            raise RuntimeError("prism MoE kernels need contiguous tensors")
+        if t.get_device() != index:
+            raise RuntimeError(f"tensors are on different devices: cuda:{index} and "
+                               f"cuda:{t.get_device()}")
+    return index
 
 
-def _on(device):
-    """Context that makes ``device`` current (kernels launch on the current device)."""
-    torch = _torch()
-    if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def _launch(index: int, what: str, fn, *args) -> None:
+    """``fn(*args, stream)`` with device ``index`` current, on its current torch stream."""
+    cuda = _torch().cuda
+    if cuda.current_device() == index:
+        status = fn(*args, cuda.current_stream().cuda_stream)
+    else:
+        with cuda.device(index):
+            status = fn(*args, cuda.current_stream().cuda_stream)
+    if status != OK:
+        check(status, what)
 
 
 def route_scored(logits, top_k: int, *, scoring: str = "softmax", bias=None, num_groups: int = 1,
@@ -228,19 +244,18 @@ def route_scored(logits, top_k: int, *, scoring: str = "softmax", bias=None, num
         raise RuntimeError("route_scored: logits must be [T, E]")
     dev = _one_device(logits, bias)
     T, E = logits.shape
-    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (E,)):
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (E,)):
         raise RuntimeError(f"route_scored: bias must be float32 [{E}]")
     out_dtype = logits.dtype if out_dtype is None else out_dtype
-    dt, wdt = dtype_code(logits.dtype), dtype_code(out_dtype)
-    ids = torch.empty(T, max(int(top_k), 0), dtype=torch.int64, device=dev)
-    w = torch.empty(T, max(int(top_k), 0), dtype=out_dtype, device=dev)
-    counts = torch.empty(E, dtype=torch.int32, device=dev) if with_counts else None
+    shape = (T, max(int(top_k), 0))
+    ids = logits.new_empty(shape, dtype=torch.int64)
+    w = logits.new_empty(shape, dtype=out_dtype)
+    counts = logits.new_empty((E,), dtype=torch.int32) if with_counts else None
     router = Router(SCORINGS[scoring], ptr(bias), num_groups, topk_groups,
-                    GROUP_SCORES[group_score], int(bool(renorm)), float(scale))
-    with _on(dev):
-        check(load().prism_moe_route_scored(ptr(logits), dt, T, E, top_k, ctypes.byref(router),
-                                            ptr(ids), ptr(w), wdt, ptr(counts), stream_of(dev)),
-              "prism_moe_route_scored")
+                    GROUP_SCORES[group_score], 1 if renorm else 0, scale)
+    _launch(dev, "prism_moe_route_scored", load().prism_moe_route_scored, logits.data_ptr(),
+            dtype_code(logits.dtype), T, E, top_k, ctypes.byref(router), ids.data_ptr(),
+            w.data_ptr(), dtype_code(out_dtype), ptr(counts))
     return ids, w, counts
 
 
@@ -333,13 +348,11 @@ def linear_w4(x, weight, out=None):
     dev = _one_device(x, weight.qweight, out)
     M, N = x.shape[0], weight.out_features
     if out is None:
-        out = torch.empty(M, N, dtype=x.dtype, device=dev)
+        out = x.new_empty((M, N))
     elif tuple(out.shape) != (M, N) or out.dtype != x.dtype:
         raise RuntimeError("linear_w4: out must be [M, N] in x's dtype")
-    with _on(dev):
-        check(load().prism_moe_linear_w4(ptr(x), M, weight.in_features, N,
-                                         ctypes.byref(_w4(weight)), ptr(out), stream_of(dev)),
-              "prism_moe_linear_w4")
+    _launch(dev, "prism_moe_linear_w4", load().prism_moe_linear_w4, x.data_ptr(), M,
+            weight.in_features, N, ctypes.byref(_w4(weight)), out.data_ptr())
     return out
 
 
@@ -381,12 +394,11 @@ def expert_swiglu_w4(x_sorted, seg_offsets, w_gate_up, w_down, seg_expert=None, 
         raise RuntimeError("expert_swiglu_w4: y must look like x_sorted")
     lib = load()
     ws_bytes = lib.prism_moe_expert_w4_workspace_size(R, I)
-    ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=dev)
-    with _on(dev):
-        check(lib.prism_moe_expert_swiglu_w4(
-            ptr(x_sorted), R, H, I, ptr(seg_offsets), ptr(seg_expert), nseg, El,
-            ctypes.byref(_w4(w_gate_up)), ctypes.byref(_w4(w_down)), ptr(y), ptr(ws), ws_bytes,
-            ptr(device_error), stream_of(dev)), "prism_moe_expert_swiglu_w4")
+    ws = x_sorted.new_empty((max(ws_bytes, 1),), dtype=torch.uint8)
+    _launch(dev, "prism_moe_expert_swiglu_w4", lib.prism_moe_expert_swiglu_w4,
+            x_sorted.data_ptr(), R, H, I, seg_offsets.data_ptr(), ptr(seg_expert), nseg, El,
+            ctypes.byref(_w4(w_gate_up)), ctypes.byref(_w4(w_down)), y.data_ptr(), ws.data_ptr(),
+            ws_bytes, ptr(device_error))
     return y
 
 
@@ -538,12 +550,12 @@ def block_forward_routed(x, topk_ids, topk_weights, w_gate_up, w_down, out=None,
     dt = dtype_code(x.dtype)
     dense = (None, None) if w4 else (ptr(w_gate_up), ptr(w_down))
     quant = (ctypes.byref(_w4(w_gate_up)), ctypes.byref(_w4(w_down))) if w4 else (None, None)
-    with _on(dev):
+    with torch.cuda.device(dev):
         nbytes = lib.prism_moe_block_workspace_size(T, H, I, E, k, dt)
-        ws = _routed_workspace(dev, nbytes)
+        ws = _routed_workspace(x.device, nbytes)
         check(lib.prism_moe_block_forward_routed(
             ptr(x), ptr(topk_ids), ptr(topk_weights), dt, T, H, I, E, k, *dense, *quant, ptr(out),
-            ptr(ws), ws.numel(), stream_of(dev),
+            ptr(ws), ws.numel(), stream_of(x.device),
             ctypes.byref(epilogue) if epilogue is not None else None),
             "prism_moe_block_forward_routed")
     return out

@@ -9,8 +9,16 @@
 // One warp per token, keys in registers. A group's experts are spread over its own L lanes
 // (L = 32 / next_pow2(groups)): lane g * L + j holds experts g * per + j + L * i, so a group's best
 // keys meet in log2(L) shuffles whatever the sizes, and one group is the plain 32-lane layout.
-// Keys are compared as order-preserving 64-bit integers (NaN above everything, as torch ranks it;
-// 0 = no candidate): three warp-wide integer reductions find the best key and its lowest index.
+// Keys are compared as order-preserving integers (NaN above everything, as torch ranks it; 0 = no
+// candidate); warp-wide integer reductions find the best key and its lowest index. Lanes of up to 8
+// experts sort theirs first, so that taking the winner is a shift.
+//
+// The choice is that of 64-bit keys, made in 32 bits where those decide it. Without a bias the keys
+// are the logits themselves (both scores increase with the logit), exactly; with one they are
+// fp32 scores + bias, whose error is bounded. Any two neighbours in the order of the k + 1 best (and
+// any two groups at the cut) that are closer than their errors, and not the same logit and bias,
+// send the row to choose_exact, which does the same on 64-bit keys; so do NaN, infinities and
+// scores that saturate. On normal logits with a random bias that is fewer than 1 row in 1000.
 #include "common.cuh"
 #include "internal.h"
 
@@ -46,6 +54,26 @@ __device__ __forceinline__ uint32_t warp_best(uint64_t key, uint32_t idx) {
   return __reduce_min_sync(kFull, hi == mh && lo == ml ? idx : 0xffffffffu);
 }
 
+__device__ __forceinline__ uint32_t order_key32(float v) {
+  if (isnan(v)) return ~0u;
+  const uint32_t b = __float_as_uint(v + 0.f);
+  return (b >> 31) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float key_value32(uint32_t k) {   // 0 (no candidate) reads as NaN
+  return k == ~0u ? __int_as_float(0x7fc00000) : __uint_as_float((k >> 31) ? (k & 0x7fffffffu) : ~k);
+}
+
+// Two largest of a group's lanes.
+template <typename Key>
+__device__ __forceinline__ void join_top2(Key& a, Key& b, int lanes) {
+  for (int off = lanes >> 1; off > 0; off >>= 1) {
+    const Key oa = __shfl_xor_sync(kFull, a, off), ob = __shfl_xor_sync(kFull, b, off);
+    const Key lo = oa < a ? oa : a, hb = ob > b ? ob : b;
+    a = oa > a ? oa : a;
+    b = lo > hb ? lo : hb;
+  }
+}
+
 struct ScoredParams {
   const void* logits;
   const float* bias;
@@ -59,11 +87,15 @@ struct ScoredParams {
   int32_t* counts;
 };
 
+struct Choice {
+  int id;        // lane j: the j-th expert
+  float logit;   // and its logit
+};
+
+// The choice from 64-bit keys (logits read again: rows come here rarely).
 template <bool kBf16, int EPT>
-__global__ void __launch_bounds__(32 * kScoredWarps) route_scored_kernel(const ScoredParams p) {
+__device__ __noinline__ Choice choose_exact(const ScoredParams& p, int64_t t) {
   const int lane = threadIdx.x & 31;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * kScoredWarps + (threadIdx.x >> 5);
-  if (t >= p.T) return;
   const int grp = lane / p.lanes, sub = lane % p.lanes;
   auto expert = [&](int i) { return grp * p.per + sub + p.lanes * i; };
   auto valid = [&](int i) { return grp < p.groups && sub + p.lanes * i < p.per; };
@@ -73,9 +105,7 @@ __global__ void __launch_bounds__(32 * kScoredWarps) route_scored_kernel(const S
 #pragma unroll
   for (int i = 0; i < EPT; ++i)
     l[i] = valid(i) ? load_logit<kBf16>(p.logits, t * p.E + expert(i)) : 0.f;
-
-  // scores in 64 bits: the choice compares values that can lie closer than 32 bits resolve
-  double top = 0.0, inv = 1.0;
+  double top = 0.0, sum = 1.0;
   if (!p.sigmoid) {
     float m = -__int_as_float(0x7f800000);
 #pragma unroll
@@ -86,25 +116,21 @@ __global__ void __launch_bounds__(32 * kScoredWarps) route_scored_kernel(const S
       m = (o > m || isnan(o)) ? o : m;
     }
     top = m;
-    double sum = 0.0;
+    sum = 0.0;
 #pragma unroll
     for (int i = 0; i < EPT; ++i)
       if (valid(i)) sum += exp(static_cast<double>(l[i]) - top);
     for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(kFull, sum, off);
-    inv = sum;
   }
-  auto score = [&](float v) {
-    return p.sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(v)))
-                     : exp(static_cast<double>(v) - top) / inv;
-  };
 #pragma unroll
   for (int i = 0; i < EPT; ++i) {
     key[i] = 0;
-    if (valid(i))
-      key[i] = order_key(score(l[i]) + (p.bias ? static_cast<double>(p.bias[expert(i)]) : 0.0));
+    if (valid(i)) {
+      const double s = p.sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(l[i])))
+                                 : exp(static_cast<double>(l[i]) - top) / sum;
+      key[i] = order_key(s + (p.bias ? static_cast<double>(p.bias[expert(i)]) : 0.0));
+    }
   }
-
-  // ---- groups: the keep best, equal scores by ascending group
   if (p.groups > 1) {
     uint64_t a = 0, b = 0;
 #pragma unroll
@@ -113,12 +139,7 @@ __global__ void __launch_bounds__(32 * kScoredWarps) route_scored_kernel(const S
       a = key[i] > a ? key[i] : a;
       b = lo > b ? lo : b;
     }
-    for (int off = p.lanes >> 1; off > 0; off >>= 1) {
-      const uint64_t oa = __shfl_xor_sync(kFull, a, off), ob = __shfl_xor_sync(kFull, b, off);
-      const uint64_t lo = oa < a ? oa : a, hb = ob > b ? ob : b;
-      a = oa > a ? oa : a;
-      b = lo > hb ? lo : hb;
-    }
+    join_top2(a, b, p.lanes);
     uint64_t gs = 0;
     if (grp < p.groups) gs = p.top2 && p.per > 1 ? order_key(key_value(a) + key_value(b)) : a;
     int rank = 0;
@@ -131,10 +152,7 @@ __global__ void __launch_bounds__(32 * kScoredWarps) route_scored_kernel(const S
       for (int i = 0; i < EPT; ++i) key[i] = 0;
     }
   }
-
-  // ---- the k largest keys
-  int my_i = 0;
-  double my_s = 0.0;
+  Choice mine{0, 0.f};
   for (int j = 0; j < p.k; ++j) {
     uint64_t best = 0;
     int at = 0;
@@ -144,9 +162,8 @@ __global__ void __launch_bounds__(32 * kScoredWarps) route_scored_kernel(const S
         best = key[i];
         at = i;
       }
-    const uint32_t mine = static_cast<uint32_t>(expert(at));
-    const uint32_t win = warp_best(best, best ? mine : 0xfffffffeu);
-    const bool owner = best != 0 && mine == win;
+    const uint32_t win = warp_best(best, best ? static_cast<uint32_t>(expert(at)) : 0xfffffffeu);
+    const bool owner = best != 0 && static_cast<uint32_t>(expert(at)) == win;
     float lv = 0.f;
 #pragma unroll
     for (int i = 0; i < EPT; ++i)
@@ -155,25 +172,226 @@ __global__ void __launch_bounds__(32 * kScoredWarps) route_scored_kernel(const S
         if (owner) key[i] = 0;
       }
     lv = __shfl_sync(kFull, lv, __ffs(__ballot_sync(kFull, owner)) - 1);
-    if (lane == j) {
-      my_i = static_cast<int>(win);
-      my_s = score(lv);
+    if (lane == j) mine = {static_cast<int>(win), lv};
+  }
+  return mine;
+}
+
+// Sort a lane's keys in descending order, equal keys by ascending index (odd-even transposition:
+// N rounds of neighbours; N is 2, 4 or 8).
+template <int N>
+__device__ __forceinline__ void sort_lane(uint32_t (&key)[N], int (&at)[N]) {
+#pragma unroll
+  for (int r = 0; r < N; ++r)
+#pragma unroll
+    for (int i = r & 1; i + 1 < N; i += 2)
+      if (key[i + 1] > key[i]) {   // neighbours never swap when equal: the order stays by index
+        const uint32_t k = key[i];
+        key[i] = key[i + 1];
+        key[i + 1] = k;
+        const int a = at[i];
+        at[i] = at[i + 1];
+        at[i + 1] = a;
+      }
+}
+
+template <bool kBf16, int EPT>
+__global__ void __launch_bounds__(32 * kScoredWarps) route_scored_kernel(const __grid_constant__ ScoredParams p) {
+  constexpr bool kSorted = EPT <= 8;
+  const int lane = threadIdx.x & 31;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * kScoredWarps + (threadIdx.x >> 5);
+  if (t >= p.T) return;
+  const int grp = lane / p.lanes, sub = lane % p.lanes;
+  const int first = grp * p.per + sub;
+  const int mine = grp < p.groups ? (p.per - sub + p.lanes - 1) / p.lanes : 0;   // this lane's experts
+
+  float l[EPT];
+#pragma unroll
+  for (int i = 0; i < EPT; ++i)
+    l[i] = i < mine ? load_logit<kBf16>(p.logits, t * p.E + first + p.lanes * i) : 0.f;
+  uint32_t key[EPT];
+  int at[EPT];
+  uint32_t top_key = 0;
+#pragma unroll
+  for (int i = 0; i < EPT; ++i) {
+    at[i] = i;
+    key[i] = i < mine ? order_key32(l[i]) : 0u;
+    top_key = max(top_key, key[i]);
+  }
+  const float top = key_value32(__reduce_max_sync(kFull, top_key));   // largest logit, or NaN
+  bool unsure = !(fabsf(top) <= 3.4028235e38f);
+
+  // ---- fp32 scores where they are needed: as keys with a bias, or for the sum of a softmax
+  const bool need_sum = !p.sigmoid && (p.bias || !p.renorm);
+  float sum = 1.f;
+  if (need_sum) {
+    float e[EPT];
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) e[i] = i < mine ? expf(l[i] - top) : 0.f;
+#pragma unroll
+    for (int w = EPT / 2; w > 0; w >>= 1)
+#pragma unroll
+      for (int i = 0; i < w; ++i) e[i] += e[i + w];
+    sum = e[0];
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(kFull, sum, off);
+  }
+  auto score = [&](float v) {
+    return p.sigmoid ? 1.f / (1.f + expf(-v)) : expf(v - top) / sum;
+  };
+  if (p.bias) {
+#pragma unroll
+    for (int i = 0; i < EPT; ++i)
+      if (i < mine) key[i] = order_key32(score(l[i]) + p.bias[first + p.lanes * i]);
+  }
+  // Error of any fp32 score of this row. Sigmoid: expf (2 ulp), a sum and a division, 2^-21 of the
+  // score. Softmax: expf, its argument (|l - top| 2^-24, but e^-x x < 0.4), a division and a sum
+  // whose 2^6 lane terms and 32 lanes meet in a tree (11 roundings): 2^-19 of the largest.
+  const float score_err = p.bias ? (p.sigmoid ? 0x1p-21f : 0x1p-19f) * score(top) : 0.f;
+  if constexpr (kSorted && EPT > 1) sort_lane(key, at);
+
+  // ---- groups: the keep best, equal scores by ascending group
+  if (p.groups > 1) {
+    uint32_t a = 0, b = 0;
+    if constexpr (kSorted) {
+      a = key[0];
+      if constexpr (EPT > 1) b = key[1];
+    } else {
+#pragma unroll
+      for (int i = 0; i < EPT; ++i) {
+        const uint32_t lo = min(key[i], a);
+        a = max(a, key[i]);
+        b = max(b, lo);
+      }
+    }
+    join_top2(a, b, p.lanes);
+    const bool two = p.top2 && p.per > 1;
+    const float va = key_value32(a), vb = two ? key_value32(b) : 0.f;
+    float gs = va, err = 0.f;
+    if (p.bias) {
+      gs = va + vb;
+      err = 2.f * score_err + 0x1p-22f * (fabsf(va) + fabsf(vb));
+    } else if (two) {   // keys are logits: their scores, up to the softmax's common factor
+      gs = p.sigmoid ? score(va) + score(vb) : expf(va - top) + expf(vb - top);
+      err = p.sigmoid ? 0x1p-21f * gs : 0x1p-20f;
+    }
+    int rank = 0;
+    for (int g = 0; g < p.groups; ++g) {
+      const float o = __shfl_sync(kFull, gs, g * p.lanes);
+      rank += (o > gs || (o == gs && g < grp)) ? 1 : 0;
+    }
+    const bool kept = grp < p.groups && rank < p.keep;
+    // certain where the worst that stays and the best that goes are further apart than their errors
+    float low = kept ? gs - err : __int_as_float(0x7f800000);
+    float high = grp < p.groups && !kept ? gs + err : -__int_as_float(0x7f800000);
+    for (int off = 16; off > 0; off >>= 1) {
+      low = fminf(low, __shfl_xor_sync(kFull, low, off));
+      high = fmaxf(high, __shfl_xor_sync(kFull, high, off));
+    }
+    const bool exact = !p.bias && !two;   // logits: equal ones are ties, distinct ones decided
+    unsure |= !(low > high || (exact && low == high)) || !(gs == gs);
+    if (exact)
+      unsure |= (low - high > 0.f && low - high < 0x1p-40f) ||
+                (p.sigmoid ? fabsf(low) > 16.f || fabsf(high) > 16.f : !(top - low <= 600.f));
+    if (!kept) {
+#pragma unroll
+      for (int i = 0; i < EPT; ++i) key[i] = 0;
     }
   }
 
-  if (p.renorm) {
-    double sum = lane < p.k ? my_s : 0.0;
-    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(kFull, sum, off);
-    my_s /= sum + 1e-20;
+  // ---- the k largest keys, and the next one to compare with
+  uint32_t my_key = 0, next_key = 0, next_id = 0;
+  Choice my{0, 0.f};
+  for (int j = 0; j <= p.k; ++j) {
+    uint32_t best = 0;
+    int pos = 0;
+    if constexpr (kSorted) {
+      best = key[0];
+      pos = at[0];
+    } else {
+#pragma unroll
+      for (int i = 0; i < EPT; ++i)
+        if (key[i] > best) {
+          best = key[i];
+          pos = i;
+        }
+    }
+    next_key = __reduce_max_sync(kFull, best);
+    const uint32_t id = static_cast<uint32_t>(first + p.lanes * pos);
+    next_id = __reduce_min_sync(kFull, best == next_key ? id : 0xffffffffu);
+    if (lane == j) {
+      my_key = next_key;
+      my.id = static_cast<int>(next_id);
+    }
+    if (best == next_key && id == next_id) {
+      if constexpr (kSorted) {
+#pragma unroll
+        for (int i = 0; i + 1 < EPT; ++i) {
+          key[i] = key[i + 1];
+          at[i] = at[i + 1];
+        }
+        key[EPT - 1] = 0;
+      } else {
+#pragma unroll
+        for (int i = 0; i < EPT; ++i)
+          if (i == pos) key[i] = 0;
+      }
+    }
+  }
+  if (lane >= p.k) {   // every other lane stands for the next one (key 0: there is none)
+    my_key = next_key;
+    my.id = static_cast<int>(next_id);
+  }
+  const bool have = my_key != 0;
+  if (have) my.logit = load_logit<kBf16>(p.logits, t * p.E + my.id);   // in the cache
+  const float v = key_value32(my_key), mb = have && p.bias ? p.bias[my.id] : 0.f;
+  float nv = __shfl_down_sync(kFull, v, 1), nl = __shfl_down_sync(kFull, my.logit, 1);
+  float nb = __shfl_down_sync(kFull, mb, 1);
+  if (p.k == 32 && lane == 31) {
+    nv = key_value32(next_key);
+    nl = next_key ? load_logit<kBf16>(p.logits, t * p.E + next_id) : 0.f;
+    nb = next_key && p.bias ? p.bias[next_id] : 0.f;
   }
   if (lane < p.k) {
-    const float w = static_cast<float>(my_s * static_cast<double>(p.scale));
-    p.ids[t * p.k + lane] = my_i;
+    const bool next = lane + 1 < p.k || next_key != 0;
+    if (p.bias) {
+      const float err = 2.f * score_err + 0x1p-22f * (fabsf(v) + fabsf(nv));
+      if (next) unsure |= !(v - nv > err) && !(my.logit == nl && mb == nb);
+      unsure |= !(fabsf(v) <= 3.4028235e38f);
+    } else {
+      // where 64-bit scores could merge distinct logits: next to 0 or 1, or next to each other
+      if (next) unsure |= v - nv > 0.f && v - nv < 0x1p-40f;
+      unsure |= p.sigmoid ? !(fabsf(v) <= 16.f) : !(top - v <= 600.f);
+    }
+  }
+  if (__any_sync(kFull, unsure)) my = choose_exact<kBf16, EPT>(p, t);
+
+  // ---- weights: scores of the chosen, the softmax's argument with the rounding of v - top put back
+  float s = 0.f;
+  if (lane < p.k) {
+    if (p.sigmoid) {
+      s = 1.f / (1.f + expf(-my.logit));
+    } else {
+      const float d = my.logit - top, z = d - my.logit;
+      const float lost = (my.logit - (d - z)) - (top + z);
+      const float e = expf(d);
+      s = (lost == lost ? fmaf(e, lost, e) : e) / sum;   // a logit of -inf: e is 0
+      // a NaN or infinite logit leaves no weight of its token a number, as in softmax itself
+      if (!(fabsf(top) <= 3.4028235e38f)) s = __int_as_float(0x7fc00000);
+    }
+  }
+  if (p.renorm) {
+    float total = s;
+    for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(kFull, total, off);
+    s /= total + 1e-20f;
+  }
+  if (lane < p.k) {
+    const float w = s * p.scale;
+    p.ids[t * p.k + lane] = my.id;
     if (p.w_bf16)
       reinterpret_cast<uint16_t*>(p.w)[t * p.k + lane] = float_to_bf16_bits(w);
     else
       reinterpret_cast<float*>(p.w)[t * p.k + lane] = w;
-    if (p.counts) atomicAdd(p.counts + my_i, 1);
+    if (p.counts) atomicAdd(p.counts + my.id, 1);
   }
 }
 

@@ -1,9 +1,9 @@
 """Scored routing on the GPU (``capi.route_scored`` / ``torch.ops.prism_moe.route_scored``) against a
 plain implementation in 64 bits: choices exactly, weights to the rounding of their type.
 
-Weights: the kernel's scores carry a relative error of at most 2^-20 (fp32 arithmetic: one
-exponential of 2 ulp, a division, a sum of up to 32 positive terms, each step at most 2^-23), far
-below the final rounding of bf16, 2^-8 at most; fp32 outputs are held to 2^-20.
+Weights, in fp32: expf is off by 2 ulp (2^-22), twice in a softmax; its sum of up to 1024 terms goes
+through 11 roundings, that of the chosen through 6, and there are three divisions and products: at
+most 2^-22 * 2 + 20 * 2^-24 < 2^-18 of the value, before the rounding to the output's type.
 """
 import pytest
 import torch
@@ -13,7 +13,7 @@ from oracle.scored_routing import route_scored_ref
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
-RTOL = {torch.float32: 2.0 ** -20, torch.bfloat16: 2.0 ** -8 + 2.0 ** -20}
+RTOL = {torch.float32: 2.0 ** -18, torch.bfloat16: 2.0 ** -8 + 2.0 ** -18}
 
 
 def check(logits, k, out_dtype=None, **kw):
