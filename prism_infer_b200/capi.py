@@ -215,13 +215,14 @@ def _one_device(first, *others) -> int:
 
 
 def _launch(index: int, what: str, fn, *args) -> None:
-    """``fn(*args, stream)`` with device ``index`` current, on its current torch stream."""
-    cuda = _torch().cuda
-    if cuda.current_device() == index:
-        status = fn(*args, cuda.current_stream().cuda_stream)
+    """``fn(*args, stream)`` with device ``index`` current, on its current torch stream (the raw
+    handle: a Stream object costs more host time than the launch)."""
+    torch = _torch()
+    if torch.cuda.current_device() == index:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with cuda.device(index):
-            status = fn(*args, cuda.current_stream().cuda_stream)
+        with torch.cuda.device(index):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if status != OK:
         check(status, what)
 

@@ -7,8 +7,8 @@
 //   w_j   = s[ids_j] / (sum_j s[ids_j] + 1e-20) * scale   (the division only with renorm)
 //
 // One warp per token, keys in registers. A group's experts are spread over its own L lanes
-// (L = 32 / next_pow2(groups)): lane g * L + j holds experts g * per + j + L * i, so a group's best
-// keys meet in log2(L) shuffles whatever the sizes, and one group is the plain 32-lane layout.
+// (L = 32 / next_pow2(groups)), consecutive ones on each, so a group's best keys meet in log2(L)
+// shuffles whatever the sizes, and a lane reads its logits in vectors.
 // Keys are compared as order-preserving integers (NaN above everything, as torch ranks it; 0 = no
 // candidate); warp-wide integer reductions find the best key and its lowest index. Lanes of up to 8
 // experts sort theirs first, so that taking the winner is a shift.
@@ -17,8 +17,9 @@
 // are the logits themselves (both scores increase with the logit), exactly; with one they are
 // fp32 scores + bias, whose error is bounded. Any two neighbours in the order of the k + 1 best (and
 // any two groups at the cut) that are closer than their errors, and not the same logit and bias,
-// send the row to choose_exact, which does the same on 64-bit keys; so do NaN, infinities and
-// scores that saturate. On normal logits with a random bias that is fewer than 1 row in 1000.
+// are looked at in 64 bits: sigmoid keys with a bias among a few more candidates, all else (NaN,
+// infinities and scores that saturate too) by choose_exact, on 64-bit keys of the whole row. On
+// normal logits with a random bias about 1 row in 500 looks again, and nearly none goes on.
 #include "common.cuh"
 #include "internal.h"
 
@@ -26,6 +27,7 @@ namespace prism {
 namespace {
 
 constexpr int kScoredWarps = 4;
+constexpr int kSpare = 4;   // candidates beyond the k that a close order looks at
 constexpr unsigned kFull = 0xffffffffu;
 
 template <bool kBf16>
@@ -55,9 +57,9 @@ __device__ __forceinline__ uint32_t warp_best(uint64_t key, uint32_t idx) {
 }
 
 __device__ __forceinline__ uint32_t order_key32(float v) {
-  if (isnan(v)) return ~0u;
-  const uint32_t b = __float_as_uint(v + 0.f);
-  return (b >> 31) ? ~b : (b | 0x80000000u);
+  // adding zero makes -0 +0 and every NaN the canonical one, 0x7fffffff, whose key is ~0
+  const uint32_t b = __float_as_uint(__fadd_rn(v, 0.f));
+  return b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float key_value32(uint32_t k) {   // 0 (no candidate) reads as NaN
   return k == ~0u ? __int_as_float(0x7fc00000) : __uint_as_float((k >> 31) ? (k & 0x7fffffffu) : ~k);
@@ -78,7 +80,8 @@ struct ScoredParams {
   const void* logits;
   const float* bias;
   int64_t T;
-  int E, k, groups, keep, per, lanes;   // per = E / groups; lanes per group
+  int E, k, groups, keep, per, lanes, each;   // per = E / groups; lanes per group; experts per lane
+  bool vec;   // a lane's logits and biases may be read in 16-byte vectors
   int sigmoid, top2, renorm;
   float scale;
   int64_t* ids;
@@ -86,6 +89,42 @@ struct ScoredParams {
   int w_bf16;
   int32_t* counts;
 };
+
+// A lane's ``mine`` consecutive values from element ``at`` on (0 beyond them).
+template <bool kBf16, int EPT>
+__device__ __forceinline__ void load_lane(const ScoredParams& p, const void* src, int64_t at,
+                                          int mine, float (&v)[EPT]) {
+  if constexpr (EPT >= 8 || (!kBf16 && EPT == 4)) {
+    if (p.vec && mine == EPT) {
+      if constexpr (kBf16) {
+        const uint4* q = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(src) + at);
+#pragma unroll
+        for (int i = 0; i < EPT / 8; ++i) {
+          const uint4 u = q[i];
+          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            v[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
+            v[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+          }
+        }
+      } else {
+        const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(src) + at);
+#pragma unroll
+        for (int i = 0; i < EPT / 4; ++i) {
+          const float4 u = q[i];
+          v[4 * i] = u.x;
+          v[4 * i + 1] = u.y;
+          v[4 * i + 2] = u.z;
+          v[4 * i + 3] = u.w;
+        }
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < EPT; ++i) v[i] = i < mine ? load_logit<kBf16>(src, at + i) : 0.f;
+}
 
 struct Choice {
   int id;        // lane j: the j-th expert
@@ -97,8 +136,8 @@ template <bool kBf16, int EPT>
 __device__ __noinline__ Choice choose_exact(const ScoredParams& p, int64_t t) {
   const int lane = threadIdx.x & 31;
   const int grp = lane / p.lanes, sub = lane % p.lanes;
-  auto expert = [&](int i) { return grp * p.per + sub + p.lanes * i; };
-  auto valid = [&](int i) { return grp < p.groups && sub + p.lanes * i < p.per; };
+  auto expert = [&](int i) { return grp * p.per + sub * p.each + i; };
+  auto valid = [&](int i) { return grp < p.groups && i < p.each && sub * p.each + i < p.per; };
 
   float l[EPT];
   uint64_t key[EPT];
@@ -202,13 +241,11 @@ __global__ void __launch_bounds__(32 * kScoredWarps) route_scored_kernel(const _
   const int64_t t = static_cast<int64_t>(blockIdx.x) * kScoredWarps + (threadIdx.x >> 5);
   if (t >= p.T) return;
   const int grp = lane / p.lanes, sub = lane % p.lanes;
-  const int first = grp * p.per + sub;
-  const int mine = grp < p.groups ? (p.per - sub + p.lanes - 1) / p.lanes : 0;   // this lane's experts
+  const int first = grp * p.per + sub * p.each;
+  const int mine = grp < p.groups ? max(0, min(p.each, p.per - sub * p.each)) : 0;   // this lane's experts
 
   float l[EPT];
-#pragma unroll
-  for (int i = 0; i < EPT; ++i)
-    l[i] = i < mine ? load_logit<kBf16>(p.logits, t * p.E + first + p.lanes * i) : 0.f;
+  load_lane<kBf16, EPT>(p, p.logits, t * p.E + first, mine, l);
   uint32_t key[EPT];
   int at[EPT];
   uint32_t top_key = 0;
@@ -236,17 +273,19 @@ __global__ void __launch_bounds__(32 * kScoredWarps) route_scored_kernel(const _
     for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(kFull, sum, off);
   }
   auto score = [&](float v) {
-    return p.sigmoid ? 1.f / (1.f + expf(-v)) : expf(v - top) / sum;
+    return p.sigmoid ? __fdividef(1.f, 1.f + expf(-v)) : __fdividef(expf(v - top), sum);
   };
   if (p.bias) {
+    float b[EPT];
+    load_lane<false, EPT>(p, p.bias, first, mine, b);
 #pragma unroll
     for (int i = 0; i < EPT; ++i)
-      if (i < mine) key[i] = order_key32(score(l[i]) + p.bias[first + p.lanes * i]);
+      if (i < mine) key[i] = order_key32(score(l[i]) + b[i]);
   }
-  // Error of any fp32 score of this row. Sigmoid: expf (2 ulp), a sum and a division, 2^-21 of the
-  // score. Softmax: expf, its argument (|l - top| 2^-24, but e^-x x < 0.4), a division and a sum
+  // Error of any fp32 score of this row. Sigmoid: expf (2 ulp), a sum and a division (2 ulp), 2^-20
+  // of the score. Softmax: expf, its argument (|l - top| 2^-24, but e^-x x < 0.4), a division and a sum
   // whose 2^6 lane terms and 32 lanes meet in a tree (11 roundings): 2^-19 of the largest.
-  const float score_err = p.bias ? (p.sigmoid ? 0x1p-21f : 0x1p-19f) * score(top) : 0.f;
+  const float score_err = p.bias ? (p.sigmoid ? 0x1p-20f : 0x1p-19f) * score(top) : 0.f;
   if constexpr (kSorted && EPT > 1) sort_lane(key, at);
 
   // ---- groups: the keep best, equal scores by ascending group
@@ -272,7 +311,7 @@ __global__ void __launch_bounds__(32 * kScoredWarps) route_scored_kernel(const _
       err = 2.f * score_err + 0x1p-22f * (fabsf(va) + fabsf(vb));
     } else if (two) {   // keys are logits: their scores, up to the softmax's common factor
       gs = p.sigmoid ? score(va) + score(vb) : expf(va - top) + expf(vb - top);
-      err = p.sigmoid ? 0x1p-21f * gs : 0x1p-20f;
+      err = p.sigmoid ? 0x1p-20f * gs : 0x1p-20f;
     }
     int rank = 0;
     for (int g = 0; g < p.groups; ++g) {
@@ -299,9 +338,8 @@ __global__ void __launch_bounds__(32 * kScoredWarps) route_scored_kernel(const _
   }
 
   // ---- the k largest keys, and the next one to compare with
-  uint32_t my_key = 0, next_key = 0, next_id = 0;
-  Choice my{0, 0.f};
-  for (int j = 0; j <= p.k; ++j) {
+  uint32_t next_key = 0, next_id = 0;
+  auto take_next = [&]() {   // the warp's best key and its lowest index, taken off its lane
     uint32_t best = 0;
     int pos = 0;
     if constexpr (kSorted) {
@@ -316,12 +354,8 @@ __global__ void __launch_bounds__(32 * kScoredWarps) route_scored_kernel(const _
         }
     }
     next_key = __reduce_max_sync(kFull, best);
-    const uint32_t id = static_cast<uint32_t>(first + p.lanes * pos);
+    const uint32_t id = static_cast<uint32_t>(first + pos);
     next_id = __reduce_min_sync(kFull, best == next_key ? id : 0xffffffffu);
-    if (lane == j) {
-      my_key = next_key;
-      my.id = static_cast<int>(next_id);
-    }
     if (best == next_key && id == next_id) {
       if constexpr (kSorted) {
 #pragma unroll
@@ -335,6 +369,15 @@ __global__ void __launch_bounds__(32 * kScoredWarps) route_scored_kernel(const _
         for (int i = 0; i < EPT; ++i)
           if (i == pos) key[i] = 0;
       }
+    }
+  };
+  uint32_t my_key = 0;
+  Choice my{0, 0.f};
+  for (int j = 0; j <= p.k; ++j) {
+    take_next();
+    if (lane == j) {
+      my_key = next_key;
+      my.id = static_cast<int>(next_id);
     }
   }
   if (lane >= p.k) {   // every other lane stands for the next one (key 0: there is none)
@@ -351,11 +394,12 @@ __global__ void __launch_bounds__(32 * kScoredWarps) route_scored_kernel(const _
     nl = next_key ? load_logit<kBf16>(p.logits, t * p.E + next_id) : 0.f;
     nb = next_key && p.bias ? p.bias[next_id] : 0.f;
   }
+  bool close = false;   // in the wrong order, perhaps
   if (lane < p.k) {
     const bool next = lane + 1 < p.k || next_key != 0;
     if (p.bias) {
       const float err = 2.f * score_err + 0x1p-22f * (fabsf(v) + fabsf(nv));
-      if (next) unsure |= !(v - nv > err) && !(my.logit == nl && mb == nb);
+      if (next) close = !(v - nv > err) && !(my.logit == nl && mb == nb);
       unsure |= !(fabsf(v) <= 3.4028235e38f);
     } else {
       // where 64-bit scores could merge distinct logits: next to 0 or 1, or next to each other
@@ -363,7 +407,48 @@ __global__ void __launch_bounds__(32 * kScoredWarps) route_scored_kernel(const _
       unsure |= p.sigmoid ? !(fabsf(v) <= 16.f) : !(top - v <= 600.f);
     }
   }
-  if (__any_sync(kFull, unsure)) my = choose_exact<kBf16, EPT>(p, t);
+  unsure = __any_sync(kFull, unsure);
+  if (__any_sync(kFull, close) && !unsure) {
+    // Sigmoid keys need no other expert's: a few more candidates, all of them in 64 bits, one to a
+    // lane, and the order is certain where the last one is out of reach of the k-th.
+    const int m = p.k + kSpare;
+    unsure = !p.sigmoid || m > 32;
+    if (!unsure) {
+      for (int j = p.k + 1; j < m; ++j) {
+        take_next();
+        if (lane == j) {
+          my_key = next_key;
+          my.id = static_cast<int>(next_id);
+        }
+      }
+      const bool there = lane < m && my_key != 0;
+      double key64 = 0.0;
+      if (there) {
+        my.logit = load_logit<kBf16>(p.logits, t * p.E + my.id);
+        key64 = 1.0 / (1.0 + exp(-static_cast<double>(my.logit))) + static_cast<double>(p.bias[my.id]);
+      }
+      const int n = __popc(__ballot_sync(kFull, there));
+      int rank = lane;
+      if (there) rank = 0;
+      for (int i = 0; i < n; ++i) {
+        const double o = __shfl_sync(kFull, key64, i);
+        const int oid = __shfl_sync(kFull, my.id, i);
+        if (there && (o > key64 || (o == key64 && oid < my.id))) ++rank;
+      }
+      int src = lane;
+      for (int i = 0; i < n; ++i)
+        if (__shfl_sync(kFull, rank, i) == lane) src = i;
+      my.id = __shfl_sync(kFull, my.id, src);
+      my.logit = __shfl_sync(kFull, my.logit, src);
+      key64 = __shfl_sync(kFull, key64, src);
+      if (n == m) {   // there may be more: none of them may reach the k-th
+        const float last = key_value32(next_key);
+        const float kth = static_cast<float>(__shfl_sync(kFull, key64, p.k - 1));
+        unsure = !(kth - last > 2.f * score_err + 0x1p-21f * (fabsf(kth) + fabsf(last)));
+      }
+    }
+  }
+  if (unsure) my = choose_exact<kBf16, EPT>(p, t);
 
   // ---- weights: scores of the chosen, the softmax's argument with the rounding of v - top put back
   float s = 0.f;
@@ -444,9 +529,13 @@ int route_scored(const void* logits, int dtype, int64_t T, int E, int k,
   p.w = w;
   p.w_bf16 = w_dtype == PRISM_MOE_BF16;
   p.counts = counts;
-  const int ept = static_cast<int>(ceil_div(p.per, p.lanes));
-  return dtype == PRISM_MOE_BF16 ? launch_scored<true>(p, ept, st)
-                                 : launch_scored<false>(p, ept, st);
+  p.each = static_cast<int>(ceil_div(p.per, p.lanes));
+  // rows, groups and lanes all start at multiples of 16 bytes of logits (and of 4 biases)
+  const int unit = dtype == PRISM_MOE_BF16 ? 8 : 4;
+  p.vec = E % unit == 0 && p.per % unit == 0 && p.each % unit == 0 &&
+          (reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(r.bias)) % 16 == 0;
+  return dtype == PRISM_MOE_BF16 ? launch_scored<true>(p, p.each, st)
+                                 : launch_scored<false>(p, p.each, st);
 }
 
 }  // namespace prism
