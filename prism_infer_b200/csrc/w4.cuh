@@ -34,6 +34,13 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t word, int i, uint32_t zer
   return d;
 }
 
+// bf16 pair 16 + code of inputs (2 i, 2 i + 1): the code in the upper four of the seven fraction bits
+// under the exponent of 16.
+__device__ __forceinline__ uint32_t code16_pair(uint32_t word, int i) {
+  const uint32_t c = i == 0 ? word << 3 : word >> (4 * i - 3);
+  return (c & 0x00780078u) | 0x41804180u;
+}
+
 // The PG scales of one row and chunk (global or shared memory), widened to fp32 (exact).
 template <int PG>
 __device__ __forceinline__ void load_scales(const uint16_t* p, float (&s)[PG]) {
@@ -70,6 +77,22 @@ __device__ __forceinline__ void load_zeros(const uint8_t* z, int64_t at, uint32_
     for (int i = 0; i < PG; ++i)
       out[i] = (((v >> (8 * i)) & 0xfu) * 0x00010001u) | 0x43004300u;
   }
+}
+
+// 16 + zero for each of the PG groups, as code16_pair's sums need it; 8 without zero points.
+template <int PG, bool kZeros>
+__device__ __forceinline__ void load_zero_points(const uint8_t* z, float (&out)[PG]) {
+  uint32_t v = 0x08080808u;
+  if constexpr (kZeros) {
+    if constexpr (PG == 1)
+      v = *z;
+    else if constexpr (PG == 2)
+      v = *reinterpret_cast<const uint16_t*>(z);
+    else
+      v = *reinterpret_cast<const uint32_t*>(z);
+  }
+#pragma unroll
+  for (int i = 0; i < PG; ++i) out[i] = 16.f + static_cast<float>((v >> (8 * i)) & 0xfu);
 }
 
 // silu(g) * u in fp32.
@@ -113,6 +136,40 @@ __device__ __forceinline__ void build_row_blocks(const int32_t* seg_offsets, int
     carry += __shfl_sync(0xffffffffu, incl, 31);
   }
   if (lane == 0) prefix[nseg] = carry;
+}
+
+// The same by all threads of a block (at most 1024 segments, blocks of up to 256 threads): every
+// offset is loaded at once, so the list costs one memory latency. Ends with a barrier.
+__device__ __forceinline__ void build_row_blocks_cta(const int32_t* seg_offsets, int nseg,
+                                                     int64_t rows_cap, int bm, int32_t* prefix,
+                                                     int64_t max_rows) {
+  __shared__ int32_t warp_sum[8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int each = (nseg + blockDim.x - 1) / blockDim.x;
+  const int first = threadIdx.x * each;
+  int32_t mine = 0;
+  for (int i = 0; i < each; ++i)
+    if (first + i < nseg) {
+      const RowSpan r = segment_rows(seg_offsets, first + i, rows_cap);
+      const int64_t len = r.end - r.begin;
+      const int32_t b = len > 0 && len <= max_rows ? static_cast<int32_t>((len + bm - 1) / bm) : 0;
+      prefix[first + i] = mine;   // within this thread's run
+      mine += b;
+    }
+  int32_t incl = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int32_t y = __shfl_up_sync(0xffffffffu, incl, off);
+    if (lane >= off) incl += y;
+  }
+  if (lane == 31) warp_sum[warp] = incl;
+  __syncthreads();
+  int32_t before = incl - mine;
+  for (int w = 0; w < warp; ++w) before += warp_sum[w];
+  for (int i = 0; i < each; ++i)
+    if (first + i < nseg) prefix[first + i] += before;
+  if (threadIdx.x == blockDim.x - 1) prefix[nseg] = before + mine;
+  __syncthreads();
 }
 
 }  // namespace prism

@@ -11,10 +11,19 @@
 // signed integer, exactly. The instruction multiplies integers by activations and sums in fp32; the
 // scale is applied to the fp32 sum of each group, so no weight is ever rounded.
 //
+// The subtraction of 128 + zero that code_pair does would be a third of the decoding. It is left out
+// here: the instruction sums (16 + code) * x (w4.cuh, code16_pair), exactly up to its fp32 sum, and
+// (16 + zero) * sum(x) of the group is taken off together with the scale; sum(x) of each group comes
+// from one more instruction per input step, on a matrix of ones, once per block of rows. The price
+// is cancellation: sums carry 16 .. 31 instead of -8 .. 7, about four times the fp32 error of the
+// plain sum, still 2^-18 of it at 4096 inputs.
+//
 // What bounds it: few rows reuse nothing, so every hit weight crosses HBM once and that is the floor.
 // A block's warps split the inputs (kw ways) and keep their part of x in registers while the block
-// streams its row tiles; the partial sums meet in shared memory in a fixed order. Blocks walk a
-// device-side list of (segment, output tile, 8 * NT rows), so the host needs no counts.
+// streams its row tiles; the partial sums meet in shared memory in a fixed order. Every lane copies
+// the 16-byte pieces that it will use itself (cp.async, kDepth row tiles ahead, across the borders
+// of blocks of rows), so no barrier stands between a copy and its use. Blocks take equal runs of a
+// device-side list of (segment's rows, output tiles), so the host needs no counts.
 #include <algorithm>
 
 #include "internal.h"
@@ -27,6 +36,8 @@ namespace {
 constexpr int kWarps = 8;
 constexpr int kSmallRows = 16;
 constexpr int kCh = 2;          // 128-input chunks a warp keeps in registers per pass
+constexpr int kDepth = 3;       // row tiles in flight per warp, the one in use included
+constexpr int kMaxRt = 4;       // row tiles per item
 constexpr int kColStride = 20;  // floats between the columns of a partial tile: no bank conflicts
 
 struct SmallParams {
@@ -57,137 +68,248 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+template <int B>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+  if constexpr (B == 16)
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src));
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(B));
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Scales and zero points of one chunk of a row tile, 4 lanes to a row g: lane t = 0 and 1 copy the
+// scales of rows g and g + 8, t = 2 and 3 the zero points, in pieces of kMetaBytes (which hold
+// neighbouring rows too where a row has fewer bytes than a copy must have).
+template <int PG>
+struct Meta {
+  static constexpr int kBytes = PG == 4 ? 8 : 4;
+  static constexpr int kScaleRows = PG == 1 ? 2 : 1;                // rows in a piece of scales
+  static constexpr int kZeroRows = PG == 4 ? 2 : PG == 2 ? 2 : 4;   // rows in a piece of zero points
+};
+
 template <int G, bool kZeros, bool kSwiGLU, int NT>
 __global__ void __launch_bounds__(32 * kWarps, 2) w4_small_kernel(const SmallParams p) {
   constexpr int PG = 128 / G;   // groups per chunk
-  extern __shared__ float smem[];
-  int32_t* prefix = reinterpret_cast<int32_t*>(smem);
-  float* part = smem + (p.nseg + 1 + 3) / 4 * 4;
+  using M = Meta<PG>;
+  constexpr int kMetaSlot = 32 * M::kBytes;
+  constexpr int kSlot = kCh * (1024 + kMetaSlot);
+  extern __shared__ uint4 smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(smem_raw);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int nwarps = blockDim.x >> 5;
+  uint8_t* ring = smem + warp * kDepth * kSlot;
+  const uint32_t ring_at = smem_u32(ring);
+  float* part = reinterpret_cast<float*>(smem + nwarps * kDepth * kSlot);
   const int g = lane >> 2, t = lane & 3;
   const int wk = warp % p.kw, wr = warp / p.kw;
-  const int nwarps = blockDim.x >> 5;
-  const int tile_floats = 8 * NT * kColStride;
+  constexpr int kTile = 8 * NT * kColStride;          // floats of a partial tile
+  int32_t* prefix = reinterpret_cast<int32_t*>(part + 2 * p.kw * p.rt * kTile);
 
-  if (warp == 0) build_row_blocks(p.seg_offsets, p.nseg, p.rows_cap, 8 * NT, prefix, 0, p.max_rows);
-  __syncthreads();
-  const int64_t total = static_cast<int64_t>(prefix[p.nseg]) * p.blocks_n;
+  build_row_blocks_cta(p.seg_offsets, p.nseg, p.rows_cap, 8 * NT, prefix, p.max_rows);
+  const int total = prefix[p.nseg] * p.blocks_n;
+  // this block's run of items
+  const int64_t bid = blockIdx.x, blocks = gridDim.x;
+  const int item0 = static_cast<int>(total * bid / blocks);
+  const int item1 = static_cast<int>(total * (bid + 1) / blocks);
+  if (item0 >= item1) return;
 
-  for (int64_t item = blockIdx.x; item < total; item += gridDim.x) {
-    const int sg = find_segment(prefix, p.nseg, static_cast<int32_t>(item / p.blocks_n));
-    const int units = prefix[sg + 1] - prefix[sg];
-    const int64_t rem = item - static_cast<int64_t>(prefix[sg]) * p.blocks_n;
-    const int nb = static_cast<int>(rem / units), tb = static_cast<int>(rem % units);
-    const RowSpan span = segment_rows(p.seg_offsets, sg, p.rows_cap);
-    const int64_t row0 = span.begin + static_cast<int64_t>(tb) * 8 * NT;
-    const int rows = static_cast<int>(min(static_cast<int64_t>(8 * NT), span.end - row0));
+  // ---- the stream of row tiles: item by item, pass by pass, every rw-th tile of the item
+  struct Cursor {
+    int item, pass, i, tiles;   // i: row tile within the item, tiles: of the item
+    int64_t base;               // first row tile of the item in the stack; < 0: no such expert
+  };
+  auto open = [&](Cursor& c) {
+    if (c.item >= item1) return;
+    const int unit = c.item / p.blocks_n, nb = c.item % p.blocks_n;
+    const int sg = find_segment(prefix, p.nseg, unit);
     const int e = p.seg_expert ? p.seg_expert[sg] : (p.num_mats == 1 ? 0 : sg);
-    if (e < 0 || e >= p.num_mats) {   // an id no weights belong to: recorded, never read
-      if (threadIdx.x == 0) record_device_error(p.err, PRISM_MOE_ERR_ARG);
-      continue;
+    c.tiles = min(p.tiles - nb * p.rt, p.rt);
+    c.base = e >= 0 && e < p.num_mats ? static_cast<int64_t>(e) * p.tiles + nb * p.rt : -1;
+  };
+  auto settle = [&](Cursor& c) {   // on to the next tile that this warp has
+    while (c.item < item1 && c.i >= c.tiles) {
+      c.i = wr;
+      if (++c.pass == p.passes) {
+        c.pass = 0;
+        ++c.item;
+        open(c);
+      }
     }
-    const int64_t mat = static_cast<int64_t>(e) * p.tiles;
-    const int tile_end = min(p.tiles - nb * p.rt, p.rt);
+  };
+  auto advance = [&](Cursor& c) {
+    c.i += p.rw;
+    settle(c);
+  };
+  auto fetch = [&](const Cursor& c, int slot) {
+    if (c.item < item1 && c.base >= 0) {
+      const int c0 = (c.pass * p.kw + wk) * kCh;
+      const int64_t chunk = (c.base + c.i) * p.chunks + c0;
+#pragma unroll
+      for (int ch = 0; ch < kCh; ++ch)
+        if (c0 + ch < p.chunks) {
+          const uint32_t to = ring_at + slot * kSlot + ch * (1024 + kMetaSlot);
+          const uint8_t* from = p.q + (chunk + ch) * 1024 + lane * 16;
+          copy_async<16>(to + lane * 16, from);
+          copy_async<16>(to + lane * 16 + 512, from + 512);
+          const int row = g + 8 * (t & 1);
+          const int64_t first = (chunk + ch) * 16 * PG;
+          if (t < 2)
+            copy_async<M::kBytes>(to + 1024 + lane * M::kBytes,
+                                  p.s + first + (row & ~(M::kScaleRows - 1)) * PG);
+          else if (kZeros)
+            copy_async<M::kBytes>(to + 1024 + lane * M::kBytes,
+                                  p.z + first + (row & ~(M::kZeroRows - 1)) * PG);
+        }
+    }
+    copy_commit();
+  };
+  Cursor ahead{item0, 0, wr, 0, -1};
+  open(ahead);
+  settle(ahead);
+  int fill = 0;   // slot of the next copy
+#pragma unroll
+  for (int d = 0; d < kDepth - 1; ++d) {
+    fetch(ahead, fill);
+    advance(ahead);
+    fill = fill + 1 == kDepth ? 0 : fill + 1;
+  }
 
+  uint4 xb[kCh][NT][4];
+  float sx[kCh][PG][NT][2];   // sum of x over each group, columns 2 t and 2 t + 1
+  int loaded_unit = -1, loaded_pass = -1, use = 0;
+  int rows = 0;
+  int64_t row0 = 0;
+  for (int item = item0, round = 0; item < item1; ++item, round ^= 1) {
+    const int unit = item / p.blocks_n, nb = item % p.blocks_n;
+    Cursor now{item, 0, wr, 0, -1};
+    open(now);
+    if (unit != loaded_unit) {
+      const int sg = find_segment(prefix, p.nseg, unit);
+      const RowSpan span = segment_rows(p.seg_offsets, sg, p.rows_cap);
+      row0 = span.begin + static_cast<int64_t>(unit - prefix[sg]) * 8 * NT;
+      rows = static_cast<int>(min(static_cast<int64_t>(8 * NT), span.end - row0));
+    }
+    float* sums = part + round * p.kw * p.rt * kTile;
     for (int pass = 0; pass < p.passes; ++pass) {
       const int c0 = (pass * p.kw + wk) * kCh;
-      uint4 wq[2][kCh][2];
-      auto load_tile = [&](int i, uint4(&w)[kCh][2]) {
-        const int64_t base = (mat + nb * p.rt + i) * p.chunks;
+      if (unit != loaded_unit || pass != loaded_pass) {
+        // this warp's part of x: rows g (+ 8 nt), inputs 8 t .. 8 t + 7 of each 32
+        loaded_unit = unit;
+        loaded_pass = pass;
 #pragma unroll
         for (int c = 0; c < kCh; ++c)
-          if (c0 + c < p.chunks) {
-            const uint8_t* at = p.q + (base + c0 + c) * 1024 + lane * 16;
-            w[c][0] = load_stream(at);
-            w[c][1] = load_stream(at + 512);
-          }
-      };
-      if (wr < tile_end) load_tile(wr, wq[0]);
-      // this warp's part of x: rows g (+ 8 nt), inputs 8 t .. 8 t + 7 of each 32
-      uint4 xb[kCh][NT][4];
 #pragma unroll
-      for (int c = 0; c < kCh; ++c)
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+            for (int j = 0; j < 4; ++j) {
+              const int k = (c0 + c) * 128 + j * 32 + t * 8;
+              const bool ok = g + 8 * nt < rows && k < p.K;
+              xb[c][nt][j] =
+                  ok ? *reinterpret_cast<const uint4*>(p.x + (row0 + g + 8 * nt) * p.ld_x + k)
+                     : make_uint4(0, 0, 0, 0);
+            }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int k = (c0 + c) * 128 + j * 32 + t * 8;
-            const bool ok = g + 8 * nt < rows && k < p.K;
-            xb[c][nt][j] = ok ? *reinterpret_cast<const uint4*>(p.x + (row0 + g + 8 * nt) * p.ld_x + k)
-                              : make_uint4(0, 0, 0, 0);
-          }
-      int buf = 0;
+        for (int c = 0; c < kCh; ++c)
+#pragma unroll
+          for (int gr = 0; gr < PG; ++gr)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              float ones[4] = {};
+              constexpr uint32_t one = 0x3f803f80u;
+#pragma unroll
+              for (int j = gr * (4 / PG); j < (gr + 1) * (4 / PG); ++j) {
+                mma_16816(ones, one, one, one, one, xb[c][nt][j].x, xb[c][nt][j].y);
+                mma_16816(ones, one, one, one, one, xb[c][nt][j].z, xb[c][nt][j].w);
+              }
+              sx[c][gr][nt][0] = ones[0];
+              sx[c][gr][nt][1] = ones[1];
+            }
+      }
 #pragma unroll 1
-      for (int i = wr; i < tile_end; i += p.rw, buf ^= 1) {
-        uint4 w[kCh][2];
-#pragma unroll
-        for (int c = 0; c < kCh; ++c) {
-          w[c][0] = wq[0][c][0];
-          w[c][1] = wq[0][c][1];
-        }
-        if (i + p.rw < tile_end) load_tile(i + p.rw, wq[0]);
+      for (int i = wr; i < now.tiles; i += p.rw) {
+        __syncwarp();   // every lane has read the slot that the next copies fill
+        fetch(ahead, fill);
+        advance(ahead);
+        fill = fill + 1 == kDepth ? 0 : fill + 1;
+        copy_wait<kDepth - 1>();
+        __syncwarp();   // scales and zero points were copied by other lanes of the row
+        const uint8_t* slot = ring + use * kSlot;
+        use = use + 1 == kDepth ? 0 : use + 1;
         float acc[NT][4] = {};
 #pragma unroll
         for (int c = 0; c < kCh; ++c) {
-          if (c0 + c >= p.chunks) continue;
-          const int64_t chunk = (mat + nb * p.rt + i) * p.chunks + c0 + c;
-          float sc[2][PG];
-          uint32_t zr[2][PG];
+          if (c0 + c >= p.chunks || now.base < 0) continue;
+          const uint8_t* at = slot + c * (1024 + kMetaSlot);
+          const uint4 w0 = *reinterpret_cast<const uint4*>(at + lane * 16);
+          const uint4 w1 = *reinterpret_cast<const uint4*>(at + lane * 16 + 512);
+          const uint8_t* meta = at + 1024 + g * 4 * M::kBytes;
+          float sc[2][PG], zp[2][PG];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const int64_t at = (chunk * 16 + g + 8 * h) * PG;
-            load_scales<PG>(p.s + at, sc[h]);
-            load_zeros<PG, kZeros>(p.z, at, zr[h]);
+            load_scales<PG>(reinterpret_cast<const uint16_t*>(meta + h * M::kBytes) +
+                                (g & (M::kScaleRows - 1)) * PG,
+                            sc[h]);
+            load_zero_points<PG, kZeros>(meta + (2 + h) * M::kBytes + (g & (M::kZeroRows - 1)) * PG,
+                                         zp[h]);
           }
 #pragma unroll
           for (int gr = 0; gr < PG; ++gr) {
-            float part_acc[NT][4] = {};
+            float sum[NT][4] = {};
 #pragma unroll
             for (int j = gr * (4 / PG); j < (gr + 1) * (4 / PG); ++j) {
-              const uint32_t w0 = word_of(w[c][0], j), w1 = word_of(w[c][1], j);
+              const uint32_t word0 = word_of(w0, j), word1 = word_of(w1, j);
               uint32_t a[2][4];
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
-                a[0][q] = code_pair(w0, q, zr[0][gr]);
-                a[1][q] = code_pair(w1, q, zr[1][gr]);
+                a[0][q] = code16_pair(word0, q);
+                a[1][q] = code16_pair(word1, q);
               }
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
-                mma_16816(part_acc[nt], a[0][0], a[1][0], a[0][1], a[1][1], xb[c][nt][j].x,
+                mma_16816(sum[nt], a[0][0], a[1][0], a[0][1], a[1][1], xb[c][nt][j].x,
                           xb[c][nt][j].y);
-                mma_16816(part_acc[nt], a[0][2], a[1][2], a[0][3], a[1][3], xb[c][nt][j].z,
+                mma_16816(sum[nt], a[0][2], a[1][2], a[0][3], a[1][3], xb[c][nt][j].z,
                           xb[c][nt][j].w);
               }
             }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              acc[nt][0] = fmaf(sc[0][gr], part_acc[nt][0], acc[nt][0]);
-              acc[nt][1] = fmaf(sc[0][gr], part_acc[nt][1], acc[nt][1]);
-              acc[nt][2] = fmaf(sc[1][gr], part_acc[nt][2], acc[nt][2]);
-              acc[nt][3] = fmaf(sc[1][gr], part_acc[nt][3], acc[nt][3]);
-            }
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                acc[nt][q] = fmaf(sc[q >> 1][gr],
+                                  fmaf(-zp[q >> 1][gr], sx[c][gr][nt][q & 1], sum[nt][q]),
+                                  acc[nt][q]);
           }
         }
-        float* mine = part + (wk * p.rt + i) * tile_floats;
+        float* mine = sums + (wk * p.rt + i) * kTile;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            float* at = mine + (8 * nt + 2 * t + (q & 1)) * kColStride + g + 8 * (q >> 1);
-            *at = pass == 0 ? acc[nt][q] : *at + acc[nt][q];   // the same lane's own sum
+            float* to = mine + (8 * nt + 2 * t + (q & 1)) * kColStride + g + 8 * (q >> 1);
+            *to = pass == 0 ? acc[nt][q] : *to + acc[nt][q];   // the same lane's own sum
           }
       }
     }
+    // one barrier per item: partial sums have two buffers, and a warp cannot be two items ahead
     __syncthreads();
+    if (now.base < 0) {   // an id no weights belong to: recorded, nothing written
+      if (threadIdx.x == 0) record_device_error(p.err, PRISM_MOE_ERR_ARG);
+      continue;
+    }
     // sum of the kw partial tiles, two outputs per thread, neighbours along the output row
     constexpr int kPairs = kSwiGLU ? 4 : 8;   // output pairs of one row tile
-    const int per_row = tile_end * kPairs;
+    const int per_row = now.tiles * kPairs;
     for (int i = threadIdx.x; i < rows * per_row; i += nwarps * 32) {
       const int col = i / per_row, pr = i % per_row;
       const int tile = pr / kPairs, r = pr % kPairs * 2;
-      const float* at = part + tile * tile_floats + col * kColStride + r;
+      const float* at = sums + tile * kTile + col * kColStride + r;
       float2 a = make_float2(0.f, 0.f), b = make_float2(0.f, 0.f);
-      for (int k = 0; k < p.kw; ++k, at += p.rt * tile_floats) {
+      for (int k = 0; k < p.kw; ++k, at += p.rt * kTile) {
         const float2 v = *reinterpret_cast<const float2*>(at);
         a.x += v.x;
         a.y += v.y;
@@ -205,8 +327,8 @@ __global__ void __launch_bounds__(32 * kWarps, 2) w4_small_kernel(const SmallPar
       if (n < p.n_out)
         *reinterpret_cast<uint32_t*>(p.out + (row0 + col) * p.n_out + n) = pack_bf16x2(a.x, a.y);
     }
-    __syncthreads();
   }
+  copy_wait<0>();
 }
 
 template <int G, bool kZeros, bool kSwiGLU, int NT>
@@ -217,26 +339,32 @@ int launch_small(SmallParams p, int64_t units, cudaStream_t st) {
   p.kw = static_cast<int>(ceil_div(p.chunks, p.passes * kCh));
   p.rw = std::max(1, kWarps / p.kw);
   const int sms = num_sms();
-  // row tiles per item: long items reuse x and amortise the joining of partial sums, short ones
-  // fill the GPU when the call is small
+  // row tiles per item: several share a barrier, few fill the GPU when the call is small
   p.rt = p.rw;
-  while (p.rt * 2 <= 8 && units * ceil_div(p.tiles, p.rt * 2) >= 4 * sms) p.rt *= 2;
+  while (p.rt * 2 <= kMaxRt && units * ceil_div(p.tiles, p.rt * 2) >= 4 * sms) p.rt *= 2;
   p.blocks_n = static_cast<int>(ceil_div(p.tiles, p.rt));
-  const int bytes = static_cast<int>(sizeof(float)) *
-                    ((p.nseg + 4) / 4 * 4 + p.kw * p.rt * 8 * NT * kColStride);
-  constexpr int kMaxBytes = 4 * ((kMaxW4Segments + 4) + 8 * 8 * 8 * NT * kColStride);
+  constexpr int kSlot = kCh * (1024 + 32 * Meta<128 / G>::kBytes);
+  constexpr int kTile = 8 * NT * kColStride;
+  const int warps = p.kw * p.rw;
+  const int bytes = warps * kDepth * kSlot + 2 * p.kw * p.rt * kTile * 4 + (p.nseg + 4) / 4 * 16;
+  constexpr int kMaxBytes = kWarps * kDepth * kSlot + 2 * kWarps * kMaxRt * kTile * 4 +
+                            (kMaxW4Segments + 4) / 4 * 16;
+  static_assert(kMaxBytes <= 232448, "shared memory budget");
   if (int r = ensure_smem_attr(reinterpret_cast<const void*>(kern), kMaxBytes)) return r;
   const int64_t items = units * p.blocks_n;
-  const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(items, 2 * sms)));
-  kern<<<grid, 32 * p.kw * p.rw, bytes, st>>>(p);
+  PRISM_CHECK_ARG(items < (int64_t(1) << 31), "4-bit product: too many outputs");
+  const int per_sm = std::max(1, std::min({65536 / (128 * 32 * warps), 232448 / (bytes + 1024), 4}));
+  const int grid =
+      static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(items, per_sm * sms)));
+  kern<<<grid, 32 * warps, bytes, st>>>(p);
   PRISM_LAUNCH_CHECK("w4_small_kernel launch");
   return PRISM_MOE_OK;
 }
 
 template <int G, bool kZeros, bool kSwiGLU>
 int launch_rows(const SmallParams& p, int64_t units8, int64_t units16, cudaStream_t st) {
-  // 16 rows at a time once segments average more than 8
-  if (p.rows_cap > 8 * static_cast<int64_t>(p.nseg))
+  // 16 rows at a time once segments average more than 5
+  if (p.rows_cap > 5 * static_cast<int64_t>(p.nseg))
     return launch_small<G, kZeros, kSwiGLU, 2>(p, units16, st);
   return launch_small<G, kZeros, kSwiGLU, 1>(p, units8, st);
 }
@@ -256,13 +384,16 @@ int launch_zeros(const SmallParams& p, bool swiglu, int64_t u8, int64_t u16, cud
 }  // namespace
 
 int w4_product(const W4Problem& pr, cudaStream_t st) {
-  // Segments of at most kSmallRows rows run here, longer ones on the other kernel; the host does
-  // not know the segments' lengths, so a call whose rows could make both kinds launches both.
-  if (pr.rows_cap > kSmallRows)
-    if (int r = w4_product_large(pr, kSmallRows, st)) return r;
-  if (pr.nseg == 1 && pr.rows_cap > kSmallRows && !pr.seg_offsets) return PRISM_MOE_OK;
   SmallParams p{};
-  p.max_rows = kSmallRows;
+  p.max_rows = int64_t(1) << 31;
+  // Few rows per segment on average: this kernel alone (a longer segment runs in blocks of 16 rows,
+  // its weights from L2 after the first). Else segments of at most kSmallRows rows run here and
+  // longer ones on the other kernel; the host does not know the lengths and launches both.
+  if (pr.rows_cap > std::max<int64_t>(kSmallRows, pr.seg_offsets ? 8 * pr.nseg : 0)) {
+    if (int r = w4_product_large(pr, kSmallRows, st)) return r;
+    if (!pr.seg_offsets) return PRISM_MOE_OK;
+    p.max_rows = kSmallRows;
+  }
   p.x = static_cast<const uint16_t*>(pr.x);
   p.ld_x = pr.K;
   p.K = static_cast<int>(pr.K);
@@ -281,7 +412,7 @@ int w4_product(const W4Problem& pr, cudaStream_t st) {
   p.err = pr.err;
   // most row blocks there can be, however the rows fall into segments
   const int64_t hit = std::min<int64_t>(pr.nseg, pr.rows_cap);
-  const int64_t u8 = std::min(hit + pr.rows_cap / 8, 2 * hit), u16 = hit;
+  const int64_t u8 = hit + pr.rows_cap / 8, u16 = hit + pr.rows_cap / 16;
   switch (pr.w.group_size) {
     case 32: return launch_zeros<32>(p, pr.swiglu, u8, u16, st);
     case 64: return launch_zeros<64>(p, pr.swiglu, u8, u16, st);

@@ -1,15 +1,19 @@
 """Products with 4-bit weights on the GPU against 64-bit arithmetic on the same codes and scales.
 
-Bounds, element by element. The kernels multiply integers (code - zero) by bf16 activations, exactly,
-and sum in fp32: a sum of n partial sums in whatever order is off by at most n * 2^-22 of the sum of
-the terms' magnitudes (2^-24 for each rounding, four times that for the tensor cores' alignment of
-their addends). n is the 16-input steps of one group, the groups, and the joining of up to 16 parts.
+Bounds, element by element. The kernels multiply small integers by bf16 activations, exactly, and
+sum in fp32: a sum of n partial sums in whatever order is off by at most n * 2^-22 of the sum of the
+terms' magnitudes (2^-24 for each rounding, four times that for the tensor cores' alignment of their
+addends). n is the 16-input steps of one group, the groups, and the joining of up to 16 parts. The
+integers are code - zero for many rows; for few rows 16 + code and 16 + zero are summed apart, 31 at
+most each: terms of up to 62 * scale * |x| in all.
 Outputs are rounded to bf16: 2^-8 of the value. In the experts, silu(g) * u is rounded to bf16
 between the products (2^-8 of each h, passed on by |w_down|), and |silu'| <= 1.1.
 Over a whole output the 2-norm of the difference stays below 2^-8 of the result's: a rounding's
 error is spread over [-2^-8, 2^-8] at most, so its rms is at most 2^-8 / sqrt(3), and two of them
 (h and y) come to 2^-8 * sqrt(2/3).
 """
+from dataclasses import replace
+
 import pytest
 import torch
 
@@ -37,13 +41,20 @@ def rows(seed, M, K):
     return torch.randn(M, K, generator=gen_of(seed), device=DEV).to(torch.bfloat16)
 
 
+def most(w):
+    """62 * scale of every weight, rows as dequantize_w4 gives them."""
+    zeros = torch.zeros(w.scales.shape, dtype=torch.uint8, device=w.device)
+    ones = replace(w, qweight=torch.full_like(w.qweight, 0xff), zeros=zeros)
+    return dequantize_w4(ones, torch.float64) * (62 / 15)
+
+
 def steps(w):
     return (w.group_size // 16 + w.in_features // w.group_size + 16) * 2.0 ** -22
 
 
 def check_linear(x, w, y):
     wd, xd = dequantize_w4(w, torch.float64), x.double()
-    ref, mag = xd @ wd.t(), xd.abs() @ wd.abs().t()
+    ref, mag = xd @ wd.t(), xd.abs() @ most(w).t()
     off = (y.double() - ref).abs()
     assert (off <= HALF * ref.abs() + steps(w) * mag * (1 + HALF)).all(), off.max()
     if ref.numel() >= 256:
@@ -53,6 +64,7 @@ def check_linear(x, w, y):
 def check_experts(x, bounds, experts, gu, dn, y):
     """``experts[s]`` is segment s's expert (None: the segment is left alone)."""
     all_gu, all_dn = dequantize_w4(gu, torch.float64), dequantize_w4(dn, torch.float64)
+    most_gu, most_dn = most(gu), most(dn)
     diff = total = 0.0
     for s, e in enumerate(experts):
         a, b = bounds[s], bounds[s + 1]
@@ -61,12 +73,12 @@ def check_experts(x, bounds, experts, gu, dn, y):
         wg, wu = all_gu[e].chunk(2)
         wd, xd = all_dn[e], x[a:b].double()
         g, u = xd @ wg.t(), xd @ wu.t()
-        dg, du = (steps(gu) * (xd.abs() @ w.abs().t()) for w in (wg, wu))
+        dg, du = (steps(gu) * (xd.abs() @ w.t()) for w in most_gu[e].chunk(2))
         sg = g * torch.sigmoid(g)
         h = sg * u
         dh = (HALF + 2.0 ** -20) * h.abs() + (1.1 * u.abs() * dg + (sg.abs() + 1.1 * dg) * du) * 1.01
         ref = h @ wd.t()
-        mag = (h.abs() + dh) @ wd.abs().t()
+        mag = (h.abs() + dh) @ most_dn[e].t()
         off = (y[a:b].double() - ref).abs()
         tol = (dh @ wd.abs().t() + steps(dn) * mag) * (1 + HALF) + HALF * ref.abs()
         assert (off <= tol).all(), (s, e, (off - tol).max().item())
