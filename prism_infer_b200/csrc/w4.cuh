@@ -28,17 +28,19 @@ __device__ __forceinline__ uint32_t word_of(const uint4& v, int j) {
 // bf16 pair (code - zero) of inputs (2 i, 2 i + 1); ``zero`` holds 128 + zero twice. Both the value
 // 128 + code (128 .. 143, 7 fraction bits suffice) and the difference are exact.
 __device__ __forceinline__ uint32_t code_pair(uint32_t word, int i, uint32_t zero) {
-  const uint32_t c = ((word >> (4 * i)) & 0x000f000fu) | 0x43004300u;
-  uint32_t d;
+  uint32_t c, d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(c) : "r"(word >> (4 * i)), "r"(0x000f000fu), "r"(0x43004300u));
   asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(c), "r"(zero));
   return d;
 }
 
 // bf16 pair 16 + code of inputs (2 i, 2 i + 1): the code in the upper four of the seven fraction bits
-// under the exponent of 16.
+// under the exponent of 16. Mask and exponent go in with one three-input operation.
 __device__ __forceinline__ uint32_t code16_pair(uint32_t word, int i) {
   const uint32_t c = i == 0 ? word << 3 : word >> (4 * i - 3);
-  return (c & 0x00780078u) | 0x41804180u;
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(c), "r"(0x00780078u), "r"(0x41804180u));
+  return d;
 }
 
 // The PG scales of one row and chunk (global or shared memory), widened to fp32 (exact).

@@ -36,7 +36,9 @@ namespace {
 constexpr int kWarps = 8;
 constexpr int kSmallRows = 16;
 constexpr int kCh = 2;          // 128-input chunks a warp keeps in registers per pass
-constexpr int kDepth = 3;       // row tiles in flight per warp, the one in use included
+constexpr int kDepth = 2;       // steps in flight per warp, the one in use included
+constexpr int kMaxKwRt = 4;     // kw * rt <= kWarps * kMaxKwRt
+constexpr int kTps = 2;         // row tiles per step
 constexpr int kMaxRt = 4;       // row tiles per item
 constexpr int kColStride = 20;  // floats between the columns of a partial tile: no bank conflicts
 
@@ -68,12 +70,15 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <int B>
+// ``B`` bytes from src + kFrom to shared memory at dst + kTo.
+template <int B, int kTo, int kFrom>
 __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
   if constexpr (B == 16)
-    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src));
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0+%2], [%1+%3], 16;" ::"r"(dst), "l"(src),
+                 "n"(kTo), "n"(kFrom));
   else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(B));
+    asm volatile("cp.async.ca.shared.global [%0+%2], [%1+%3], %4;" ::"r"(dst), "l"(src), "n"(kTo),
+                 "n"(kFrom), "n"(B));
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;"); }
 template <int N>
@@ -92,11 +97,11 @@ struct Meta {
 };
 
 template <int G, bool kZeros, bool kSwiGLU, int NT>
-__global__ void __launch_bounds__(32 * kWarps, 2) w4_small_kernel(const SmallParams p) {
+__global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 2 : 1) w4_small_kernel(const SmallParams p) {
   constexpr int PG = 128 / G;   // groups per chunk
   using M = Meta<PG>;
   constexpr int kMetaSlot = 32 * M::kBytes;
-  constexpr int kSlot = kCh * (1024 + kMetaSlot);
+  constexpr int kSlot = kTps * kCh * (1024 + kMetaSlot);
   extern __shared__ uint4 smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(smem_raw);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -117,88 +122,92 @@ __global__ void __launch_bounds__(32 * kWarps, 2) w4_small_kernel(const SmallPar
   const int item1 = static_cast<int>(total * (bid + 1) / blocks);
   if (item0 >= item1) return;
 
-  // ---- the stream of row tiles: item by item, pass by pass, every rw-th tile of the item
-  struct Cursor {
-    int item, pass, i, tiles;   // i: row tile within the item, tiles: of the item
-    int64_t base;               // first row tile of the item in the stack; < 0: no such expert
+  // ---- the stream of steps: item by item, pass by pass, kTps row tiles a step. Every item has the
+  // same steps and every step the same copies: what lies past the last tile or chunk is read from
+  // the last one instead and its sums are not used (or its x is zero).
+  struct Place {
+    int unit, nb, base;   // unit's rows, item of the unit, first row tile of its matrix (< 0: none)
   };
-  auto open = [&](Cursor& c) {
-    if (c.item >= item1) return;
-    const int unit = c.item / p.blocks_n, nb = c.item % p.blocks_n;
+  auto matrix = [&](int unit) {
     const int sg = find_segment(prefix, p.nseg, unit);
     const int e = p.seg_expert ? p.seg_expert[sg] : (p.num_mats == 1 ? 0 : sg);
-    c.tiles = min(p.tiles - nb * p.rt, p.rt);
-    c.base = e >= 0 && e < p.num_mats ? static_cast<int64_t>(e) * p.tiles + nb * p.rt : -1;
+    return e >= 0 && e < p.num_mats ? e * p.tiles : -1;
   };
-  auto settle = [&](Cursor& c) {   // on to the next tile that this warp has
-    while (c.item < item1 && c.i >= c.tiles) {
-      c.i = wr;
-      if (++c.pass == p.passes) {
-        c.pass = 0;
-        ++c.item;
-        open(c);
+  auto step_on = [&](Place& at, bool more) {
+    if (++at.nb == p.blocks_n) {
+      at.nb = 0;
+      ++at.unit;
+      if (more) at.base = matrix(at.unit);
+    }
+  };
+  const int first_i = wr * kTps, next_i = p.rw * kTps;
+  // this lane's pieces: 16 bytes of rows g and g + 8, and scales (t < 2) or zero points
+  const int meta_row = g + 8 * (t & 1);
+  const uint8_t* q_lane = p.q + lane * 16;
+  const uint8_t* m_lane =
+      t < 2 ? reinterpret_cast<const uint8_t*>(p.s) + (meta_row & ~(M::kScaleRows - 1)) * PG * 2
+            : p.z + (meta_row & ~(M::kZeroRows - 1)) * PG;
+  const int m_stride = t < 2 ? 32 * PG : 16 * PG;
+  const uint32_t ring_lane = ring_at + lane * 16, ring_meta = ring_at + lane * M::kBytes;
+  Place ahead{item0 / p.blocks_n, item0 % p.blocks_n, 0};
+  ahead.base = matrix(ahead.unit);
+  Place now = ahead;
+  int ahead_item = item0, ahead_pass = 0, ahead_i = first_i;
+  uint32_t fill = 0, use = 0;   // byte offsets of the slots
+  auto fetch = [&]() {
+    if (ahead_item < item1) {
+      const int c0 = (ahead_pass * p.kw + wk) * kCh;
+      const int tile0 = ahead.nb * p.rt + ahead_i;
+#pragma unroll
+      for (int u = 0; u < kTps; ++u) {
+        const int row = (max(ahead.base, 0) + min(tile0 + u, p.tiles - 1)) * p.chunks;
+#pragma unroll
+        for (int ch = 0; ch < kCh; ++ch) {
+          const int chunk = row + min(c0 + ch, p.chunks - 1);
+          const uint8_t* from = q_lane + static_cast<int64_t>(chunk) * 1024;
+          const uint32_t to = ring_lane + fill + (u * kCh + ch) * (1024 + kMetaSlot);
+          copy_async<16, 0, 0>(to, from);
+          copy_async<16, 512, 512>(to, from);
+          if (kZeros || t < 2)
+            copy_async<M::kBytes, 1024, 0>(ring_meta + fill + (u * kCh + ch) * (1024 + kMetaSlot),
+                                           m_lane + static_cast<int64_t>(chunk) * m_stride);
+        }
+      }
+      ahead_i += next_i;
+      if (ahead_i >= p.rt) {
+        ahead_i = first_i;
+        if (++ahead_pass == p.passes) {
+          ahead_pass = 0;
+          ++ahead_item;
+          step_on(ahead, ahead_item < item1);
+        }
       }
     }
-  };
-  auto advance = [&](Cursor& c) {
-    c.i += p.rw;
-    settle(c);
-  };
-  auto fetch = [&](const Cursor& c, int slot) {
-    if (c.item < item1 && c.base >= 0) {
-      const int c0 = (c.pass * p.kw + wk) * kCh;
-      const int64_t chunk = (c.base + c.i) * p.chunks + c0;
-#pragma unroll
-      for (int ch = 0; ch < kCh; ++ch)
-        if (c0 + ch < p.chunks) {
-          const uint32_t to = ring_at + slot * kSlot + ch * (1024 + kMetaSlot);
-          const uint8_t* from = p.q + (chunk + ch) * 1024 + lane * 16;
-          copy_async<16>(to + lane * 16, from);
-          copy_async<16>(to + lane * 16 + 512, from + 512);
-          const int row = g + 8 * (t & 1);
-          const int64_t first = (chunk + ch) * 16 * PG;
-          if (t < 2)
-            copy_async<M::kBytes>(to + 1024 + lane * M::kBytes,
-                                  p.s + first + (row & ~(M::kScaleRows - 1)) * PG);
-          else if (kZeros)
-            copy_async<M::kBytes>(to + 1024 + lane * M::kBytes,
-                                  p.z + first + (row & ~(M::kZeroRows - 1)) * PG);
-        }
-    }
     copy_commit();
+    fill = fill == (kDepth - 1) * kSlot ? 0 : fill + kSlot;
   };
-  Cursor ahead{item0, 0, wr, 0, -1};
-  open(ahead);
-  settle(ahead);
-  int fill = 0;   // slot of the next copy
 #pragma unroll
-  for (int d = 0; d < kDepth - 1; ++d) {
-    fetch(ahead, fill);
-    advance(ahead);
-    fill = fill + 1 == kDepth ? 0 : fill + 1;
-  }
+  for (int d = 0; d < kDepth - 1; ++d) fetch();
 
   uint4 xb[kCh][NT][4];
   float sx[kCh][PG][NT][2];   // sum of x over each group, columns 2 t and 2 t + 1
-  int loaded_unit = -1, loaded_pass = -1, use = 0;
+  int loaded_unit = -1, loaded_pass = -1;
   int rows = 0;
   int64_t row0 = 0;
   for (int item = item0, round = 0; item < item1; ++item, round ^= 1) {
-    const int unit = item / p.blocks_n, nb = item % p.blocks_n;
-    Cursor now{item, 0, wr, 0, -1};
-    open(now);
-    if (unit != loaded_unit) {
-      const int sg = find_segment(prefix, p.nseg, unit);
+    if (now.unit != loaded_unit) {
+      const int sg = find_segment(prefix, p.nseg, now.unit);
       const RowSpan span = segment_rows(p.seg_offsets, sg, p.rows_cap);
-      row0 = span.begin + static_cast<int64_t>(unit - prefix[sg]) * 8 * NT;
+      row0 = span.begin + static_cast<int64_t>(now.unit - prefix[sg]) * 8 * NT;
       rows = static_cast<int>(min(static_cast<int64_t>(8 * NT), span.end - row0));
     }
     float* sums = part + round * p.kw * p.rt * kTile;
+    float* mine = sums + wk * p.rt * kTile + 2 * t * kColStride + g;
     for (int pass = 0; pass < p.passes; ++pass) {
-      const int c0 = (pass * p.kw + wk) * kCh;
-      if (unit != loaded_unit || pass != loaded_pass) {
+      if (now.unit != loaded_unit || pass != loaded_pass) {
         // this warp's part of x: rows g (+ 8 nt), inputs 8 t .. 8 t + 7 of each 32
-        loaded_unit = unit;
+        const int c0 = (pass * p.kw + wk) * kCh;
+        loaded_unit = now.unit;
         loaded_pass = pass;
 #pragma unroll
         for (int c = 0; c < kCh; ++c)
@@ -230,80 +239,82 @@ __global__ void __launch_bounds__(32 * kWarps, 2) w4_small_kernel(const SmallPar
             }
       }
 #pragma unroll 1
-      for (int i = wr; i < now.tiles; i += p.rw) {
+      for (int i0 = first_i; i0 < p.rt; i0 += next_i) {
         __syncwarp();   // every lane has read the slot that the next copies fill
-        fetch(ahead, fill);
-        advance(ahead);
-        fill = fill + 1 == kDepth ? 0 : fill + 1;
+        fetch();
         copy_wait<kDepth - 1>();
         __syncwarp();   // scales and zero points were copied by other lanes of the row
-        const uint8_t* slot = ring + use * kSlot;
-        use = use + 1 == kDepth ? 0 : use + 1;
-        float acc[NT][4] = {};
+        const uint8_t* slot = ring + use;
+        use = use == (kDepth - 1) * kSlot ? 0 : use + kSlot;
 #pragma unroll
-        for (int c = 0; c < kCh; ++c) {
-          if (c0 + c >= p.chunks || now.base < 0) continue;
-          const uint8_t* at = slot + c * (1024 + kMetaSlot);
-          const uint4 w0 = *reinterpret_cast<const uint4*>(at + lane * 16);
-          const uint4 w1 = *reinterpret_cast<const uint4*>(at + lane * 16 + 512);
-          const uint8_t* meta = at + 1024 + g * 4 * M::kBytes;
-          float sc[2][PG], zp[2][PG];
+        for (int u = 0; u < kTps; ++u) {
+          float acc[NT][4] = {};
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            load_scales<PG>(reinterpret_cast<const uint16_t*>(meta + h * M::kBytes) +
-                                (g & (M::kScaleRows - 1)) * PG,
-                            sc[h]);
-            load_zero_points<PG, kZeros>(meta + (2 + h) * M::kBytes + (g & (M::kZeroRows - 1)) * PG,
-                                         zp[h]);
-          }
+          for (int c = 0; c < kCh; ++c) {
+            const uint8_t* at = slot + (u * kCh + c) * (1024 + kMetaSlot);
+            const uint4 w0 = *reinterpret_cast<const uint4*>(at + lane * 16);
+            const uint4 w1 = *reinterpret_cast<const uint4*>(at + lane * 16 + 512);
+            const uint8_t* meta = at + 1024 + g * 4 * M::kBytes;
+            float sc[2][PG], zp[2][PG];
 #pragma unroll
-          for (int gr = 0; gr < PG; ++gr) {
-            float sum[NT][4] = {};
-#pragma unroll
-            for (int j = gr * (4 / PG); j < (gr + 1) * (4 / PG); ++j) {
-              const uint32_t word0 = word_of(w0, j), word1 = word_of(w1, j);
-              uint32_t a[2][4];
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                a[0][q] = code16_pair(word0, q);
-                a[1][q] = code16_pair(word1, q);
-              }
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                mma_16816(sum[nt], a[0][0], a[1][0], a[0][1], a[1][1], xb[c][nt][j].x,
-                          xb[c][nt][j].y);
-                mma_16816(sum[nt], a[0][2], a[1][2], a[0][3], a[1][3], xb[c][nt][j].z,
-                          xb[c][nt][j].w);
-              }
+            for (int h = 0; h < 2; ++h) {
+              load_scales<PG>(reinterpret_cast<const uint16_t*>(meta + h * M::kBytes) +
+                                  (g & (M::kScaleRows - 1)) * PG,
+                              sc[h]);
+              load_zero_points<PG, kZeros>(
+                  meta + (2 + h) * M::kBytes + (g & (M::kZeroRows - 1)) * PG, zp[h]);
             }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int gr = 0; gr < PG; ++gr) {
+              float sum[NT][4] = {};
 #pragma unroll
-              for (int q = 0; q < 4; ++q)
-                acc[nt][q] = fmaf(sc[q >> 1][gr],
-                                  fmaf(-zp[q >> 1][gr], sx[c][gr][nt][q & 1], sum[nt][q]),
-                                  acc[nt][q]);
+              for (int j = gr * (4 / PG); j < (gr + 1) * (4 / PG); ++j) {
+                const uint32_t word0 = word_of(w0, j), word1 = word_of(w1, j);
+                uint32_t a[2][4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  a[0][q] = code16_pair(word0, q);
+                  a[1][q] = code16_pair(word1, q);
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                  mma_16816(sum[nt], a[0][0], a[1][0], a[0][1], a[1][1], xb[c][nt][j].x,
+                            xb[c][nt][j].y);
+                  mma_16816(sum[nt], a[0][2], a[1][2], a[0][3], a[1][3], xb[c][nt][j].z,
+                            xb[c][nt][j].w);
+                }
+              }
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                  acc[nt][q] = fmaf(sc[q >> 1][gr],
+                                    fmaf(-zp[q >> 1][gr], sx[c][gr][nt][q & 1], sum[nt][q]),
+                                    acc[nt][q]);
+            }
           }
+          float* to = mine + (i0 + u) * kTile;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              float* v = to + (8 * nt + (q & 1)) * kColStride + 8 * (q >> 1);
+              *v = pass == 0 ? acc[nt][q] : *v + acc[nt][q];   // the same lane's own sum
+            }
         }
-        float* mine = sums + (wk * p.rt + i) * kTile;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            float* to = mine + (8 * nt + 2 * t + (q & 1)) * kColStride + g + 8 * (q >> 1);
-            *to = pass == 0 ? acc[nt][q] : *to + acc[nt][q];   // the same lane's own sum
-          }
       }
     }
     // one barrier per item: partial sums have two buffers, and a warp cannot be two items ahead
     __syncthreads();
-    if (now.base < 0) {   // an id no weights belong to: recorded, nothing written
+    const int nb = now.nb, base = now.base, tiles_here = min(p.tiles - nb * p.rt, p.rt);
+    step_on(now, item + 1 < item1);
+    if (base < 0) {   // an id no weights belong to: recorded, nothing written
       if (threadIdx.x == 0) record_device_error(p.err, PRISM_MOE_ERR_ARG);
       continue;
     }
     // sum of the kw partial tiles, two outputs per thread, neighbours along the output row
     constexpr int kPairs = kSwiGLU ? 4 : 8;   // output pairs of one row tile
-    const int per_row = now.tiles * kPairs;
+    const int per_row = tiles_here * kPairs;
     for (int i = threadIdx.x; i < rows * per_row; i += nwarps * 32) {
       const int col = i / per_row, pr = i % per_row;
       const int tile = pr / kPairs, r = pr % kPairs * 2;
@@ -339,21 +350,29 @@ int launch_small(SmallParams p, int64_t units, cudaStream_t st) {
   p.kw = static_cast<int>(ceil_div(p.chunks, p.passes * kCh));
   p.rw = std::max(1, kWarps / p.kw);
   const int sms = num_sms();
-  // row tiles per item: several share a barrier, few fill the GPU when the call is small
-  p.rt = p.rw;
-  while (p.rt * 2 <= kMaxRt && units * ceil_div(p.tiles, p.rt * 2) >= 4 * sms) p.rt *= 2;
-  p.blocks_n = static_cast<int>(ceil_div(p.tiles, p.rt));
-  constexpr int kSlot = kCh * (1024 + 32 * Meta<128 / G>::kBytes);
+  // row tiles per item and step: several share a barrier and the bookkeeping, few fill the GPU when
+  // the call is small
+  p.rt = p.rw * kTps;
+  while (p.rt * 2 <= kMaxRt && units * ceil_div(p.tiles, p.rt * 2) >= 2 * sms) p.rt *= 2;
+  constexpr int kSlot = kTps * kCh * (1024 + 32 * Meta<128 / G>::kBytes);
   constexpr int kTile = 8 * NT * kColStride;
+  constexpr int kSmSmem = 233472;   // of one SM, 1 KB of it reserved per block
   const int warps = p.kw * p.rw;
-  const int bytes = warps * kDepth * kSlot + 2 * p.kw * p.rt * kTile * 4 + (p.nseg + 4) / 4 * 16;
-  constexpr int kMaxBytes = kWarps * kDepth * kSlot + 2 * kWarps * kMaxRt * kTile * 4 +
+  auto bytes_of = [&](int rt) {
+    return warps * kDepth * kSlot + 2 * p.kw * rt * kTile * 4 + (p.nseg + 4) / 4 * 16;
+  };
+  // two blocks per SM where shorter items allow it
+  if (NT == 1 && 2 * (bytes_of(p.rt) + 1024) > kSmSmem && p.rt >= 2 * kTps * p.rw) p.rt /= 2;
+  const int bytes = bytes_of(p.rt);
+  p.blocks_n = static_cast<int>(ceil_div(p.tiles, p.rt));
+  constexpr int kMaxBytes = kWarps * kDepth * kSlot + 2 * kWarps * kMaxKwRt * kTile * 4 +
                             (kMaxW4Segments + 4) / 4 * 16;
   static_assert(kMaxBytes <= 232448, "shared memory budget");
   if (int r = ensure_smem_attr(reinterpret_cast<const void*>(kern), kMaxBytes)) return r;
   const int64_t items = units * p.blocks_n;
   PRISM_CHECK_ARG(items < (int64_t(1) << 31), "4-bit product: too many outputs");
-  const int per_sm = std::max(1, std::min({65536 / (128 * 32 * warps), 232448 / (bytes + 1024), 4}));
+  const int per_sm = std::max(
+      1, std::min({65536 / ((NT == 1 ? 128 : 256) * 32 * warps), kSmSmem / (bytes + 1024), 4}));
   const int grid =
       static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(items, per_sm * sms)));
   kern<<<grid, 32 * warps, bytes, st>>>(p);
