@@ -363,8 +363,9 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
 
 }  // namespace
 
-int encode_bf16_map(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
-                    const uint64_t* stride_bytes, const uint32_t* box) {
+int encode_map(CUtensorMap* map, CUtensorMapDataType type, CUtensorMapSwizzle swizzle,
+               const void* base, int rank, const uint64_t* dims, const uint64_t* stride_bytes,
+               const uint32_t* box) {
   auto enc = tensor_map_encoder();
   if (!enc) {
     set_error("cuTensorMapEncodeTiled unavailable from the driver");
@@ -378,14 +379,20 @@ int encode_bf16_map(CUtensorMap* map, const void* base, int rank, const uint64_t
     es[i] = 1;
   }
   for (int i = 0; i < rank - 1; ++i) s[i] = stride_bytes[i];
-  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), d,
-                         s, b, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+  const CUresult r = enc(map, type, rank, const_cast<void*>(base), d, s, b, es,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     set_error("cuTensorMapEncodeTiled failed (CUresult %d, rank %d)", static_cast<int>(r), rank);
     return PRISM_MOE_ERR_CUDA;
   }
   return PRISM_MOE_OK;
+}
+
+int encode_bf16_map(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
+                    const uint64_t* stride_bytes, const uint32_t* box) {
+  return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, CU_TENSOR_MAP_SWIZZLE_128B, base, rank,
+                    dims, stride_bytes, box);
 }
 
 namespace {

@@ -9,7 +9,10 @@
 
 namespace prism {
 
-// Encode a bf16 tensor map with 128-byte swizzle (expert_gemm_sm100.cu).
+// Encode a tensor map; the bf16 form has the 128-byte swizzle (expert_gemm_sm100.cu).
+int encode_map(CUtensorMap* map, CUtensorMapDataType type, CUtensorMapSwizzle swizzle,
+               const void* base, int rank, const uint64_t* dims, const uint64_t* stride_bytes,
+               const uint32_t* box);
 int encode_bf16_map(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
                     const uint64_t* stride_bytes, const uint32_t* box);
 

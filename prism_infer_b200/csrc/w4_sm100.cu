@@ -12,10 +12,13 @@
 // Warp roles (512 threads, one CTA per SM, persistent over a device-side tile list):
 //   warp 0        TMA of the activation rows (64 inputs x 64 rows per copy, 128-byte swizzle)
 //   warp 1        TMEM owner and MMA issuer
-//   warp 2        bulk copies of packed weights, 128 inputs of 8 row tiles (1 KB each) per slot, and
-//                 of their zero points
-//   warp 3        bulk copies of scales, 128 inputs of 8 row tiles per slot (their readers run up to
-//                 two chunks behind the decoders, so they have a ring of their own)
+//   warp 2        TMA of packed weights, 128 inputs of 8 row tiles (1 KB each) per copy, and of their
+//                 zero points
+//   warp 3        TMA of scales, 128 inputs of 8 row tiles per copy (their readers run up to two
+//                 chunks behind the decoders, so they have a ring of their own)
+//                 These four run their loops as whole warps and elect a lane for the copy or MMA, so
+//                 that its operands are uniform registers; in a one-lane branch each had to be moved
+//                 there, and issuing a stage took longer than its products.
 //   warps 4-7     decode: 16 bytes (four words) per lane and row -> K-major, swizzled bf16 A tile
 //   warps 8-15    accumulate: two warps per TMEM lane quarter, each half of the columns; a lane owns
 //                 one weight row, so a group's scale is one register
@@ -34,30 +37,42 @@ namespace prism {
 namespace {
 
 constexpr int kRowsW = 128;      // weight rows per tile
-constexpr int kTok = 256;        // activation rows per tile, at most
+constexpr int kNarrowRows = 64;  // average rows per segment up to which tiles are narrow
 constexpr int kTokBox = 64;      // activation rows per copy
-constexpr int kAStage = kRowsW * kBK * 2;
-constexpr int kBStage = kTok * kBK * 2;
-constexpr int kStage = kAStage + kBStage;
-constexpr int kNumStages = 4;
 constexpr int kPackStage = 8 * 1024;
-constexpr int kPackStages = 3;
 constexpr int kThreadsW4 = 512;
-constexpr int kMaxScaleSlots = 8;
 constexpr size_t kPrefixW4 = ((kMaxW4Segments + 1) * 4 + 15) / 16 * 16;
 
+// The two shapes: 256 activation rows (many rows per segment: one decoding serves them all) or 64
+// (tens of rows: short stages and more of them keep enough weights in flight to follow HBM, and twice
+// the decoding warps).
+template <bool kNarrow>
+struct Shape {
+  static constexpr int kTok = kNarrow ? 64 : 256;        // activation rows per tile, at most
+  static constexpr int kAStage = kRowsW * kBK * 2;
+  static constexpr int kStage = kAStage + kTok * kBK * 2;
+  static constexpr int kStages = kNarrow ? 6 : 4;
+  static constexpr int kPackStages = kNarrow ? 6 : 3;
+  static constexpr int kDecWarps = kNarrow ? 8 : 4;
+  static constexpr int kAccWarps = kNarrow ? 4 : 8;
+  static constexpr int kBufs = kNarrow ? 4 : 2;          // TMEM buffers, one group each
+  static constexpr uint32_t kTmem = kBufs * kTok;        // TMEM columns
+};
+
 // Shared memory after the stages: packed slots, zero-point slots, scale slots, barriers, prefix.
-template <int G>
+template <int G, bool kNarrow>
 struct Smem {
+  using P = Shape<kNarrow>;
   static constexpr int kPG = 128 / G;                 // groups per chunk
   static constexpr int kZeroSlot = kRowsW * kPG;      // bytes
   static constexpr int kScaleSlot = kRowsW * kPG * 2;
-  static constexpr int kScaleSlots = kPG == 4 ? 4 : kMaxScaleSlots;
-  static constexpr int kPacked = kNumStages * kStage;
-  static constexpr int kZeros = kPacked + kPackStages * kPackStage;
-  static constexpr int kScales = kZeros + kPackStages * kZeroSlot;
+  static constexpr int kScaleSlots = kPG == 4 && !kNarrow ? 4 : 8;
+  static constexpr int kPacked = P::kStages * P::kStage;
+  static constexpr int kZeros = kPacked + P::kPackStages * kPackStage;
+  static constexpr int kScales = kZeros + P::kPackStages * kZeroSlot;
   static constexpr int kBars = kScales + kScaleSlots * kScaleSlot;
-  static constexpr int kPrefix = kBars + 320;
+  static constexpr int kNumBars = 2 * (P::kStages + P::kPackStages + kScaleSlots + P::kBufs) + 1;
+  static constexpr int kPrefix = kBars + (kNumBars * 8 + 8 + 15) / 16 * 16;
   static constexpr int kBytes = 1024 + kPrefix + static_cast<int>(kPrefixW4);
   static_assert(kBytes <= 232448, "shared memory budget");
 };
@@ -76,14 +91,6 @@ struct LargeParams {
   uint64_t wait_ns;
 };
 
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes,
-                                          uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-          smem_u32(dst)),
-      "l"(src), "r"(bytes), "r"(smem_u32(bar))
-      : "memory");
-}
 __device__ __forceinline__ void fence_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
@@ -104,8 +111,8 @@ __device__ __forceinline__ void fma2(float2& a, uint32_t v0, uint32_t v1, uint64
 }
 
 // acc[0 .. 32 kBatches) += s * (the accumulator's columns from ``taddr``), 32 columns per wait.
-template <int kBatches>
-__device__ __forceinline__ void add_scaled(float2 (&acc)[64], uint32_t taddr, float s) {
+template <int kBatches, int kPairs>
+__device__ __forceinline__ void add_scaled(float2 (&acc)[kPairs], uint32_t taddr, float s) {
   const float2 s2 = make_float2(s, s);
   const uint64_t ss = *reinterpret_cast<const uint64_t*>(&s2);
 #pragma unroll
@@ -120,78 +127,199 @@ __device__ __forceinline__ void add_scaled(float2 (&acc)[64], uint32_t taddr, fl
   }
 }
 
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok));
+  return ok != 0;
+}
+// Barriers, copies and accesses by shared-memory address.
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, uint32_t abort,
+                                         uint64_t limit_ns) {
+  if (bar_try(bar, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
+  while (true) {
+    if (bar_try(bar, parity)) return true;
+    if (lds32(abort)) return false;
+    if (global_timer_ns() - t0 > limit_ns) return false;
+  }
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void bar_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void copy_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0,
+                                        int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void copy_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0,
+                                        int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts128(uint32_t addr, const uint4& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z),
+               "r"(v.w)
+               : "memory");
+}
+// kBytes (1, 2, 4 or 8) at ``addr``, low bytes first.
+template <int kBytes>
+__device__ __forceinline__ uint2 lds_small(uint32_t addr) {
+  uint2 v = make_uint2(0, 0);
+  if constexpr (kBytes == 8)
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  else if constexpr (kBytes == 4)
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v.x) : "r"(addr) : "memory");
+  else if constexpr (kBytes == 2)
+    asm volatile("{\n\t.reg .u16 h;\n\tld.shared.u16 h, [%1];\n\tcvt.u32.u16 %0, h;\n\t}"
+                 : "=r"(v.x)
+                 : "r"(addr)
+                 : "memory");
+  else
+    asm volatile("{\n\t.reg .u16 h;\n\tld.shared.u8 h, [%1];\n\tcvt.u32.u16 %0, h;\n\t}"
+                 : "=r"(v.x)
+                 : "r"(addr)
+                 : "memory");
+  return v;
+}
+
 struct Tile {
-  int sg, e, mt;        // segment, matrix, M tile
-  int64_t row0;         // first activation row
+  int e, mt;            // matrix, M tile
+  int row0;             // first activation row
   int rows, cols;       // valid activation rows; MMA N (a multiple of 16)
+  int c0;               // first chunk: tiles that share activations start at different ones
+  int64_t begin, end;   // before finish(): the segment's rows as the table has them
+  int part, parts;      //                  this tile's part of them
 };
 
-__device__ __forceinline__ Tile tile_at(const LargeParams& p, const int32_t* prefix, int64_t item) {
+// A tile is looked up one ahead: the loads are issued by look_up and used by finish.
+__device__ __forceinline__ Tile look_up(const LargeParams& p, const int32_t* prefix, int item) {
   Tile t;
-  const int unit = static_cast<int>(item / p.tiles_n);
-  t.mt = static_cast<int>(item % p.tiles_n);
-  t.sg = find_segment(prefix, p.nseg, unit);
-  const RowSpan span = segment_rows(p.seg_offsets, t.sg, p.rows_cap);
+  const int unit = item / p.tiles_n;
+  t.mt = item % p.tiles_n;
+  const int sg = find_segment(prefix, p.nseg, unit);
+  t.part = unit - prefix[sg];
+  t.parts = prefix[sg + 1] - prefix[sg];
+  t.begin = p.seg_offsets ? p.seg_offsets[sg] : 0;
+  t.end = p.seg_offsets ? p.seg_offsets[sg + 1] : p.rows_cap;
+  t.e = p.seg_expert ? p.seg_expert[sg] : (p.num_mats == 1 ? 0 : sg);
+  return t;
+}
+__device__ __forceinline__ Tile finish(const LargeParams& p, Tile t) {
+  const int begin = static_cast<int>(max(t.begin, static_cast<int64_t>(0)));
+  const int end = static_cast<int>(min(t.end, p.rows_cap));
   // a segment's rows in equal parts, each a multiple of 16
-  const int parts = prefix[t.sg + 1] - prefix[t.sg];
-  const int64_t len = span.end - span.begin;
-  const int64_t per = ((len + parts - 1) / parts + 15) / 16 * 16;
-  t.row0 = span.begin + (unit - prefix[t.sg]) * per;
-  t.rows = static_cast<int>(max(static_cast<int64_t>(0), min(per, span.end - t.row0)));
+  const int per = ((end - begin + t.parts - 1) / t.parts + 15) / 16 * 16;
+  t.row0 = begin + t.part * per;
+  t.rows = max(0, min(per, end - t.row0));
   t.cols = max(16, (t.rows + 15) / 16 * 16);
-  t.e = p.seg_expert ? p.seg_expert[t.sg] : (p.num_mats == 1 ? 0 : t.sg);
+  t.c0 = static_cast<int>(static_cast<int64_t>(t.mt) * p.chunks / p.tiles_n);
   return t;
 }
 
-template <int G, bool kZeros, bool kSwiGLU>
+// Ring position: slot and phase.
+template <int kSlots>
+struct Ring {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++slot == kSlots) {
+      slot = 0;
+      phase ^= 1;
+    }
+  }
+};
+
+template <int G, bool kZeros, bool kSwiGLU, bool kNarrow>
 __global__ void __launch_bounds__(kThreadsW4, 1)
-    w4_large_kernel(const __grid_constant__ CUtensorMap tmap_x, const LargeParams p) {
-  using S = Smem<G>;
+    w4_large_kernel(const __grid_constant__ CUtensorMap map_x,
+                    const __grid_constant__ CUtensorMap map_q,
+                    const __grid_constant__ CUtensorMap map_s,
+                    const __grid_constant__ CUtensorMap map_z, const LargeParams p) {
+  using P = Shape<kNarrow>;
+  using S = Smem<G, kNarrow>;
   constexpr int PG = S::kPG;
+  constexpr int kTok = P::kTok, kStage = P::kStage, kAStage = P::kAStage;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  uint8_t* packed = smem + S::kPacked;
-  uint8_t* zeros = smem + S::kZeros;
-  uint8_t* scales = smem + S::kScales;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBars);
-  uint64_t* empty = full + kNumStages;
-  uint64_t* pk_full = empty + kNumStages;
-  uint64_t* pk_empty = pk_full + kPackStages;
-  uint64_t* sc_full = pk_empty + kPackStages;
-  uint64_t* sc_empty = sc_full + kMaxScaleSlots;
-  uint64_t* acc_full = sc_empty + kMaxScaleSlots;
-  uint64_t* acc_empty = acc_full + 2;
-  uint64_t* drain = acc_empty + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
-  volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int32_t* prefix = reinterpret_cast<int32_t*>(smem + S::kPrefix);
+  const uint32_t base = smem_u32(smem);
+  const uint32_t packed = base + S::kPacked, zeros = base + S::kZeros, scales = base + S::kScales;
+  const uint32_t full = base + S::kBars, empty = full + 8 * P::kStages;
+  const uint32_t pk_full = empty + 8 * P::kStages, pk_empty = pk_full + 8 * P::kPackStages;
+  const uint32_t sc_full = pk_empty + 8 * P::kPackStages, sc_empty = sc_full + 8 * S::kScaleSlots;
+  const uint32_t acc_full = sc_empty + 8 * S::kScaleSlots, acc_empty = acc_full + 8 * P::kBufs;
+  const uint32_t drain = acc_empty + 8 * P::kBufs, abort = drain + 12;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (drain - base) + 8);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + (abort - base));
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kNumStages; ++s) {
-      mbar_init(&full[s], 1 + 4);   // the copies' arrival and four decoding warps
-      mbar_init(&empty[s], 1);
-    }
-    for (int s = 0; s < kPackStages; ++s) {
-      mbar_init(&pk_full[s], 1);
-      mbar_init(&pk_empty[s], 4);
-    }
-    for (int i = 0; i < S::kScaleSlots; ++i) {
-      mbar_init(&sc_full[i], 1);
-      mbar_init(&sc_empty[i], 8);
-    }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 8);
-    }
-    mbar_init(drain, 1);
-    *abort = 0;
+    auto init = [&](uint32_t bar, int n, int count) {
+      for (int i = 0; i < n; ++i)
+        mbar_init(reinterpret_cast<uint64_t*>(smem + (bar - base)) + i, count);
+    };
+    init(full, P::kStages, 1 + P::kDecWarps);   // the copies' arrival and the decoding warps
+    init(empty, P::kStages, 1);
+    init(pk_full, P::kPackStages, 1);
+    init(pk_empty, P::kPackStages, P::kDecWarps);
+    init(sc_full, S::kScaleSlots, 1);
+    init(sc_empty, S::kScaleSlots, P::kAccWarps);
+    init(acc_full, P::kBufs, 1);
+    init(acc_empty, P::kBufs, P::kAccWarps);
+    init(drain, 1, 1);
+    *abort_flag = 0;
     fence_mbar_init();
-    tma_prefetch_desc(&tmap_x);
+    tma_prefetch_desc(&map_x);
+    tma_prefetch_desc(&map_q);
+    tma_prefetch_desc(&map_s);
+    if (kZeros) tma_prefetch_desc(&map_z);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, kTmemCols);
+    tmem_alloc(tmem_slot, P::kTmem);
     tmem_relinquish();
   }
   if (warp == 2) build_row_blocks(p.seg_offsets, p.nseg, p.rows_cap, kTok, prefix, p.min_rows);
@@ -199,275 +327,236 @@ __global__ void __launch_bounds__(kThreadsW4, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const int64_t total = static_cast<int64_t>(prefix[p.nseg]) * p.tiles_n;
+  const int total = prefix[p.nseg] * p.tiles_n;
   auto give_up = [&]() {
-    *abort = 1;
+    *abort_flag = 1;
     record_device_error(p.err, PRISM_MOE_ERR_TIMEOUT);
   };
-  auto usable = [&](const Tile& t) { return t.e >= 0 && t.e < p.num_mats && t.rows > 0; };
+  // ``body(tile)`` for every tile of this CTA, false to stop; tiles whose segment names no expert are
+  // left out by every role alike
+  auto for_tiles = [&](auto body) {
+    bool ok = true;
+    Tile next;
+    if (blockIdx.x < total) next = look_up(p, prefix, blockIdx.x);
+    for (int item = blockIdx.x; ok && item < total;) {
+      const Tile t = finish(p, next);
+      item += gridDim.x;
+      if (item < total) next = look_up(p, prefix, item);
+      if (t.e >= 0 && t.e < p.num_mats && t.rows > 0)
+        ok = body(t);
+      else if (warp == 2 && lane == 0 && t.rows > 0)
+        record_device_error(p.err, PRISM_MOE_ERR_ARG);
+    }
+    return ok;
+  };
+  auto next_chunk = [&](int c) { return c + 1 == p.chunks ? 0 : c + 1; };
+  auto wait = [&](uint32_t bar, uint32_t parity) { return bar_wait(bar, parity, abort, p.wait_ns); };
 
   if (warp < 4) {
-    reg_dealloc<40>();
-    if (warp == 0 && lane == 0) {
+    if constexpr (!kNarrow) reg_dealloc<40>();
+    bool ok = true;
+    if (warp == 0) {
       // ---------------------------------------------------------------- activation rows
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int64_t item = blockIdx.x; ok && item < total; item += gridDim.x) {
-        const Tile t = tile_at(p, prefix, item);
-        if (!usable(t)) continue;
+      Ring<P::kStages> st;
+      ok = for_tiles([&](const Tile& t) {
         const int boxes = (t.cols + kTokBox - 1) / kTokBox;
-        for (int kb = 0; kb < p.num_kb; ++kb) {
-          if (!mbar_wait_bounded(&empty[stage], phase ^ 1, abort, p.wait_ns)) {
-            ok = false;
-            break;
+        for (int i = 0, c = t.c0; i < p.chunks; ++i, c = next_chunk(c))
+          for (int kb = 2 * c; kb < min(2 * c + 2, p.num_kb); ++kb) {
+            if (!__all_sync(0xffffffffu, wait(empty + 8 * st.slot, st.phase ^ 1))) return false;
+            if (elect_one()) {
+              bar_expect(full + 8 * st.slot, boxes * kTokBox * kBK * 2);
+              const uint32_t b = base + st.slot * kStage + kAStage;
+              for (int x = 0; x < boxes; ++x)
+                copy_2d(b + x * kTokBox * kBK * 2, &map_x, full + 8 * st.slot, kb * kBK,
+                        t.row0 + x * kTokBox);
+            }
+            __syncwarp();
+            st.next();
           }
-          mbar_arrive_expect_tx(&full[stage], boxes * kTokBox * kBK * 2);
-          uint8_t* b = smem + stage * kStage + kAStage;
-          for (int i = 0; i < boxes; ++i)
-            tma_load_2d(b + i * kTokBox * kBK * 2, &tmap_x, &full[stage], kb * kBK,
-                        static_cast<int32_t>(t.row0) + i * kTokBox);
-          if (++stage == kNumStages) {
-            stage = 0;
-            phase ^= 1;
-          }
-        }
-      }
-      if (!ok) give_up();
-    } else if (warp == 1 && lane == 0) {
+        return true;
+      });
+    } else if (warp == 1) {
       // ---------------------------------------------------------------- MMA issuer
-      int stage = 0, buf = 0;
-      uint32_t phase = 0, acc_phase = 0;
-      bool ok = true;
-      for (int64_t item = blockIdx.x; ok && item < total; item += gridDim.x) {
-        const Tile t = tile_at(p, prefix, item);
-        if (!usable(t)) continue;
+      Ring<P::kStages> st;
+      Ring<P::kBufs> buf;
+      const uint64_t desc_a = smem_desc_sw128(base), desc_b = smem_desc_sw128(base + kAStage);
+      ok = for_tiles([&](const Tile& t) {
         const uint32_t idesc = idesc_bf16_f32(kRowsW, t.cols);
-        for (int kb = 0; ok && kb < p.num_kb; ++kb) {
-          if (!mbar_wait_bounded(&full[stage], phase, abort, p.wait_ns)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t a0 = smem_u32(smem + stage * kStage), b0 = a0 + kAStage;
+        for (int i = 0, c = t.c0; i < p.chunks; ++i, c = next_chunk(c)) {
+          const int kb_end = min(2 * c + 2, p.num_kb);
+          for (int kb = 2 * c; kb < kb_end; ++kb) {
+            if (!__all_sync(0xffffffffu, wait(full + 8 * st.slot, st.phase))) return false;
+            const uint32_t off = st.slot * (kStage >> 4);
 #pragma unroll
-          for (int kk = 0; kk < kBK / 16; ++kk) {
-            // a new group starts: its buffer must have been read
-            const bool first = G == 128 ? (kb & 1) == 0 && kk == 0 : (kk * 16) % G == 0;
-            if (first) {
-              if (!mbar_wait_bounded(&acc_empty[buf], acc_phase ^ 1, abort, p.wait_ns)) {
-                ok = false;
-                break;
-              }
+            for (int k0 = 0; k0 < 4; k0 += (G == 32 ? 2 : 4)) {   // the 16-input steps of one group
+              // a new group starts: its buffer must have been read
+              const bool first = G != 128 || kb == 2 * c;
+              if (first && !__all_sync(0xffffffffu, wait(acc_empty + 8 * buf.slot, buf.phase ^ 1)))
+                return false;
               tc_fence_after();
+              const bool last = G != 128 || kb + 1 == kb_end;
+              if (elect_one()) {
+#pragma unroll
+                for (int kk = k0; kk < k0 + (G == 32 ? 2 : 4); ++kk)
+                  tc_mma_bf16(tmem_base + buf.slot * kTok, desc_a + off + kk * 2,
+                              desc_b + off + kk * 2, idesc, first && kk == k0 ? 0u : 1u);
+                if (last) bar_commit(acc_full + 8 * buf.slot);
+                if (k0 + (G == 32 ? 2 : 4) == 4) bar_commit(empty + 8 * st.slot);
+              }
+              __syncwarp();
+              if (last) buf.next();
             }
-            tc_mma_bf16(tmem_base + buf * kTok, smem_desc_sw128(a0 + kk * 32),
-                        smem_desc_sw128(b0 + kk * 32), idesc, first ? 0u : 1u);
-            const bool last = G == 128 ? ((kb & 1) == 1 || kb + 1 == p.num_kb) && kk == 3
-                                       : (kk * 16 + 16) % G == 0;
-            if (last) {
-              tc_commit(&acc_full[buf]);
-              buf ^= 1;
-              acc_phase ^= buf == 0 ? 1u : 0u;
-            }
-          }
-          if (!ok) break;
-          tc_commit(&empty[stage]);
-          if (++stage == kNumStages) {
-            stage = 0;
-            phase ^= 1;
+            st.next();
           }
         }
-      }
-      if (!ok) give_up();
-      if (*abort) {
-        tc_commit(drain);   // completes once every MMA issued above has finished
-        volatile int never = 0;
-        mbar_wait_bounded(drain, 0, &never, kDrainNs);
+        return true;
+      });
+      if (!ok && lane == 0) give_up();
+      __syncwarp();
+      if (*abort_flag) {
+        if (elect_one()) bar_commit(drain);   // completes once every MMA issued above has finished
+        __syncwarp();
+        const uint64_t t0 = global_timer_ns();
+        while (!bar_try(drain, 0) && global_timer_ns() - t0 < kDrainNs) {
+        }
       }
     } else if (warp == 2) {
       // ---------------------------------------------------------------- packed weights
-      int slot = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int64_t item = blockIdx.x; ok && item < total; item += gridDim.x) {
-        const Tile t = tile_at(p, prefix, item);
-        if (!usable(t)) {
-          if (lane == 0 && t.rows > 0) record_device_error(p.err, PRISM_MOE_ERR_ARG);
-          continue;
-        }
-        const int valid = min(8, p.tiles - t.mt * 8);
-        const int64_t first = (static_cast<int64_t>(t.e) * p.tiles + t.mt * 8 + lane) * p.chunks;
-        for (int c = 0; c < p.chunks; ++c) {
-          ok = mbar_wait_bounded(&pk_empty[slot], phase ^ 1, abort, p.wait_ns);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          constexpr int zb = kZeros ? 16 * PG : 0;   // zero points of one row tile
-          if (lane == 0) mbar_arrive_expect_tx(&pk_full[slot], valid * (1024 + zb));
+      Ring<P::kPackStages> pk;
+      ok = for_tiles([&](const Tile& t) {
+        const int tile0 = t.e * p.tiles + t.mt * 8;
+        for (int i = 0, c = t.c0; i < p.chunks; ++i, c = next_chunk(c), pk.next()) {
+          if (!__all_sync(0xffffffffu, wait(pk_empty + 8 * pk.slot, pk.phase ^ 1))) return false;
+          if (elect_one()) {
+            const uint32_t bar = pk_full + 8 * pk.slot;
+            bar_expect(bar, kPackStage + (kZeros ? S::kZeroSlot : 0));
+            copy_3d(packed + pk.slot * kPackStage, &map_q, bar, 0, c, tile0);
+            if constexpr (kZeros) copy_3d(zeros + pk.slot * S::kZeroSlot, &map_z, bar, 0, c, tile0);
+          }
           __syncwarp();
-          if (lane < valid) {
-            bulk_load(packed + slot * kPackStage + lane * 1024, p.q + (first + c) * 1024, 1024,
-                      &pk_full[slot]);
-            if constexpr (kZeros)
-              bulk_load(zeros + slot * S::kZeroSlot + lane * zb, p.z + (first + c) * zb, zb,
-                        &pk_full[slot]);
-          }
-          if (++slot == kPackStages) {
-            slot = 0;
-            phase ^= 1;
-          }
         }
-      }
-      if (!ok && lane == 0) give_up();
-    } else if (warp == 3) {
+        return true;
+      });
+    } else {
       // ---------------------------------------------------------------- scales
-      int slot = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      constexpr int bytes = 32 * PG;   // of one row tile and chunk
-      for (int64_t item = blockIdx.x; ok && item < total; item += gridDim.x) {
-        const Tile t = tile_at(p, prefix, item);
-        if (!usable(t)) continue;
-        const int valid = min(8, p.tiles - t.mt * 8);
-        const int64_t first = (static_cast<int64_t>(t.e) * p.tiles + t.mt * 8 + lane) * p.chunks;
-        for (int c = 0; c < p.chunks; ++c) {
-          ok = mbar_wait_bounded(&sc_empty[slot], phase ^ 1, abort, p.wait_ns);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(&sc_full[slot], valid * bytes);
-          __syncwarp();
-          if (lane < valid)
-            bulk_load(scales + slot * S::kScaleSlot + lane * bytes,
-                      reinterpret_cast<const uint8_t*>(p.s) + (first + c) * bytes, bytes,
-                      &sc_full[slot]);
-          if (++slot == S::kScaleSlots) {
-            slot = 0;
-            phase ^= 1;
+      Ring<S::kScaleSlots> sc;
+      ok = for_tiles([&](const Tile& t) {
+        for (int i = 0, c = t.c0; i < p.chunks; ++i, c = next_chunk(c), sc.next()) {
+          if (!__all_sync(0xffffffffu, wait(sc_empty + 8 * sc.slot, sc.phase ^ 1))) return false;
+          if (elect_one()) {
+            bar_expect(sc_full + 8 * sc.slot, S::kScaleSlot);
+            copy_3d(scales + sc.slot * S::kScaleSlot, &map_s, sc_full + 8 * sc.slot, 0, c,
+                    t.e * p.tiles + t.mt * 8);
           }
+          __syncwarp();
         }
-      }
-      if (!ok && lane == 0) give_up();
+        return true;
+      });
     }
-  } else if (warp < 8) {
+    if (!ok && lane == 0) give_up();
+  } else if (warp < 8 || (kNarrow && warp >= 12)) {
     // ------------------------------------------------------------------ decode
-    reg_dealloc<88>();
-    const int w = warp - 4, g = lane >> 2, tq = lane & 3;
+    if constexpr (!kNarrow) reg_dealloc<88>();
+    constexpr int kTiles = 8 / P::kDecWarps;   // row tiles per warp
+    const int w = warp < 8 ? warp - 4 : warp - 8, g = lane >> 2, tq = lane & 3;
     const bool odd = g & 1;
-    int stage = 0, slot = 0;
-    uint32_t phase = 0, pk_phase = 0;
-    bool ok = true;
-    for (int64_t item = blockIdx.x; ok && item < total; item += gridDim.x) {
-      const Tile t = tile_at(p, prefix, item);
-      if (!usable(t)) continue;
-      for (int c = 0; ok && c < p.chunks; ++c) {
-        ok = mbar_wait_bounded(&pk_full[slot], pk_phase, abort, p.wait_ns);
-        if (!ok) break;
-        // rows g and g + 8 of row tiles 2 w and 2 w + 1
-        uint32_t zr[4][PG];
+    Ring<P::kStages> st;
+    Ring<P::kPackStages> pk;
+    // this lane's row g of the warp's first row tile: packed bytes, zero points, place in the A tile
+    const uint32_t from = packed + kTiles * w * 1024 + lane * 16;
+    const uint32_t zfrom = zeros + (kTiles * w * 16 + g) * PG;
+    const uint32_t to = base + kTiles * w * 2048 + g * 128;
+    const uint32_t at0 = ((odd ? 4 : 0) + tq) ^ g, at1 = ((odd ? 0 : 4) + tq) ^ g;
+    const bool ok = for_tiles([&](const Tile& t) {
+      for (int i = 0, c = t.c0; i < p.chunks; ++i, c = next_chunk(c)) {
+        if (!__all_sync(0xffffffffu, wait(pk_full + 8 * pk.slot, pk.phase))) return false;
+        // rows g and g + 8 of this warp's row tiles
+        uint32_t zr[2 * kTiles][PG];
+        uint4 v[2 * kTiles];
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          load_zeros<PG, kZeros>(zeros + slot * S::kZeroSlot,
-                                 ((2 * w + (r >> 1)) * 16 + g + 8 * (r & 1)) * PG, zr[r]);
-        uint4 v[4];
+        for (int r = 0; r < 2 * kTiles; ++r) {
+          v[r] = lds128(from + pk.slot * kPackStage + r * 512);
+          uint32_t z = 0x08080808u;
+          if constexpr (kZeros) z = lds_small<PG>(zfrom + pk.slot * S::kZeroSlot + r * 8 * PG).x;
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          v[r] = *reinterpret_cast<const uint4*>(packed + slot * kPackStage + (2 * w + (r >> 1)) * 1024 +
-                                                 (r & 1) * 512 + lane * 16);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&pk_empty[slot]);
-        if (++slot == kPackStages) {
-          slot = 0;
-          pk_phase ^= 1;
+          for (int j = 0; j < PG; ++j)
+            zr[r][j] = kZeros ? (((z >> (8 * j)) & 0xfu) * 0x00010001u) | 0x43004300u : 0x43084308u;
         }
+        __syncwarp();
+        if (lane == 0) bar_arrive(pk_empty + 8 * pk.slot);
+        pk.next();
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           if (2 * c + half >= p.num_kb) break;
-          ok = mbar_wait_bounded(&empty[stage], phase ^ 1, abort, p.wait_ns);
-          if (!ok) break;
-          uint8_t* a = smem + stage * kStage;
+          if (!__all_sync(0xffffffffu, wait(empty + 8 * st.slot, st.phase ^ 1))) return false;
+          const uint32_t a = to + st.slot * kStage;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int row = (2 * w + (r >> 1)) * 16 + (r & 1) * 8 + g;
-            uint8_t* arow = a + (row >> 3) * 1024 + (row & 7) * 128;
+          for (int r = 0; r < 2 * kTiles; ++r) {
             // lanes of odd rows take the two words in the other order: their 16-byte stores then
             // fall into the other half of the banks
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const uint32_t w0 = word_of(v[r], 2 * half + i), w1 = word_of(v[r], 2 * half + 1 - i);
+            for (int i2 = 0; i2 < 2; ++i2) {
+              const uint32_t w0 = word_of(v[r], 2 * half + i2), w1 = word_of(v[r], 2 * half + 1 - i2);
               const uint32_t word = odd ? w1 : w0;
-              const int jj = odd ? 1 - i : i;
               uint32_t zero = zr[r][0];
               if constexpr (PG == 2) zero = zr[r][half];
-              if constexpr (PG == 4) zero = odd ? zr[r][2 * half + 1 - i] : zr[r][2 * half + i];
-              const uint4 d = make_uint4(code_pair(word, 0, zero), code_pair(word, 1, zero),
-                                         code_pair(word, 2, zero), code_pair(word, 3, zero));
-              *reinterpret_cast<uint4*>(arow + (((4 * jj + tq) ^ g) << 4)) = d;
+              if constexpr (PG == 4) zero = odd ? zr[r][2 * half + 1 - i2] : zr[r][2 * half + i2];
+              sts128(a + r * 1024 + ((i2 ? at1 : at0) << 4),
+                     make_uint4(code_pair(word, 0, zero), code_pair(word, 1, zero),
+                                code_pair(word, 2, zero), code_pair(word, 3, zero)));
             }
           }
           fence_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&full[stage]);
-          if (++stage == kNumStages) {
-            stage = 0;
-            phase ^= 1;
-          }
+          if (lane == 0) bar_arrive(full + 8 * st.slot);
+          st.next();
         }
       }
-    }
-    if (!ok) give_up();
+      return true;
+    });
+    if (!ok && lane == 0) give_up();
   } else {
     // ------------------------------------------------------------------ accumulate
-    reg_alloc<192>();
-    const int q = warp & 3, side = (warp - 8) >> 2;
-    int buf = 0;
-    uint32_t acc_phase = 0;
-    bool ok = true;
-    int slot = 0;
-    uint32_t sc_phase = 0;
+    if constexpr (!kNarrow) reg_alloc<192>();
+    const int q = warp & 3, side = (warp - 8) >> 2;   // narrow: one side, all columns
+    constexpr int kPairs = kNarrow ? 32 : 64;          // pairs of columns held, at most
+    Ring<P::kBufs> buf;
+    Ring<S::kScaleSlots> sl;
+    const int row = q * 32 + lane;                     // weight row in the tile
     const int groups = G == 128 ? p.chunks : p.num_kb * (G == 32 ? 2 : 1);
-    for (int64_t item = blockIdx.x; ok && item < total; item += gridDim.x) {
-      const Tile t = tile_at(p, prefix, item);
-      if (!usable(t)) continue;
-      const int left = (t.cols / 16 + 1) / 2 * 16;            // columns of side 0
+    const bool ok = for_tiles([&](const Tile& t) {
+      const int left = kNarrow ? t.cols : (t.cols / 16 + 1) / 2 * 16;   // columns of side 0
       const int col0 = side ? left : 0, ncols = side ? t.cols - left : left;
-      const int row = q * 32 + lane;                          // weight row in the tile
-      float2 acc[64];
+      float2 acc[kPairs];
 #pragma unroll
-      for (int i = 0; i < 64; ++i) acc[i] = make_float2(0.f, 0.f);
+      for (int i = 0; i < kPairs; ++i) acc[i] = make_float2(0.f, 0.f);
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + col0;
-      for (int c = 0; ok && c < p.chunks; ++c) {
-        ok = mbar_wait_bounded(&sc_full[slot], sc_phase, abort, p.wait_ns);
-        if (!ok) break;
-        float sc[PG];
-        load_scales<PG>(reinterpret_cast<const uint16_t*>(scales + slot * S::kScaleSlot) + row * PG, sc);
+      for (int i = 0, c = t.c0; i < p.chunks; ++i, c = next_chunk(c)) {
+        if (!__all_sync(0xffffffffu, wait(sc_full + 8 * sl.slot, sl.phase))) return false;
+        const uint2 raw = lds_small<2 * PG>(scales + sl.slot * S::kScaleSlot + row * 2 * PG);
+        const float sc[4] = {__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xffff0000u),
+                             __uint_as_float(raw.y << 16), __uint_as_float(raw.y & 0xffff0000u)};
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sc_empty[slot]);
-        if (++slot == S::kScaleSlots) {
-          slot = 0;
-          sc_phase ^= 1;
-        }
+        if (lane == 0) bar_arrive(sc_empty + 8 * sl.slot);
+        sl.next();
 #pragma unroll
         for (int gr = 0; gr < PG; ++gr) {
-          if (c * PG + gr >= groups) break;
-          ok = mbar_wait_bounded(&acc_full[buf], acc_phase, abort, p.wait_ns);
-          if (!ok) break;
+          if (c * PG + gr >= groups) break;   // the last chunk of an odd number of 64-input blocks
+          if (!__all_sync(0xffffffffu, wait(acc_full + 8 * buf.slot, buf.phase))) return false;
           tc_fence_after();
-          __syncwarp();
-          const uint32_t at = taddr + buf * kTok;
-          // few columns, or all 128 of this side (those past ncols hold what an earlier tile left
-          // there and are never stored)
+          const uint32_t at = taddr + buf.slot * kTok;
+          // few columns, or all 128 (64) of this side (those past ncols hold what an earlier tile
+          // left there and are never stored)
           if (ncols > 32)
-            add_scaled<4>(acc, at, sc[gr]);
+            add_scaled<kPairs / 16>(acc, at, sc[gr]);
           else if (ncols > 0)
             add_scaled<1>(acc, at, sc[gr]);
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&acc_empty[buf]);
-          buf ^= 1;
-          acc_phase ^= buf == 0 ? 1u : 0u;
+          if (lane == 0) bar_arrive(acc_empty + 8 * buf.slot);
+          buf.next();
         }
       }
-      if (!ok) break;
       // ---- output: lanes are consecutive outputs of one activation row
       const int64_t ld = p.n_out;
       if constexpr (kSwiGLU) {
@@ -476,7 +565,7 @@ __global__ void __launch_bounds__(kThreadsW4, 1)
         const bool up = lane & 8;
         const int n = (t.mt * kRowsW + q * 32) / 2 + (lane >> 4) * 8 + (lane & 7);
 #pragma unroll
-        for (int i = 0; i < 64; ++i) {
+        for (int i = 0; i < kPairs; ++i) {
           if (2 * i >= ncols) break;
           const float got = __shfl_xor_sync(0xffffffffu, up ? acc[i].x : acc[i].y, 8);
           const float h = up ? silu_mul(got, acc[i].y) : silu_mul(acc[i].x, got);
@@ -488,7 +577,7 @@ __global__ void __launch_bounds__(kThreadsW4, 1)
         const bool second = lane & 1;
         const int n = t.mt * kRowsW + row - (second ? 1 : 0);
 #pragma unroll
-        for (int i = 0; i < 64; ++i) {
+        for (int i = 0; i < kPairs; ++i) {
           if (2 * i >= ncols) break;
           const float got = __shfl_xor_sync(0xffffffffu, second ? acc[i].x : acc[i].y, 1);
           const uint32_t d = second ? pack_bf16x2(got, acc[i].y) : pack_bf16x2(acc[i].x, got);
@@ -497,12 +586,14 @@ __global__ void __launch_bounds__(kThreadsW4, 1)
             *reinterpret_cast<uint32_t*>(p.out + (t.row0 + col) * ld + n) = d;
         }
       }
-    }
-    if (!ok) give_up();
+      return true;
+    });
+    if (!ok && lane == 0) give_up();
   }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (*abort) {
+  if (*abort_flag) {
     // copies that a given-up wait left in flight land within microseconds: give them a millisecond
     const uint64_t t0 = global_timer_ns();
     while (global_timer_ns() - t0 < 1000000ull) {
@@ -511,28 +602,39 @@ __global__ void __launch_bounds__(kThreadsW4, 1)
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
-    tmem_dealloc(tmem_base, kTmemCols);
+    tmem_dealloc(tmem_base, P::kTmem);
   }
 }
 
-template <int G, bool kZeros, bool kSwiGLU>
-int launch_large(const CUtensorMap& map, const LargeParams& p, int grid, cudaStream_t st) {
-  auto kern = w4_large_kernel<G, kZeros, kSwiGLU>;
-  if (int r = ensure_smem_attr(reinterpret_cast<const void*>(kern), Smem<G>::kBytes))
+struct Maps {
+  CUtensorMap x, q, s, z;
+};
+
+template <int G, bool kZeros, bool kSwiGLU, bool kNarrow>
+int launch_shape(const Maps& map, const LargeParams& p, int grid, cudaStream_t st) {
+  auto kern = w4_large_kernel<G, kZeros, kSwiGLU, kNarrow>;
+  if (int r = ensure_smem_attr(reinterpret_cast<const void*>(kern), Smem<G, kNarrow>::kBytes))
     return r;
-  kern<<<grid, kThreadsW4, Smem<G>::kBytes, st>>>(map, p);
+  kern<<<grid, kThreadsW4, Smem<G, kNarrow>::kBytes, st>>>(map.x, map.q, map.s, map.z, p);
   PRISM_LAUNCH_CHECK("w4_large_kernel launch");
   return PRISM_MOE_OK;
 }
 
+template <int G, bool kZeros, bool kSwiGLU>
+int launch_large(const Maps& map, const LargeParams& p, bool narrow, int grid,
+                 cudaStream_t st) {
+  return narrow ? launch_shape<G, kZeros, kSwiGLU, true>(map, p, grid, st)
+                : launch_shape<G, kZeros, kSwiGLU, false>(map, p, grid, st);
+}
+
 template <int G>
-int launch_group(const CUtensorMap& map, const LargeParams& p, bool swiglu, int grid,
+int launch_group(const Maps& map, const LargeParams& p, bool swiglu, bool narrow, int grid,
                  cudaStream_t st) {
   if (p.z)
-    return swiglu ? launch_large<G, true, true>(map, p, grid, st)
-                  : launch_large<G, true, false>(map, p, grid, st);
-  return swiglu ? launch_large<G, false, true>(map, p, grid, st)
-                : launch_large<G, false, false>(map, p, grid, st);
+    return swiglu ? launch_large<G, true, true>(map, p, narrow, grid, st)
+                  : launch_large<G, true, false>(map, p, narrow, grid, st);
+  return swiglu ? launch_large<G, false, true>(map, p, narrow, grid, st)
+                : launch_large<G, false, false>(map, p, narrow, grid, st);
 }
 
 }  // namespace
@@ -556,18 +658,40 @@ int w4_product_large(const W4Problem& pr, int min_rows, cudaStream_t st) {
   p.z = static_cast<const uint8_t*>(pr.w.zeros);
   p.err = pr.err;
   p.wait_ns = wait_limit_ns();
-  CUtensorMap map;
-  const uint64_t dims[2] = {static_cast<uint64_t>(pr.K), static_cast<uint64_t>(pr.rows_cap)};
-  const uint64_t strides[1] = {static_cast<uint64_t>(pr.K) * 2};
-  const uint32_t box[2] = {kBK, kTokBox};
-  if (int r = encode_bf16_map(&map, pr.x, 2, dims, strides, box)) return r;
+  const int64_t stack = static_cast<int64_t>(p.tiles) * pr.num_mats;   // row tiles of all matrices
+  PRISM_CHECK_ARG(stack < (int64_t(1) << 31), "4-bit product: too many weight rows");
+  Maps map;
+  {
+    const uint64_t dims[2] = {static_cast<uint64_t>(pr.K), static_cast<uint64_t>(pr.rows_cap)};
+    const uint64_t strides[1] = {static_cast<uint64_t>(pr.K) * 2};
+    const uint32_t box[2] = {kBK, kTokBox};
+    if (int r = encode_bf16_map(&map.x, pr.x, 2, dims, strides, box)) return r;
+  }
+  // per chunk and 8 row tiles: 1 KB of codes, 16 rows' scales and zero points of each
+  auto tiles_map = [&](CUtensorMap* m, CUtensorMapDataType type, const void* at, int elems, int bytes) {
+    const uint64_t dims[3] = {static_cast<uint64_t>(elems), static_cast<uint64_t>(p.chunks),
+                              static_cast<uint64_t>(stack)};
+    const uint64_t strides[2] = {static_cast<uint64_t>(bytes),
+                                 static_cast<uint64_t>(bytes) * p.chunks};
+    const uint32_t box[3] = {static_cast<uint32_t>(elems), 1, 8};
+    return encode_map(m, type, CU_TENSOR_MAP_SWIZZLE_NONE, at, 3, dims, strides, box);
+  };
+  const int pg = 128 / pr.w.group_size;
+  if (int r = tiles_map(&map.q, CU_TENSOR_MAP_DATA_TYPE_UINT32, p.q, 256, 1024)) return r;
+  if (int r = tiles_map(&map.s, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.s, 16 * pg, 32 * pg)) return r;
+  map.z = map.s;
+  if (p.z)
+    if (int r = tiles_map(&map.z, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.z, 16 * pg, 16 * pg)) return r;
   const int64_t long_segs = std::min<int64_t>(pr.nseg, pr.rows_cap / (min_rows + 1));
-  const int64_t items = (pr.rows_cap / kTok + long_segs) * p.tiles_n;
+  // tens of rows per segment: narrow tiles (measured: see the table at Shape)
+  const bool narrow = pr.rows_cap <= kNarrowRows * static_cast<int64_t>(pr.nseg);
+  const int64_t items = (pr.rows_cap / (narrow ? 64 : 256) + long_segs) * p.tiles_n;
+  PRISM_CHECK_ARG(items < (int64_t(1) << 31), "4-bit product: too many tiles");
   const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(items, num_sms())));
   switch (pr.w.group_size) {
-    case 32: return launch_group<32>(map, p, pr.swiglu, grid, st);
-    case 64: return launch_group<64>(map, p, pr.swiglu, grid, st);
-    default: return launch_group<128>(map, p, pr.swiglu, grid, st);
+    case 32: return launch_group<32>(map, p, pr.swiglu, narrow, grid, st);
+    case 64: return launch_group<64>(map, p, pr.swiglu, narrow, grid, st);
+    default: return launch_group<128>(map, p, pr.swiglu, narrow, grid, st);
   }
 }
 

@@ -114,6 +114,20 @@ def test_linear_no_rows_and_operator():
     assert torch.equal(y, capi.linear_w4(x, w))
 
 
+@pytest.mark.parametrize("M", [3, 16, 40])
+def test_linear_extreme_magnitudes(M):
+    """Rows far from one another in size, and elements far from one another within a row."""
+    w = weights(5, (), 264, 1024, 128, True)
+    x = rows(6, M, 1024).float()
+    x *= torch.logspace(-30, 30, M, device=DEV).unsqueeze(1)
+    x[:, ::7] *= 2.0 ** -30
+    x[1] = 0
+    x = x.to(torch.bfloat16)
+    y = capi.linear_w4(x, w)
+    check_linear(x, w, y)
+    assert (y[1] == 0).all()
+
+
 def test_linear_rows_do_not_meet():
     """Infinities and NaN stay in their own row; a row's value does not depend on the others."""
     w = weights(3, (), 264, 512, 128, True)
