@@ -9,7 +9,7 @@
 // accumulator once per group: (128 x 256) values per group of 128 inputs are 128 packed fp32x2
 // multiply-adds per warp scheduler in the 512 cycles that the group's products take.
 //
-// Warp roles (512 threads, one CTA per SM, persistent over a device-side tile list):
+// Warp roles (persistent over a device-side tile list):
 //   warp 0        TMA of the activation rows (64 inputs x 64 rows per copy, 128-byte swizzle)
 //   warp 1        TMEM owner and MMA issuer
 //   warp 2        TMA of packed weights, 128 inputs of 8 row tiles (1 KB each) per copy, and of their
@@ -20,8 +20,8 @@
 //                 that its operands are uniform registers; in a one-lane branch each had to be moved
 //                 there, and issuing a stage took longer than its products.
 //   warps 4-7     decode: 16 bytes (four words) per lane and row -> K-major, swizzled bf16 A tile
-//   warps 8-15    accumulate: two warps per TMEM lane quarter, each half of the columns; a lane owns
-//                 one weight row, so a group's scale is one register
+//   warps 8-15    accumulate (8-11 for narrow tiles): two warps per TMEM lane quarter, each half of the
+//                 columns; a lane owns one weight row, so a group's scale is one register
 // Stages hold 64 inputs (A 16 KB + B 32 KB, four of them); a stage is full when its copies have
 // landed and the four decoding warps have arrived. Two TMEM buffers of 256 columns take turns, one
 // group each. Registers are split 40 / 88 / 192 / 192 per thread and warpgroup (512 in all, the launch's 128 x 4).
@@ -40,24 +40,30 @@ constexpr int kRowsW = 128;      // weight rows per tile
 constexpr int kNarrowRows = 64;  // average rows per segment up to which tiles are narrow
 constexpr int kTokBox = 64;      // activation rows per copy
 constexpr int kPackStage = 8 * 1024;
-constexpr int kThreadsW4 = 512;
 constexpr size_t kPrefixW4 = ((kMaxW4Segments + 1) * 4 + 15) / 16 * 16;
 
 // The two shapes: 256 activation rows (many rows per segment: one decoding serves them all) or 64
-// (tens of rows: short stages and more of them keep enough weights in flight to follow HBM, and twice
-// the decoding warps).
+// (tens of rows). With 64 a stage's work is shorter than the latency of handing it from role to role
+// (about 500 cycles each, waits and votes included), so two CTAs share an SM and take turns.
 template <bool kNarrow>
 struct Shape {
   static constexpr int kTok = kNarrow ? 64 : 256;        // activation rows per tile, at most
   static constexpr int kAStage = kRowsW * kBK * 2;
   static constexpr int kStage = kAStage + kTok * kBK * 2;
-  static constexpr int kStages = kNarrow ? 6 : 4;
-  static constexpr int kPackStages = kNarrow ? 6 : 3;
-  static constexpr int kDecWarps = kNarrow ? 8 : 4;
+  static constexpr int kStages = kNarrow ? 3 : 4;
+  static constexpr int kPackStages = 3;
   static constexpr int kAccWarps = kNarrow ? 4 : 8;
+  static constexpr int kThreads = 256 + 32 * kAccWarps;
+  static constexpr int kCtas = kNarrow ? 2 : 1;          // per SM
   static constexpr int kBufs = kNarrow ? 4 : 2;          // TMEM buffers, one group each
   static constexpr uint32_t kTmem = kBufs * kTok;        // TMEM columns
+  // registers of the control, decoding and accumulating warpgroups; their sum is the launch's
+  // (80 x 3, 128 x 4)
+  static constexpr int kRegsControl = kNarrow ? 32 : 40;
+  static constexpr int kRegsDecode = kNarrow ? 64 : 88;
+  static constexpr int kRegsAcc = kNarrow ? 144 : 192;
 };
+constexpr int kDecWarps = 4;
 
 // Shared memory after the stages: packed slots, zero-point slots, scale slots, barriers, prefix.
 template <int G, bool kNarrow>
@@ -66,7 +72,7 @@ struct Smem {
   static constexpr int kPG = 128 / G;                 // groups per chunk
   static constexpr int kZeroSlot = kRowsW * kPG;      // bytes
   static constexpr int kScaleSlot = kRowsW * kPG * 2;
-  static constexpr int kScaleSlots = kPG == 4 && !kNarrow ? 4 : 8;
+  static constexpr int kScaleSlots = kPG == 4 ? 4 : 8;
   static constexpr int kPacked = P::kStages * P::kStage;
   static constexpr int kZeros = kPacked + P::kPackStages * kPackStage;
   static constexpr int kScales = kZeros + P::kPackStages * kZeroSlot;
@@ -74,7 +80,7 @@ struct Smem {
   static constexpr int kNumBars = 2 * (P::kStages + P::kPackStages + kScaleSlots + P::kBufs) + 1;
   static constexpr int kPrefix = kBars + (kNumBars * 8 + 8 + 15) / 16 * 16;
   static constexpr int kBytes = 1024 + kPrefix + static_cast<int>(kPrefixW4);
-  static_assert(kBytes <= 232448, "shared memory budget");
+  static_assert(kBytes <= (kNarrow ? 115712 : 232448), "shared memory budget");
 };
 
 struct LargeParams {
@@ -273,7 +279,7 @@ struct Ring {
 };
 
 template <int G, bool kZeros, bool kSwiGLU, bool kNarrow>
-__global__ void __launch_bounds__(kThreadsW4, 1)
+__global__ void __launch_bounds__(Shape<kNarrow>::kThreads, Shape<kNarrow>::kCtas)
     w4_large_kernel(const __grid_constant__ CUtensorMap map_x,
                     const __grid_constant__ CUtensorMap map_q,
                     const __grid_constant__ CUtensorMap map_s,
@@ -302,10 +308,10 @@ __global__ void __launch_bounds__(kThreadsW4, 1)
       for (int i = 0; i < n; ++i)
         mbar_init(reinterpret_cast<uint64_t*>(smem + (bar - base)) + i, count);
     };
-    init(full, P::kStages, 1 + P::kDecWarps);   // the copies' arrival and the decoding warps
+    init(full, P::kStages, 1 + kDecWarps);   // the copies' arrival and the decoding warps
     init(empty, P::kStages, 1);
     init(pk_full, P::kPackStages, 1);
-    init(pk_empty, P::kPackStages, P::kDecWarps);
+    init(pk_empty, P::kPackStages, kDecWarps);
     init(sc_full, S::kScaleSlots, 1);
     init(sc_empty, S::kScaleSlots, P::kAccWarps);
     init(acc_full, P::kBufs, 1);
@@ -353,7 +359,7 @@ __global__ void __launch_bounds__(kThreadsW4, 1)
   auto wait = [&](uint32_t bar, uint32_t parity) { return bar_wait(bar, parity, abort, p.wait_ns); };
 
   if (warp < 4) {
-    if constexpr (!kNarrow) reg_dealloc<40>();
+    reg_dealloc<P::kRegsControl>();
     bool ok = true;
     if (warp == 0) {
       // ---------------------------------------------------------------- activation rows
@@ -454,11 +460,11 @@ __global__ void __launch_bounds__(kThreadsW4, 1)
       });
     }
     if (!ok && lane == 0) give_up();
-  } else if (warp < 8 || (kNarrow && warp >= 12)) {
+  } else if (warp < 8) {
     // ------------------------------------------------------------------ decode
-    if constexpr (!kNarrow) reg_dealloc<88>();
-    constexpr int kTiles = 8 / P::kDecWarps;   // row tiles per warp
-    const int w = warp < 8 ? warp - 4 : warp - 8, g = lane >> 2, tq = lane & 3;
+    reg_dealloc<P::kRegsDecode>();
+    constexpr int kTiles = 8 / kDecWarps;   // row tiles per warp
+    const int w = warp - 4, g = lane >> 2, tq = lane & 3;
     const bool odd = g & 1;
     Ring<P::kStages> st;
     Ring<P::kPackStages> pk;
@@ -517,7 +523,7 @@ __global__ void __launch_bounds__(kThreadsW4, 1)
     if (!ok && lane == 0) give_up();
   } else {
     // ------------------------------------------------------------------ accumulate
-    if constexpr (!kNarrow) reg_alloc<192>();
+    reg_alloc<P::kRegsAcc>();
     const int q = warp & 3, side = (warp - 8) >> 2;   // narrow: one side, all columns
     constexpr int kPairs = kNarrow ? 32 : 64;          // pairs of columns held, at most
     Ring<P::kBufs> buf;
@@ -615,7 +621,7 @@ int launch_shape(const Maps& map, const LargeParams& p, int grid, cudaStream_t s
   auto kern = w4_large_kernel<G, kZeros, kSwiGLU, kNarrow>;
   if (int r = ensure_smem_attr(reinterpret_cast<const void*>(kern), Smem<G, kNarrow>::kBytes))
     return r;
-  kern<<<grid, kThreadsW4, Smem<G, kNarrow>::kBytes, st>>>(map.x, map.q, map.s, map.z, p);
+  kern<<<grid, Shape<kNarrow>::kThreads, Smem<G, kNarrow>::kBytes, st>>>(map.x, map.q, map.s, map.z, p);
   PRISM_LAUNCH_CHECK("w4_large_kernel launch");
   return PRISM_MOE_OK;
 }
@@ -687,7 +693,7 @@ int w4_product_large(const W4Problem& pr, int min_rows, cudaStream_t st) {
   const bool narrow = pr.rows_cap <= kNarrowRows * static_cast<int64_t>(pr.nseg);
   const int64_t items = (pr.rows_cap / (narrow ? 64 : 256) + long_segs) * p.tiles_n;
   PRISM_CHECK_ARG(items < (int64_t(1) << 31), "4-bit product: too many tiles");
-  const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(items, num_sms())));
+  const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(items, num_sms() * (narrow ? 2 : 1))));
   switch (pr.w.group_size) {
     case 32: return launch_group<32>(map, p, pr.swiglu, narrow, grid, st);
     case 64: return launch_group<64>(map, p, pr.swiglu, narrow, grid, st);
