@@ -24,7 +24,7 @@
 //                 columns; a lane owns one weight row, so a group's scale is one register
 // Stages hold 64 inputs (A 16 KB + B 32 KB, four of them); a stage is full when its copies have
 // landed and the four decoding warps have arrived. Two TMEM buffers of 256 columns take turns, one
-// group each. Registers are split 40 / 88 / 192 / 192 per thread and warpgroup (512 in all, the launch's 128 x 4).
+// group each. Registers are split per warpgroup (Shape).
 // Every wait is bounded; one that runs out records PRISM_MOE_ERR_TIMEOUT and the CTA drains its
 // copies and MMAs before it frees TMEM.
 #include <algorithm>
@@ -58,10 +58,10 @@ struct Shape {
   static constexpr int kBufs = kNarrow ? 4 : 2;          // TMEM buffers, one group each
   static constexpr uint32_t kTmem = kBufs * kTok;        // TMEM columns
   // registers of the control, decoding and accumulating warpgroups; their sum is the launch's
-  // (80 x 3, 128 x 4)
-  static constexpr int kRegsControl = kNarrow ? 32 : 40;
-  static constexpr int kRegsDecode = kNarrow ? 64 : 88;
-  static constexpr int kRegsAcc = kNarrow ? 144 : 192;
+  // at most (80 x 3, 128 x 4)
+  static constexpr int kRegsControl = 32;
+  static constexpr int kRegsDecode = kNarrow ? 64 : 72;
+  static constexpr int kRegsAcc = kNarrow ? 144 : 200;
 };
 constexpr int kDecWarps = 4;
 
@@ -84,7 +84,7 @@ struct Smem {
 };
 
 struct LargeParams {
-  int num_kb, chunks, tiles, tiles_n;   // 64-input blocks, 128-input chunks, row tiles, M tiles
+  int chunks, tiles, tiles_n;   // 128-input chunks, row tiles, M tiles
   int n_out;
   uint16_t* out;
   int64_t rows_cap;
@@ -121,16 +121,44 @@ template <int kBatches, int kPairs>
 __device__ __forceinline__ void add_scaled(float2 (&acc)[kPairs], uint32_t taddr, float s) {
   const float2 s2 = make_float2(s, s);
   const uint64_t ss = *reinterpret_cast<const uint64_t*>(&s2);
+  uint32_t v[2][2][16];   // the next batch is on its way while this one is added
+  tmem_ld16(taddr, v[0][0]);
+  tmem_ld16(taddr + 16, v[0][1]);
 #pragma unroll
   for (int b = 0; b < kBatches; ++b) {
-    uint32_t v[2][16];
-    tmem_ld16(taddr + b * 32, v[0]);
-    tmem_ld16(taddr + b * 32 + 16, v[1]);
     tmem_wait_ld();
+    if (b + 1 < kBatches) {
+      tmem_ld16(taddr + b * 32 + 32, v[(b + 1) & 1][0]);
+      tmem_ld16(taddr + b * 32 + 48, v[(b + 1) & 1][1]);
+    }
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-      fma2(acc[b * 16 + i], v[i >> 3][2 * (i & 7)], v[i >> 3][2 * (i & 7) + 1], ss);
+      fma2(acc[b * 16 + i], v[b & 1][i >> 3][2 * (i & 7)], v[b & 1][i >> 3][2 * (i & 7) + 1], ss);
   }
+}
+
+// Lane l of each 8 holds 8 values (columns) of output l: gives it the 8 outputs of column l, in bf16.
+__device__ __forceinline__ uint4 transpose8(const float (&v)[8], int lane) {
+  uint32_t r[4];
+  const bool b0 = lane & 1, b1 = lane & 2, b2 = lane & 4;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {   // (column 2 j, 2 j + 1) -> outputs (l & ~1, l | 1) of column 2 j + b0
+    const uint32_t own = cvt_bf16x2(v[2 * j], v[2 * j + 1]);
+    const uint32_t got = __shfl_xor_sync(0xffffffffu, own, 1);
+    r[j] = __byte_perm(own, got, b0 ? 0x3276 : 0x5410);
+  }
+  // four outputs of columns b0 + 2 b1 (+ 4): the other half goes to the lane two away
+  uint32_t p[2][2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const uint32_t got = __shfl_xor_sync(0xffffffffu, b1 ? r[2 * j] : r[2 * j + 1], 2);
+    p[j][0] = b1 ? got : r[2 * j];
+    p[j][1] = b1 ? r[2 * j + 1] : got;
+  }
+  uint32_t q[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) q[j] = __shfl_xor_sync(0xffffffffu, b2 ? p[0][j] : p[1][j], 4);
+  return b2 ? make_uint4(q[0], q[1], p[1][0], p[1][1]) : make_uint4(p[0][0], p[0][1], q[0], q[1]);
 }
 
 // One lane of a converged warp.
@@ -144,11 +172,12 @@ __device__ __forceinline__ bool elect_one() {
   return ok != 0;
 }
 // Barriers, copies and accesses by shared-memory address.
-__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {   // all lanes, one answer
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "vote.sync.all.pred p, p, 0xffffffff;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(ok)
       : "r"(bar), "r"(parity)
@@ -162,12 +191,11 @@ __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
 }
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, uint32_t abort,
                                          uint64_t limit_ns) {
-  if (bar_try(bar, parity)) return true;
+  if (__builtin_expect(bar_try(bar, parity), 1)) return true;
   const uint64_t t0 = global_timer_ns();
   while (true) {
     if (bar_try(bar, parity)) return true;
-    if (lds32(abort)) return false;
-    if (global_timer_ns() - t0 > limit_ns) return false;
+    if (__any_sync(0xffffffffu, lds32(abort) != 0 || global_timer_ns() - t0 > limit_ns)) return false;
   }
 }
 __device__ __forceinline__ void bar_arrive(uint32_t bar) {
@@ -356,7 +384,10 @@ __global__ void __launch_bounds__(Shape<kNarrow>::kThreads, Shape<kNarrow>::kCta
     return ok;
   };
   auto next_chunk = [&](int c) { return c + 1 == p.chunks ? 0 : c + 1; };
-  auto wait = [&](uint32_t bar, uint32_t parity) { return bar_wait(bar, parity, abort, p.wait_ns); };
+  // every lane polls: one lane polling for all (and the divergence it brings) measured 15% slower
+  auto wait = [&](uint32_t bar, uint32_t parity) {
+    return bar_wait(bar, parity, abort, p.wait_ns);
+  };
 
   if (warp < 4) {
     reg_dealloc<P::kRegsControl>();
@@ -367,13 +398,14 @@ __global__ void __launch_bounds__(Shape<kNarrow>::kThreads, Shape<kNarrow>::kCta
       ok = for_tiles([&](const Tile& t) {
         const int boxes = (t.cols + kTokBox - 1) / kTokBox;
         for (int i = 0, c = t.c0; i < p.chunks; ++i, c = next_chunk(c))
-          for (int kb = 2 * c; kb < min(2 * c + 2, p.num_kb); ++kb) {
-            if (!__all_sync(0xffffffffu, wait(empty + 8 * st.slot, st.phase ^ 1))) return false;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {   // inputs past the last are read as zeros
+            if (!wait(empty + 8 * st.slot, st.phase ^ 1)) return false;
             if (elect_one()) {
               bar_expect(full + 8 * st.slot, boxes * kTokBox * kBK * 2);
               const uint32_t b = base + st.slot * kStage + kAStage;
               for (int x = 0; x < boxes; ++x)
-                copy_2d(b + x * kTokBox * kBK * 2, &map_x, full + 8 * st.slot, kb * kBK,
+                copy_2d(b + x * kTokBox * kBK * 2, &map_x, full + 8 * st.slot, (2 * c + half) * kBK,
                         t.row0 + x * kTokBox);
             }
             __syncwarp();
@@ -385,29 +417,28 @@ __global__ void __launch_bounds__(Shape<kNarrow>::kThreads, Shape<kNarrow>::kCta
       // ---------------------------------------------------------------- MMA issuer
       Ring<P::kStages> st;
       Ring<P::kBufs> buf;
+      constexpr int kSteps = G == 32 ? 2 : 4;   // 16-input steps of a group within 64 inputs
       const uint64_t desc_a = smem_desc_sw128(base), desc_b = smem_desc_sw128(base + kAStage);
       ok = for_tiles([&](const Tile& t) {
         const uint32_t idesc = idesc_bf16_f32(kRowsW, t.cols);
         for (int i = 0, c = t.c0; i < p.chunks; ++i, c = next_chunk(c)) {
-          const int kb_end = min(2 * c + 2, p.num_kb);
-          for (int kb = 2 * c; kb < kb_end; ++kb) {
-            if (!__all_sync(0xffffffffu, wait(full + 8 * st.slot, st.phase))) return false;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            if (!wait(full + 8 * st.slot, st.phase)) return false;
             const uint32_t off = st.slot * (kStage >> 4);
 #pragma unroll
-            for (int k0 = 0; k0 < 4; k0 += (G == 32 ? 2 : 4)) {   // the 16-input steps of one group
+            for (int k0 = 0; k0 < 4; k0 += kSteps) {
               // a new group starts: its buffer must have been read
-              const bool first = G != 128 || kb == 2 * c;
-              if (first && !__all_sync(0xffffffffu, wait(acc_empty + 8 * buf.slot, buf.phase ^ 1)))
-                return false;
+              const bool first = G != 128 || half == 0, last = G != 128 || half == 1;
+              if (first && !wait(acc_empty + 8 * buf.slot, buf.phase ^ 1)) return false;
               tc_fence_after();
-              const bool last = G != 128 || kb + 1 == kb_end;
               if (elect_one()) {
 #pragma unroll
-                for (int kk = k0; kk < k0 + (G == 32 ? 2 : 4); ++kk)
+                for (int kk = k0; kk < k0 + kSteps; ++kk)
                   tc_mma_bf16(tmem_base + buf.slot * kTok, desc_a + off + kk * 2,
                               desc_b + off + kk * 2, idesc, first && kk == k0 ? 0u : 1u);
                 if (last) bar_commit(acc_full + 8 * buf.slot);
-                if (k0 + (G == 32 ? 2 : 4) == 4) bar_commit(empty + 8 * st.slot);
+                if (k0 + kSteps == 4) bar_commit(empty + 8 * st.slot);
               }
               __syncwarp();
               if (last) buf.next();
@@ -423,7 +454,8 @@ __global__ void __launch_bounds__(Shape<kNarrow>::kThreads, Shape<kNarrow>::kCta
         if (elect_one()) bar_commit(drain);   // completes once every MMA issued above has finished
         __syncwarp();
         const uint64_t t0 = global_timer_ns();
-        while (!bar_try(drain, 0) && global_timer_ns() - t0 < kDrainNs) {
+        while (!bar_try(drain, 0) &&
+               !__any_sync(0xffffffffu, global_timer_ns() - t0 > kDrainNs)) {
         }
       }
     } else if (warp == 2) {
@@ -432,7 +464,7 @@ __global__ void __launch_bounds__(Shape<kNarrow>::kThreads, Shape<kNarrow>::kCta
       ok = for_tiles([&](const Tile& t) {
         const int tile0 = t.e * p.tiles + t.mt * 8;
         for (int i = 0, c = t.c0; i < p.chunks; ++i, c = next_chunk(c), pk.next()) {
-          if (!__all_sync(0xffffffffu, wait(pk_empty + 8 * pk.slot, pk.phase ^ 1))) return false;
+          if (!wait(pk_empty + 8 * pk.slot, pk.phase ^ 1)) return false;
           if (elect_one()) {
             const uint32_t bar = pk_full + 8 * pk.slot;
             bar_expect(bar, kPackStage + (kZeros ? S::kZeroSlot : 0));
@@ -448,7 +480,7 @@ __global__ void __launch_bounds__(Shape<kNarrow>::kThreads, Shape<kNarrow>::kCta
       Ring<S::kScaleSlots> sc;
       ok = for_tiles([&](const Tile& t) {
         for (int i = 0, c = t.c0; i < p.chunks; ++i, c = next_chunk(c), sc.next()) {
-          if (!__all_sync(0xffffffffu, wait(sc_empty + 8 * sc.slot, sc.phase ^ 1))) return false;
+          if (!wait(sc_empty + 8 * sc.slot, sc.phase ^ 1)) return false;
           if (elect_one()) {
             bar_expect(sc_full + 8 * sc.slot, S::kScaleSlot);
             copy_3d(scales + sc.slot * S::kScaleSlot, &map_s, sc_full + 8 * sc.slot, 0, c,
@@ -475,7 +507,7 @@ __global__ void __launch_bounds__(Shape<kNarrow>::kThreads, Shape<kNarrow>::kCta
     const uint32_t at0 = ((odd ? 4 : 0) + tq) ^ g, at1 = ((odd ? 0 : 4) + tq) ^ g;
     const bool ok = for_tiles([&](const Tile& t) {
       for (int i = 0, c = t.c0; i < p.chunks; ++i, c = next_chunk(c)) {
-        if (!__all_sync(0xffffffffu, wait(pk_full + 8 * pk.slot, pk.phase))) return false;
+        if (!wait(pk_full + 8 * pk.slot, pk.phase)) return false;
         // rows g and g + 8 of this warp's row tiles
         uint32_t zr[2 * kTiles][PG];
         uint4 v[2 * kTiles];
@@ -493,8 +525,7 @@ __global__ void __launch_bounds__(Shape<kNarrow>::kThreads, Shape<kNarrow>::kCta
         pk.next();
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          if (2 * c + half >= p.num_kb) break;
-          if (!__all_sync(0xffffffffu, wait(empty + 8 * st.slot, st.phase ^ 1))) return false;
+          if (!wait(empty + 8 * st.slot, st.phase ^ 1)) return false;
           const uint32_t a = to + st.slot * kStage;
 #pragma unroll
           for (int r = 0; r < 2 * kTiles; ++r) {
@@ -529,7 +560,6 @@ __global__ void __launch_bounds__(Shape<kNarrow>::kThreads, Shape<kNarrow>::kCta
     Ring<P::kBufs> buf;
     Ring<S::kScaleSlots> sl;
     const int row = q * 32 + lane;                     // weight row in the tile
-    const int groups = G == 128 ? p.chunks : p.num_kb * (G == 32 ? 2 : 1);
     const bool ok = for_tiles([&](const Tile& t) {
       const int left = kNarrow ? t.cols : (t.cols / 16 + 1) / 2 * 16;   // columns of side 0
       const int col0 = side ? left : 0, ncols = side ? t.cols - left : left;
@@ -538,7 +568,7 @@ __global__ void __launch_bounds__(Shape<kNarrow>::kThreads, Shape<kNarrow>::kCta
       for (int i = 0; i < kPairs; ++i) acc[i] = make_float2(0.f, 0.f);
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + col0;
       for (int i = 0, c = t.c0; i < p.chunks; ++i, c = next_chunk(c)) {
-        if (!__all_sync(0xffffffffu, wait(sc_full + 8 * sl.slot, sl.phase))) return false;
+        if (!wait(sc_full + 8 * sl.slot, sl.phase)) return false;
         const uint2 raw = lds_small<2 * PG>(scales + sl.slot * S::kScaleSlot + row * 2 * PG);
         const float sc[4] = {__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xffff0000u),
                              __uint_as_float(raw.y << 16), __uint_as_float(raw.y & 0xffff0000u)};
@@ -547,8 +577,7 @@ __global__ void __launch_bounds__(Shape<kNarrow>::kThreads, Shape<kNarrow>::kCta
         sl.next();
 #pragma unroll
         for (int gr = 0; gr < PG; ++gr) {
-          if (c * PG + gr >= groups) break;   // the last chunk of an odd number of 64-input blocks
-          if (!__all_sync(0xffffffffu, wait(acc_full + 8 * buf.slot, buf.phase))) return false;
+          if (!wait(acc_full + 8 * buf.slot, buf.phase)) return false;
           tc_fence_after();
           const uint32_t at = taddr + buf.slot * kTok;
           // few columns, or all 128 (64) of this side (those past ncols hold what an earlier tile
@@ -563,33 +592,41 @@ __global__ void __launch_bounds__(Shape<kNarrow>::kThreads, Shape<kNarrow>::kCta
           buf.next();
         }
       }
-      // ---- output: lanes are consecutive outputs of one activation row
+      // ---- output: lanes are outputs of one activation row; 8 lanes swap 8 columns for 16-byte stores
       const int64_t ld = p.n_out;
       if constexpr (kSwiGLU) {
-        // lanes 0-7 and 16-23 hold gate rows, the lanes 8 above them the matching up rows; each of a
-        // pair finishes one of two columns
+        // lanes 0-7 and 16-23 hold gate rows, the lanes 8 above them the matching up rows; of two
+        // columns the gate lane finishes the first, the up lane the second
         const bool up = lane & 8;
-        const int n = (t.mt * kRowsW + q * 32) / 2 + (lane >> 4) * 8 + (lane & 7);
+        const int n = (t.mt * kRowsW + q * 32) / 2 + (lane >> 4) * 8;
+        const int mine = col0 + 2 * (lane & 7) + (up ? 1 : 0);
+        uint16_t* to = p.out + (t.row0 + mine) * ld + n;
+        const int rows = n < p.n_out ? t.rows - mine : 0;
 #pragma unroll
-        for (int i = 0; i < kPairs; ++i) {
-          if (2 * i >= ncols) break;
-          const float got = __shfl_xor_sync(0xffffffffu, up ? acc[i].x : acc[i].y, 8);
-          const float h = up ? silu_mul(got, acc[i].y) : silu_mul(acc[i].x, got);
-          const int col = col0 + 2 * i + (up ? 1 : 0);
-          if (col < t.rows && n < p.n_out) p.out[(t.row0 + col) * ld + n] = float_to_bf16_bits(h);
+        for (int b = 0; b < kPairs; b += 8) {
+          if (2 * b >= ncols) break;
+          float h[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float2 a = acc[b + i];
+            const float got = __shfl_xor_sync(0xffffffffu, up ? a.x : a.y, 8);
+            h[i] = silu_mul(up ? got : a.x, up ? a.y : got);
+          }
+          const uint4 d = transpose8(h, lane);
+          if (2 * b < rows) *reinterpret_cast<uint4*>(to + 2 * b * ld) = d;
         }
       } else {
-        // neighbours swap a column: each stores two outputs of one row
-        const bool second = lane & 1;
-        const int n = t.mt * kRowsW + row - (second ? 1 : 0);
+        const int n = t.mt * kRowsW + q * 32 + (lane & 24);
+        const int mine = col0 + (lane & 7);
+        uint16_t* to = p.out + (t.row0 + mine) * ld + n;
+        const int rows = n < p.n_out ? t.rows - mine : 0;
 #pragma unroll
-        for (int i = 0; i < kPairs; ++i) {
-          if (2 * i >= ncols) break;
-          const float got = __shfl_xor_sync(0xffffffffu, second ? acc[i].x : acc[i].y, 1);
-          const uint32_t d = second ? pack_bf16x2(got, acc[i].y) : pack_bf16x2(acc[i].x, got);
-          const int col = col0 + 2 * i + (second ? 1 : 0);
-          if (col < t.rows && n < p.n_out)
-            *reinterpret_cast<uint32_t*>(p.out + (t.row0 + col) * ld + n) = d;
+        for (int b = 0; b < kPairs; b += 4) {
+          if (2 * b >= ncols) break;
+          const float v[8] = {acc[b].x,     acc[b].y,     acc[b + 1].x, acc[b + 1].y,
+                              acc[b + 2].x, acc[b + 2].y, acc[b + 3].x, acc[b + 3].y};
+          const uint4 d = transpose8(v, lane);
+          if (2 * b < rows) *reinterpret_cast<uint4*>(to + 2 * b * ld) = d;
         }
       }
       return true;
@@ -647,7 +684,6 @@ int launch_group(const Maps& map, const LargeParams& p, bool swiglu, bool narrow
 
 int w4_product_large(const W4Problem& pr, int min_rows, cudaStream_t st) {
   LargeParams p{};
-  p.num_kb = static_cast<int>(ceil_div(pr.K, kBK));
   p.chunks = static_cast<int>(ceil_div(pr.K, 128));
   p.tiles = static_cast<int>(ceil_div(pr.swiglu ? 2 * pr.n_out : pr.n_out, 16));
   p.tiles_n = static_cast<int>(ceil_div(p.tiles, 8));
