@@ -160,6 +160,7 @@ int expert_swiglu_w4(const void* xs, int64_t rows, int64_t H, int64_t I,
   p.swiglu = false;
   p.w = dn;
   p.out = y;
+  p.after_product = true;
   const int r = w4_product(p, st);
   record_stage(5, st);
   return r;

@@ -106,6 +106,8 @@ struct W4Problem {
   prism_moe_w4 w{};
   void* out = nullptr;            // [rows_cap, n_out] bf16
   int* err = nullptr;
+  bool after_product = false;     // the kernel before it in the stream is a product that wrote ``x``, and
+                                  // nothing else of this call was written by one
 };
 constexpr int kMaxW4Segments = 1024;   // the kernels keep the segments' prefix in shared memory
 int w4_product(const W4Problem& pr, cudaStream_t st);

@@ -13,14 +13,6 @@
 
 namespace prism {
 
-__device__ __forceinline__ uint4 load_stream(const uint8_t* p) {   // read once: not kept in L1
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
-
 __device__ __forceinline__ uint32_t word_of(const uint4& v, int j) {
   return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w;
 }
@@ -34,12 +26,18 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t word, int i, uint32_t zer
   return d;
 }
 
-// bf16 pair 16 + code of inputs (2 i, 2 i + 1): the code in the upper four of the seven fraction bits
-// under the exponent of 16. Mask and exponent go in with one three-input operation.
-__device__ __forceinline__ uint32_t code16_pair(uint32_t word, int i) {
-  const uint32_t c = i == 0 ? word << 3 : word >> (4 * i - 3);
+// bf16 pair offset + code of inputs (2 i, 2 i + 1). Nibbles in bits 0-3 of a half, as they are or
+// after a shift by 8, are the lowest of the seven fraction bits under the exponent of 128 (i = 0, 2);
+// nibbles in bits 4-7 move down by one bit to the highest under the exponent of 16 (i = 1, 3). Mask
+// and exponent go in with one three-input operation. Without kMixed every nibble goes under 16.
+template <bool kMixed>
+__device__ __forceinline__ uint32_t offset_pair(uint32_t word, int i) {
+  const bool low = kMixed && !(i & 1);
+  const uint32_t c = low ? (i ? word >> 8 : word) : i == 0 ? word << 3 : word >> (4 * i - 3);
   uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(c), "r"(0x00780078u), "r"(0x41804180u));
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;"
+      : "=r"(d)
+      : "r"(c), "r"(low ? 0x000f000fu : 0x00780078u), "r"(low ? 0x43004300u : 0x41804180u));
   return d;
 }
 
@@ -81,20 +79,18 @@ __device__ __forceinline__ void load_zeros(const uint8_t* z, int64_t at, uint32_
   }
 }
 
-// 16 + zero for each of the PG groups, as code16_pair's sums need it; 8 without zero points.
-template <int PG, bool kZeros>
+// The zero point of each of the PG groups.
+template <int PG>
 __device__ __forceinline__ void load_zero_points(const uint8_t* z, float (&out)[PG]) {
-  uint32_t v = 0x08080808u;
-  if constexpr (kZeros) {
-    if constexpr (PG == 1)
-      v = *z;
-    else if constexpr (PG == 2)
-      v = *reinterpret_cast<const uint16_t*>(z);
-    else
-      v = *reinterpret_cast<const uint32_t*>(z);
-  }
+  uint32_t v;
+  if constexpr (PG == 1)
+    v = *z;
+  else if constexpr (PG == 2)
+    v = *reinterpret_cast<const uint16_t*>(z);
+  else
+    v = *reinterpret_cast<const uint32_t*>(z);
 #pragma unroll
-  for (int i = 0; i < PG; ++i) out[i] = 16.f + static_cast<float>((v >> (8 * i)) & 0xfu);
+  for (int i = 0; i < PG; ++i) out[i] = static_cast<float>((v >> (8 * i)) & 0xfu);
 }
 
 // silu(g) * u in fp32.

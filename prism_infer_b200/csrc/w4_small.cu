@@ -12,11 +12,13 @@
 // scale is applied to the fp32 sum of each group, so no weight is ever rounded.
 //
 // The subtraction of 128 + zero that code_pair does would be a third of the decoding. It is left out
-// here: the instruction sums (16 + code) * x (w4.cuh, code16_pair), exactly up to its fp32 sum, and
-// (16 + zero) * sum(x) of the group is taken off together with the scale; sum(x) of each group comes
-// from one more instruction per input step, on a matrix of ones, once per block of rows. The price
-// is cancellation: sums carry 16 .. 31 instead of -8 .. 7, about four times the fp32 error of the
-// plain sum, still 2^-18 of it at 4096 inputs.
+// here: the instruction sums (offset + code) * x, and offset * x and zero * x of the group are taken
+// off together with the scale; those sums come from one or two more instructions per input step, on
+// constant matrices, once per block of rows. The offset is 128 where the nibble is used in place and
+// 16 where one bit's shift puts it under a smaller exponent (w4.cuh), which makes three shifts per
+// word: shifts and logic share a half-rate pipe and are what the loop has most of. The price is
+// cancellation: the sums carry up to 143 per input instead of 8, at most 2^-17 of their terms'
+// magnitudes at 4096 inputs where the output's rounding is 2^-8.
 //
 // What bounds it: few rows reuse nothing, so every hit weight crosses HBM once and that is the floor.
 // A block's warps split the inputs (kw ways) and keep their part of x in registers while the block
@@ -56,8 +58,11 @@ struct SmallParams {
   const uint8_t *q, *z;
   const uint16_t* s;
   int kw, rw, rt, passes;    // input splits, row-tile splits, row tiles per item, input passes
+  int rt_bits;               // rt = 1 << rt_bits
   int blocks_n;              // ceil(tiles / rt)
+  int all_chunks;            // of all matrices
   int64_t max_rows;          // longer segments are the other kernel's
+  int early;                 // may start while the kernel before it ends (see griddepcontrol)
   int* err;
 };
 
@@ -70,15 +75,16 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// ``B`` bytes from src + kFrom to shared memory at dst + kTo.
-template <int B, int kTo, int kFrom>
+__device__ __forceinline__ void wait_for_earlier() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+template <int B>
 __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
   if constexpr (B == 16)
-    asm volatile("cp.async.cg.shared.global.L2::128B [%0+%2], [%1+%3], 16;" ::"r"(dst), "l"(src),
-                 "n"(kTo), "n"(kFrom));
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src));
   else
-    asm volatile("cp.async.ca.shared.global [%0+%2], [%1+%3], %4;" ::"r"(dst), "l"(src), "n"(kTo),
-                 "n"(kFrom), "n"(B));
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(B));
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;"); }
 template <int N>
@@ -100,6 +106,10 @@ template <int G, bool kZeros, bool kSwiGLU, int NT>
 __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 2 : 1) w4_small_kernel(const SmallParams p) {
   constexpr int PG = 128 / G;   // groups per chunk
   using M = Meta<PG>;
+  // mixed offsets keep two sums per group; with four groups a chunk that is more registers than the
+  // shift is worth, and the offset is 16 for every nibble
+  constexpr bool kMixed = PG < 4;
+  constexpr bool kOff = kMixed || !kZeros;
   constexpr int kMetaSlot = 32 * M::kBytes;
   constexpr int kSlot = kTps * kCh * (1024 + kMetaSlot);
   extern __shared__ uint4 smem_raw[];
@@ -120,7 +130,10 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 2 : 1) w4_small_kernel(
   const int64_t bid = blockIdx.x, blocks = gridDim.x;
   const int item0 = static_cast<int>(total * bid / blocks);
   const int item1 = static_cast<int>(total * (bid + 1) / blocks);
-  if (item0 >= item1) return;
+  if (item0 >= item1) {
+    wait_for_earlier();   // a grid that ends before the one ahead of it would let the next one pass both
+    return;
+  }
 
   // ---- the stream of steps: item by item, pass by pass, kTps row tiles a step. Every item has the
   // same steps and every step the same copies: what lies past the last tile or chunk is read from
@@ -158,19 +171,29 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 2 : 1) w4_small_kernel(
     if (ahead_item < item1) {
       const int c0 = (ahead_pass * p.kw + wk) * kCh;
       const int tile0 = ahead.nb * p.rt + ahead_i;
+      const int chunk0 = (max(ahead.base, 0) + tile0) * p.chunks + c0;
+      // tiles and chunks past the end of a row of tiles are the next ones' in memory: only the end of
+      // the whole stack needs care
+      const bool inside = chunk0 + (kTps - 1) * p.chunks + kCh <= p.all_chunks;
 #pragma unroll
       for (int u = 0; u < kTps; ++u) {
-        const int row = (max(ahead.base, 0) + min(tile0 + u, p.tiles - 1)) * p.chunks;
+        int chunk = chunk0 + u * p.chunks;
+        const uint8_t* from = q_lane + static_cast<int64_t>(chunk) * 1024;
+        const uint8_t* meta = m_lane + static_cast<int64_t>(chunk) * m_stride;
 #pragma unroll
         for (int ch = 0; ch < kCh; ++ch) {
-          const int chunk = row + min(c0 + ch, p.chunks - 1);
-          const uint8_t* from = q_lane + static_cast<int64_t>(chunk) * 1024;
+          if (!inside) {
+            chunk = min(chunk0 + u * p.chunks + ch, p.all_chunks - 1);
+            from = q_lane + static_cast<int64_t>(chunk) * 1024;
+            meta = m_lane + static_cast<int64_t>(chunk) * m_stride;
+          }
           const uint32_t to = ring_lane + fill + (u * kCh + ch) * (1024 + kMetaSlot);
-          copy_async<16, 0, 0>(to, from);
-          copy_async<16, 512, 512>(to, from);
+          copy_async<16>(to, from);
+          copy_async<16>(to + 512, from + 512);
           if (kZeros || t < 2)
-            copy_async<M::kBytes, 1024, 0>(ring_meta + fill + (u * kCh + ch) * (1024 + kMetaSlot),
-                                           m_lane + static_cast<int64_t>(chunk) * m_stride);
+            copy_async<M::kBytes>(ring_meta + fill + (u * kCh + ch) * (1024 + kMetaSlot) + 1024, meta);
+          from += 1024;
+          meta += m_stride;
         }
       }
       ahead_i += next_i;
@@ -189,8 +212,14 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 2 : 1) w4_small_kernel(
 #pragma unroll
   for (int d = 0; d < kDepth - 1; ++d) fetch();
 
+  // From here on this kernel reads what the one before it wrote. Everything above (the list, the
+  // weights in flight) may run while that one ends; a kernel behind may start likewise.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  wait_for_earlier();
   uint4 xb[kCh][NT][4];
-  float sx[kCh][PG][NT][2];   // sum of x over each group, columns 2 t and 2 t + 1
+  // sums over each group, columns 2 t and 2 t + 1: of offset * x (with zero point 8 where there are
+  // none), and of x
+  float off[kOff ? kCh : 1][PG][NT][2], sx[kZeros ? kCh : 1][PG][NT][2];
   int loaded_unit = -1, loaded_pass = -1;
   int rows = 0;
   int64_t row0 = 0;
@@ -227,15 +256,27 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 2 : 1) w4_small_kernel(
           for (int gr = 0; gr < PG; ++gr)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              float ones[4] = {};
-              constexpr uint32_t one = 0x3f803f80u;
+              float o[4] = {}, ones[4] = {};
+              constexpr uint32_t one = 0x3f803f80u;                      // 1
+              constexpr uint32_t at_0 = !kMixed ? (kZeros ? 0x41804180u : 0x41c041c0u)
+                                                : (kZeros ? 0x43004300u : 0x43084308u);   // 128 (+ 8)
+              constexpr uint32_t at_1 = kZeros ? 0x41804180u : 0x41c041c0u;   // 16 (+ 8)
 #pragma unroll
               for (int j = gr * (4 / PG); j < (gr + 1) * (4 / PG); ++j) {
-                mma_16816(ones, one, one, one, one, xb[c][nt][j].x, xb[c][nt][j].y);
-                mma_16816(ones, one, one, one, one, xb[c][nt][j].z, xb[c][nt][j].w);
+                if constexpr (kOff) {
+                  mma_16816(o, at_0, at_0, at_1, at_1, xb[c][nt][j].x, xb[c][nt][j].y);
+                  mma_16816(o, at_0, at_0, at_1, at_1, xb[c][nt][j].z, xb[c][nt][j].w);
+                }
+                if constexpr (kZeros) {
+                  mma_16816(ones, one, one, one, one, xb[c][nt][j].x, xb[c][nt][j].y);
+                  mma_16816(ones, one, one, one, one, xb[c][nt][j].z, xb[c][nt][j].w);
+                }
               }
-              sx[c][gr][nt][0] = ones[0];
-              sx[c][gr][nt][1] = ones[1];
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                if constexpr (kOff) off[c][gr][nt][q] = o[q];
+                if constexpr (kZeros) sx[c][gr][nt][q] = ones[q];
+              }
             }
       }
 #pragma unroll 1
@@ -261,8 +302,8 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 2 : 1) w4_small_kernel(
               load_scales<PG>(reinterpret_cast<const uint16_t*>(meta + h * M::kBytes) +
                                   (g & (M::kScaleRows - 1)) * PG,
                               sc[h]);
-              load_zero_points<PG, kZeros>(
-                  meta + (2 + h) * M::kBytes + (g & (M::kZeroRows - 1)) * PG, zp[h]);
+              if constexpr (kZeros)
+                load_zero_points<PG>(meta + (2 + h) * M::kBytes + (g & (M::kZeroRows - 1)) * PG, zp[h]);
             }
 #pragma unroll
             for (int gr = 0; gr < PG; ++gr) {
@@ -273,8 +314,8 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 2 : 1) w4_small_kernel(
                 uint32_t a[2][4];
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                  a[0][q] = code16_pair(word0, q);
-                  a[1][q] = code16_pair(word1, q);
+                  a[0][q] = offset_pair<kMixed>(word0, q);
+                  a[1][q] = offset_pair<kMixed>(word1, q);
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
@@ -287,10 +328,14 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 2 : 1) w4_small_kernel(
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                  acc[nt][q] = fmaf(sc[q >> 1][gr],
-                                    fmaf(-zp[q >> 1][gr], sx[c][gr][nt][q & 1], sum[nt][q]),
-                                    acc[nt][q]);
+                for (int q = 0; q < 4; ++q) {
+                  float d = sum[nt][q];
+                  if constexpr (kOff) d -= off[c][gr][nt][q & 1];
+                  if constexpr (kZeros)
+                    d = fmaf(kMixed ? -zp[q >> 1][gr] : -16.f - zp[q >> 1][gr],
+                             sx[c][gr][nt][q & 1], d);
+                  acc[nt][q] = fmaf(sc[q >> 1][gr], d, acc[nt][q]);
+                }
             }
           }
           float* to = mine + (i0 + u) * kTile;
@@ -314,10 +359,11 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 2 : 1) w4_small_kernel(
     }
     // sum of the kw partial tiles, two outputs per thread, neighbours along the output row
     constexpr int kPairs = kSwiGLU ? 4 : 8;   // output pairs of one row tile
-    const int per_row = tiles_here * kPairs;
-    for (int i = threadIdx.x; i < rows * per_row; i += nwarps * 32) {
-      const int col = i / per_row, pr = i % per_row;
+    const int span_bits = p.rt_bits + (kSwiGLU ? 2 : 3);   // pairs of an item's output row
+    for (int i = threadIdx.x; i < rows << span_bits; i += nwarps * 32) {
+      const int col = i >> span_bits, pr = i & ((1 << span_bits) - 1);
       const int tile = pr / kPairs, r = pr % kPairs * 2;
+      if (tile >= tiles_here) continue;
       const float* at = sums + tile * kTile + col * kColStride + r;
       float2 a = make_float2(0.f, 0.f), b = make_float2(0.f, 0.f);
       for (int k = 0; k < p.kw; ++k, at += p.rt * kTile) {
@@ -348,7 +394,8 @@ int launch_small(SmallParams p, int64_t units, cudaStream_t st) {
   // inputs: up to 8 warps x 2 chunks per pass; warps that the inputs do not need take row tiles
   p.passes = static_cast<int>(ceil_div(p.chunks, kWarps * kCh));
   p.kw = static_cast<int>(ceil_div(p.chunks, p.passes * kCh));
-  p.rw = std::max(1, kWarps / p.kw);
+  p.rw = 1;   // a power of two, and so are the row tiles of an item
+  while (2 * p.rw * p.kw <= kWarps) p.rw *= 2;
   const int sms = num_sms();
   // row tiles per item and step: several share a barrier and the bookkeeping, few fill the GPU when
   // the call is small
@@ -365,6 +412,11 @@ int launch_small(SmallParams p, int64_t units, cudaStream_t st) {
   if (NT == 1 && 2 * (bytes_of(p.rt) + 1024) > kSmSmem && p.rt >= 2 * kTps * p.rw) p.rt /= 2;
   const int bytes = bytes_of(p.rt);
   p.blocks_n = static_cast<int>(ceil_div(p.tiles, p.rt));
+  p.rt_bits = 0;
+  while ((1 << p.rt_bits) < p.rt) ++p.rt_bits;
+  const int64_t all_chunks = static_cast<int64_t>(p.tiles) * p.num_mats * p.chunks;
+  PRISM_CHECK_ARG(all_chunks < (int64_t(1) << 31) - 64, "4-bit product: too many weights");
+  p.all_chunks = static_cast<int>(all_chunks);
   constexpr int kMaxBytes = kWarps * kDepth * kSlot + 2 * kWarps * kMaxKwRt * kTile * 4 +
                             (kMaxW4Segments + 4) / 4 * 16;
   static_assert(kMaxBytes <= 232448, "shared memory budget");
@@ -375,8 +427,17 @@ int launch_small(SmallParams p, int64_t units, cudaStream_t st) {
       1, std::min({65536 / ((NT == 1 ? 128 : 256) * 32 * warps), kSmSmem / (bytes + 1024), 4}));
   const int grid =
       static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(items, per_sm * sms)));
-  kern<<<grid, 32 * warps, bytes, st>>>(p);
-  PRISM_LAUNCH_CHECK("w4_small_kernel launch");
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3(32 * warps, 1, 1);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = st;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.early ? 1 : 0;
+  PRISM_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
   return PRISM_MOE_OK;
 }
 
@@ -405,14 +466,23 @@ int launch_zeros(const SmallParams& p, bool swiglu, int64_t u8, int64_t u16, cud
 int w4_product(const W4Problem& pr, cudaStream_t st) {
   SmallParams p{};
   p.max_rows = int64_t(1) << 31;
-  // Few rows per segment on average: this kernel alone (a longer segment runs in blocks of 16 rows,
-  // its weights from L2 after the first). Else segments of at most kSmallRows rows run here and
-  // longer ones on the other kernel; the host does not know the lengths and launches both.
-  if (pr.rows_cap > std::max<int64_t>(kSmallRows, pr.seg_offsets ? 8 * pr.nseg : 0)) {
+  // Few rows: this kernel alone (a longer segment runs in blocks of 16 rows, its weights from L2
+  // after the first). Without a table: up to 16 rows, and up to 64 while the matrix is so small that
+  // the other kernel's tiles could not fill the GPU (17 x 4096 x 4096: 17 us here, 29 there;
+  // 17 x 18944 x 4096: 39 and 33). With one: segments of 10 rows on average (1280 rows of 128
+  // experts: 169 us here, 185 with both). Else segments of at most kSmallRows rows run here and longer
+  // ones on the other kernel; the host does not know the lengths and launches both.
+  const int64_t out_tiles = ceil_div(pr.swiglu ? 2 * pr.n_out : pr.n_out, 16);
+  const bool few = pr.seg_offsets
+                       ? pr.rows_cap <= std::max<int64_t>(kSmallRows, 10 * pr.nseg)
+                       : pr.rows_cap <= kSmallRows ||
+                             (pr.rows_cap <= 64 && ceil_div(pr.rows_cap, 16) * out_tiles <= 9 * num_sms());
+  if (!few) {
     if (int r = w4_product_large(pr, kSmallRows, st)) return r;
     if (!pr.seg_offsets) return PRISM_MOE_OK;
     p.max_rows = kSmallRows;
   }
+  p.early = few && pr.after_product;
   p.x = static_cast<const uint16_t*>(pr.x);
   p.ld_x = pr.K;
   p.K = static_cast<int>(pr.K);

@@ -4,8 +4,8 @@ Bounds, element by element. The kernels multiply small integers by bf16 activati
 sum in fp32: a sum of n partial sums in whatever order is off by at most n * 2^-22 of the sum of the
 terms' magnitudes (2^-24 for each rounding, four times that for the tensor cores' alignment of their
 addends). n is the 16-input steps of one group, the groups, and the joining of up to 16 parts. The
-integers are code - zero for many rows; for few rows 16 + code and 16 + zero are summed apart, 31 at
-most each: terms of up to 62 * scale * |x| in all.
+integers are code - zero for many rows; for few rows offset + code and offset + zero are summed apart,
+128 + 15 at most each: terms of up to 286 * scale * |x| in all.
 Outputs are rounded to bf16: 2^-8 of the value. In the experts, silu(g) * u is rounded to bf16
 between the products (2^-8 of each h, passed on by |w_down|), and |silu'| <= 1.1.
 Over a whole output the 2-norm of the difference stays below 2^-8 of the result's: a rounding's
@@ -42,10 +42,10 @@ def rows(seed, M, K):
 
 
 def most(w):
-    """62 * scale of every weight, rows as dequantize_w4 gives them."""
+    """286 * scale of every weight, rows as dequantize_w4 gives them."""
     zeros = torch.zeros(w.scales.shape, dtype=torch.uint8, device=w.device)
     ones = replace(w, qweight=torch.full_like(w.qweight, 0xff), zeros=zeros)
-    return dequantize_w4(ones, torch.float64) * (62 / 15)
+    return dequantize_w4(ones, torch.float64) * (286 / 15)
 
 
 def steps(w):
