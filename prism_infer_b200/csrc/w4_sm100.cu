@@ -520,9 +520,6 @@ __global__ void __launch_bounds__(Shape<kNarrow>::kThreads, Shape<kNarrow>::kCta
           for (int j = 0; j < PG; ++j)
             zr[r][j] = kZeros ? (((z >> (8 * j)) & 0xfu) * 0x00010001u) | 0x43004300u : 0x43084308u;
         }
-        __syncwarp();
-        if (lane == 0) bar_arrive(pk_empty + 8 * pk.slot);
-        pk.next();
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           if (!wait(empty + 8 * st.slot, st.phase ^ 1)) return false;
@@ -548,6 +545,11 @@ __global__ void __launch_bounds__(Shape<kNarrow>::kThreads, Shape<kNarrow>::kCta
           if (lane == 0) bar_arrive(full + 8 * st.slot);
           st.next();
         }
+        // given back once the stores above have used it: an arrival right after the loads can overtake
+        // them, and the next copy then lands under a load in flight
+        __syncwarp();
+        if (lane == 0) bar_arrive(pk_empty + 8 * pk.slot);
+        pk.next();
       }
       return true;
     });
@@ -559,6 +561,7 @@ __global__ void __launch_bounds__(Shape<kNarrow>::kThreads, Shape<kNarrow>::kCta
     constexpr int kPairs = kNarrow ? 32 : 64;          // pairs of columns held, at most
     Ring<P::kBufs> buf;
     Ring<S::kScaleSlots> sl;
+    int held = -1;
     const int row = q * 32 + lane;                     // weight row in the tile
     const bool ok = for_tiles([&](const Tile& t) {
       const int left = kNarrow ? t.cols : (t.cols / 16 + 1) / 2 * 16;   // columns of side 0
@@ -572,8 +575,10 @@ __global__ void __launch_bounds__(Shape<kNarrow>::kThreads, Shape<kNarrow>::kCta
         const uint2 raw = lds_small<2 * PG>(scales + sl.slot * S::kScaleSlot + row * 2 * PG);
         const float sc[4] = {__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xffff0000u),
                              __uint_as_float(raw.y << 16), __uint_as_float(raw.y & 0xffff0000u)};
+        // the slot before this one is given back now, when its scales have been used for certain
         __syncwarp();
-        if (lane == 0) bar_arrive(sc_empty + 8 * sl.slot);
+        if (lane == 0 && held >= 0) bar_arrive(sc_empty + 8 * held);
+        held = sl.slot;
         sl.next();
 #pragma unroll
         for (int gr = 0; gr < PG; ++gr) {

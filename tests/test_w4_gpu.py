@@ -142,6 +142,20 @@ def test_linear_rows_do_not_meet():
         assert y[1].isnan().all() and not y[2].isfinite().all()
 
 
+@pytest.mark.parametrize("M,N,K,G", [(8192, 4096, 1024, 128), (4096, 4096, 1024, 64),
+                                     (4096, 2048, 2048, 32), (64, 16384, 2048, 128),
+                                     (48, 16384, 2048, 32), (16, 16384, 2048, 128)])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_linear_large_grids_repeat(M, N, K, G, zeros):
+    """Thousands of tiles, many times: a hand-over between warps that is one instruction early shows in
+    a few tiles of a large grid only."""
+    w, x = weights(7, (), N, K, G, zeros), rows(8, M, K)
+    y = capi.linear_w4(x, w)
+    check_linear(x, w, y)
+    for _ in range(20):
+        assert torch.equal(capi.linear_w4(x, w), y)
+
+
 # ------------------------------------------------------------------------------------ experts
 
 EXPERTS = [
