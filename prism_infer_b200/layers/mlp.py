@@ -8,6 +8,8 @@ layers of Qwen3 models use: ``gate_up_proj`` is a ``MergedColumnParallelLinear``
 SwiGLU GEMMs: gate_up and SwiGLU in one tcgen05 launch (bf16; CUDA cores for fp32), down in
 the next. Parameter names and ``weight_loader`` signatures match the reference, so its
 ``load_model`` fills them unchanged. Tensor parallelism is not supported (world size 1 only).
+``quantize_`` turns a loaded MLP's weights into 4 bits with group scales (no counterpart in the
+reference).
 """
 from __future__ import annotations
 
@@ -15,6 +17,8 @@ import torch
 from torch import nn
 
 from prism_infer_b200 import ops  # noqa: F401  (registers torch.ops.prism_moe)
+from prism_infer_b200.layers.w4 import W4Holder
+from prism_infer_b200.quant import quantize_w4
 
 
 class MergedGateUp(nn.Module):
@@ -72,6 +76,18 @@ class Qwen3MLP(nn.Module):
         self.intermediate_size = intermediate_size
         self.gate_up_proj = MergedGateUp(hidden_size, [intermediate_size] * 2)
         self.down_proj = DownProj(intermediate_size, hidden_size)
+        self.w4_gate_up = self.w4_down = None
+
+    def quantize_(self, group_size: int = 128, *, symmetric: bool = True) -> "Qwen3MLP":
+        """Replace both weights by 4-bit ones (round to nearest); bf16 activations from then on."""
+        if self.w4_gate_up is not None:
+            raise RuntimeError("the MLP's weights are 4-bit already")
+        up, down = self.gate_up_proj.weight.data, self.down_proj.weight.data
+        self.w4_gate_up = W4Holder(quantize_w4(up.unsqueeze(0), group_size, symmetric=symmetric,
+                                               gate_up=True))
+        self.w4_down = W4Holder(quantize_w4(down.unsqueeze(0), group_size, symmetric=symmetric))
+        self.gate_up_proj = self.down_proj = None
+        return self
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         shape = x.shape
@@ -80,6 +96,12 @@ class Qwen3MLP(nn.Module):
             x2 = x2.contiguous()
         if x2.shape[0] == 0:
             return torch.empty_like(x)
+        if self.w4_gate_up is not None:
+            gu, dn = self.w4_gate_up, self.w4_down
+            y = torch.ops.prism_moe.expert_swiglu_w4(
+                x2, _one_segment(x2.shape[0], x2.device), gu.qweight, gu.scales, gu.zeros, dn.qweight,
+                dn.scales, dn.zeros, self.intermediate_size, gu.group_size, dn.group_size, None)
+            return y.view(shape)
         wgu = self.gate_up_proj.weight
         wd = self.down_proj.weight
         if x2.dtype != wgu.dtype:
