@@ -28,6 +28,7 @@
 // Every wait is bounded; one that runs out records PRISM_MOE_ERR_TIMEOUT and the CTA drains its
 // copies and MMAs before it frees TMEM.
 #include <algorithm>
+#include <type_traits>
 
 #include "gemm_sm100.cuh"
 #include "internal.h"
@@ -570,33 +571,42 @@ __global__ void __launch_bounds__(Shape<kNarrow>::kThreads, Shape<kNarrow>::kCta
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) acc[i] = make_float2(0.f, 0.f);
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + col0;
-      for (int i = 0, c = t.c0; i < p.chunks; ++i, c = next_chunk(c)) {
-        if (!wait(sc_full + 8 * sl.slot, sl.phase)) return false;
-        const uint2 raw = lds_small<2 * PG>(scales + sl.slot * S::kScaleSlot + row * 2 * PG);
-        const float sc[4] = {__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xffff0000u),
-                             __uint_as_float(raw.y << 16), __uint_as_float(raw.y & 0xffff0000u)};
-        // the slot before this one is given back now, when its scales have been used for certain
-        __syncwarp();
-        if (lane == 0 && held >= 0) bar_arrive(sc_empty + 8 * held);
-        held = sl.slot;
-        sl.next();
-#pragma unroll
-        for (int gr = 0; gr < PG; ++gr) {
-          if (!wait(acc_full + 8 * buf.slot, buf.phase)) return false;
-          tc_fence_after();
-          const uint32_t at = taddr + buf.slot * kTok;
-          // few columns, or all 128 (64) of this side (those past ncols hold what an earlier tile
-          // left there and are never stored)
-          if (ncols > 32)
-            add_scaled<kPairs / 16>(acc, at, sc[gr]);
-          else if (ncols > 0)
-            add_scaled<1>(acc, at, sc[gr]);
-          tc_fence_before();
+      // every chunk of the tile, 32 kBatches columns of each group (those past ncols hold what an
+      // earlier tile left there and are never stored)
+      auto add_chunks = [&](auto batches) {
+        constexpr int kBatches = decltype(batches)::value;
+        for (int i = 0; i < p.chunks; ++i) {
+          if (!wait(sc_full + 8 * sl.slot, sl.phase)) return false;
+          const uint2 raw = lds_small<2 * PG>(scales + sl.slot * S::kScaleSlot + row * 2 * PG);
+          const float sc[4] = {__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xffff0000u),
+                               __uint_as_float(raw.y << 16), __uint_as_float(raw.y & 0xffff0000u)};
+          // the slot before this one is given back now, when its scales have been used for certain
           __syncwarp();
-          if (lane == 0) bar_arrive(acc_empty + 8 * buf.slot);
-          buf.next();
+          if (lane == 0 && held >= 0) bar_arrive(sc_empty + 8 * held);
+          held = sl.slot;
+          sl.next();
+#pragma unroll
+          for (int gr = 0; gr < PG; ++gr) {
+            if (!wait(acc_full + 8 * buf.slot, buf.phase)) return false;
+            tc_fence_after();
+            if constexpr (kBatches > 0) add_scaled<kBatches>(acc, taddr + buf.slot * kTok, sc[gr]);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(acc_empty + 8 * buf.slot);
+            buf.next();
+          }
         }
+        return true;
+      };
+      bool done;
+      switch ((ncols + 31) >> 5) {   // once per tile: a choice per group would copy the sums about
+        case 0: done = add_chunks(std::integral_constant<int, 0>{}); break;
+        case 1: done = add_chunks(std::integral_constant<int, 1>{}); break;
+        case 2: done = add_chunks(std::integral_constant<int, 2>{}); break;
+        case 3: done = add_chunks(std::integral_constant<int, kNarrow ? 2 : 3>{}); break;
+        default: done = add_chunks(std::integral_constant<int, kNarrow ? 2 : 4>{}); break;
       }
+      if (!done) return false;
       // ---- output: lanes are outputs of one activation row; 8 lanes swap 8 columns for 16-byte stores
       const int64_t ld = p.n_out;
       if constexpr (kSwiGLU) {
