@@ -607,7 +607,10 @@ __global__ void __launch_bounds__(Shape<kNarrow>::kThreads, Shape<kNarrow>::kCta
         default: done = add_chunks(std::integral_constant<int, kNarrow ? 2 : 4>{}); break;
       }
       if (!done) return false;
-      // ---- output: lanes are outputs of one activation row; 8 lanes swap 8 columns for 16-byte stores
+      // ---- output: lanes are outputs of one activation row; 8 lanes swap 8 columns for 16-byte stores.
+      // A short loop over sums that move up costs less than the same code laid out for all of them,
+      // which a tile's end always finds out of the instruction cache.
+      constexpr int kTurn = 8;   // pairs of columns per turn
       const int64_t ld = p.n_out;
       if constexpr (kSwiGLU) {
         // lanes 0-7 and 16-23 hold gate rows, the lanes 8 above them the matching up rows; of two
@@ -617,31 +620,41 @@ __global__ void __launch_bounds__(Shape<kNarrow>::kThreads, Shape<kNarrow>::kCta
         const int mine = col0 + 2 * (lane & 7) + (up ? 1 : 0);
         uint16_t* to = p.out + (t.row0 + mine) * ld + n;
         const int rows = n < p.n_out ? t.rows - mine : 0;
+#pragma unroll 1
+        for (int b = 0; b < kPairs && 2 * b < ncols; b += kTurn) {
 #pragma unroll
-        for (int b = 0; b < kPairs; b += 8) {
-          if (2 * b >= ncols) break;
-          float h[8];
+          for (int j = 0; j < kTurn; j += 8) {
+            float h[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float2 a = acc[b + i];
-            const float got = __shfl_xor_sync(0xffffffffu, up ? a.x : a.y, 8);
-            h[i] = silu_mul(up ? got : a.x, up ? a.y : got);
+            for (int i = 0; i < 8; ++i) {
+              const float2 a = acc[j + i];
+              const float got = __shfl_xor_sync(0xffffffffu, up ? a.x : a.y, 8);
+              h[i] = silu_mul(up ? got : a.x, up ? a.y : got);
+            }
+            const uint4 d = transpose8(h, lane);
+            if (2 * (b + j) < rows) *reinterpret_cast<uint4*>(to) = d;
+            to += 16 * ld;
           }
-          const uint4 d = transpose8(h, lane);
-          if (2 * b < rows) *reinterpret_cast<uint4*>(to + 2 * b * ld) = d;
+#pragma unroll
+          for (int i = 0; i + kTurn < kPairs; ++i) acc[i] = acc[i + kTurn];
         }
       } else {
         const int n = t.mt * kRowsW + q * 32 + (lane & 24);
         const int mine = col0 + (lane & 7);
         uint16_t* to = p.out + (t.row0 + mine) * ld + n;
         const int rows = n < p.n_out ? t.rows - mine : 0;
+#pragma unroll 1
+        for (int b = 0; b < kPairs && 2 * b < ncols; b += kTurn) {
 #pragma unroll
-        for (int b = 0; b < kPairs; b += 4) {
-          if (2 * b >= ncols) break;
-          const float v[8] = {acc[b].x,     acc[b].y,     acc[b + 1].x, acc[b + 1].y,
-                              acc[b + 2].x, acc[b + 2].y, acc[b + 3].x, acc[b + 3].y};
-          const uint4 d = transpose8(v, lane);
-          if (2 * b < rows) *reinterpret_cast<uint4*>(to + 2 * b * ld) = d;
+          for (int j = 0; j < kTurn; j += 4) {
+            const float v[8] = {acc[j].x,     acc[j].y,     acc[j + 1].x, acc[j + 1].y,
+                                acc[j + 2].x, acc[j + 2].y, acc[j + 3].x, acc[j + 3].y};
+            const uint4 d = transpose8(v, lane);
+            if (2 * (b + j) < rows) *reinterpret_cast<uint4*>(to) = d;
+            to += 8 * ld;
+          }
+#pragma unroll
+          for (int i = 0; i + kTurn < kPairs; ++i) acc[i] = acc[i + kTurn];
         }
       }
       return true;
