@@ -138,30 +138,6 @@ __device__ __forceinline__ void add_scaled(float2 (&acc)[kPairs], uint32_t taddr
   }
 }
 
-// Lane l of each 8 holds 8 values (columns) of output l: gives it the 8 outputs of column l, in bf16.
-__device__ __forceinline__ uint4 transpose8(const float (&v)[8], int lane) {
-  uint32_t r[4];
-  const bool b0 = lane & 1, b1 = lane & 2, b2 = lane & 4;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {   // (column 2 j, 2 j + 1) -> outputs (l & ~1, l | 1) of column 2 j + b0
-    const uint32_t own = cvt_bf16x2(v[2 * j], v[2 * j + 1]);
-    const uint32_t got = __shfl_xor_sync(0xffffffffu, own, 1);
-    r[j] = __byte_perm(own, got, b0 ? 0x3276 : 0x5410);
-  }
-  // four outputs of columns b0 + 2 b1 (+ 4): the other half goes to the lane two away
-  uint32_t p[2][2];
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const uint32_t got = __shfl_xor_sync(0xffffffffu, b1 ? r[2 * j] : r[2 * j + 1], 2);
-    p[j][0] = b1 ? got : r[2 * j];
-    p[j][1] = b1 ? r[2 * j + 1] : got;
-  }
-  uint32_t q[2];
-#pragma unroll
-  for (int j = 0; j < 2; ++j) q[j] = __shfl_xor_sync(0xffffffffu, b2 ? p[0][j] : p[1][j], 4);
-  return b2 ? make_uint4(q[0], q[1], p[1][0], p[1][1]) : make_uint4(p[0][0], p[0][1], q[0], q[1]);
-}
-
 // One lane of a converged warp.
 __device__ __forceinline__ bool elect_one() {
   uint32_t ok;
@@ -607,54 +583,35 @@ __global__ void __launch_bounds__(Shape<kNarrow>::kThreads, Shape<kNarrow>::kCta
         default: done = add_chunks(std::integral_constant<int, kNarrow ? 2 : 4>{}); break;
       }
       if (!done) return false;
-      // ---- output: lanes are outputs of one activation row; 8 lanes swap 8 columns for 16-byte stores.
-      // A short loop over sums that move up costs less than the same code laid out for all of them,
-      // which a tile's end always finds out of the instruction cache.
-      constexpr int kTurn = 8;   // pairs of columns per turn
+      // ---- output: a lane is one output of every activation row, so 32 lanes store 64 bytes of a row
+      // (16-byte stores after swapping columns between lanes took half as long again: the shuffles
+      // cost more than the stores they save)
       const int64_t ld = p.n_out;
       if constexpr (kSwiGLU) {
         // lanes 0-7 and 16-23 hold gate rows, the lanes 8 above them the matching up rows; of two
         // columns the gate lane finishes the first, the up lane the second
         const bool up = lane & 8;
-        const int n = (t.mt * kRowsW + q * 32) / 2 + (lane >> 4) * 8;
-        const int mine = col0 + 2 * (lane & 7) + (up ? 1 : 0);
+        const int n = (t.mt * kRowsW + q * 32) / 2 + (lane >> 4) * 8 + (lane & 7);
+        const int mine = col0 + (up ? 1 : 0);
         uint16_t* to = p.out + (t.row0 + mine) * ld + n;
-        const int rows = n < p.n_out ? t.rows - mine : 0;
-#pragma unroll 1
-        for (int b = 0; b < kPairs && 2 * b < ncols; b += kTurn) {
+        const int rows = n < p.n_out ? min(t.rows, col0 + ncols) - mine : 0;
 #pragma unroll
-          for (int j = 0; j < kTurn; j += 8) {
-            float h[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float2 a = acc[j + i];
-              const float got = __shfl_xor_sync(0xffffffffu, up ? a.x : a.y, 8);
-              h[i] = silu_mul(up ? got : a.x, up ? a.y : got);
-            }
-            const uint4 d = transpose8(h, lane);
-            if (2 * (b + j) < rows) *reinterpret_cast<uint4*>(to) = d;
-            to += 16 * ld;
-          }
-#pragma unroll
-          for (int i = 0; i + kTurn < kPairs; ++i) acc[i] = acc[i + kTurn];
+        for (int i = 0; i < kPairs; ++i) {
+          const float got = __shfl_xor_sync(0xffffffffu, up ? acc[i].x : acc[i].y, 8);
+          const float h = silu_mul(up ? got : acc[i].x, up ? acc[i].y : got);
+          if (2 * i < rows) *to = float_to_bf16_bits(h);
+          to += 2 * ld;
         }
       } else {
-        const int n = t.mt * kRowsW + q * 32 + (lane & 24);
-        const int mine = col0 + (lane & 7);
-        uint16_t* to = p.out + (t.row0 + mine) * ld + n;
-        const int rows = n < p.n_out ? t.rows - mine : 0;
-#pragma unroll 1
-        for (int b = 0; b < kPairs && 2 * b < ncols; b += kTurn) {
+        const int n = t.mt * kRowsW + row;
+        uint16_t* to = p.out + (t.row0 + col0) * ld + n;
+        const int rows = n < p.n_out ? min(ncols, t.rows - col0) : 0;
 #pragma unroll
-          for (int j = 0; j < kTurn; j += 4) {
-            const float v[8] = {acc[j].x,     acc[j].y,     acc[j + 1].x, acc[j + 1].y,
-                                acc[j + 2].x, acc[j + 2].y, acc[j + 3].x, acc[j + 3].y};
-            const uint4 d = transpose8(v, lane);
-            if (2 * (b + j) < rows) *reinterpret_cast<uint4*>(to) = d;
-            to += 8 * ld;
-          }
-#pragma unroll
-          for (int i = 0; i + kTurn < kPairs; ++i) acc[i] = acc[i + kTurn];
+        for (int i = 0; i < kPairs; ++i) {
+          const uint32_t d = cvt_bf16x2(acc[i].x, acc[i].y);
+          if (2 * i < rows) to[0] = static_cast<uint16_t>(d);
+          if (2 * i + 1 < rows) to[ld] = static_cast<uint16_t>(d >> 16);
+          to += 2 * ld;
         }
       }
       return true;
