@@ -200,7 +200,8 @@ int prism_moe_expert_swiglu(const void* x_sorted, int dtype, int64_t rows_capaci
  * 4-bit weights with group scales: W[n, k] = (code[n, k] - zero) * scale, one scale (and zero
  * point) per row and group of group_size (32, 64 or 128) consecutive inputs; K must be a multiple of
  * group_size. Held in tiles of 16 rows by 128 inputs (N padded to 16, K to 128; the padding's codes
- * may be anything, its scales must be finite):
+ * may be anything). Scales must be finite, the padding's too: a row tile's products may also meet the
+ * scales next to it, with activations of zero.
  *   qweight [N/16][ceil(K/128)][16][64] bytes: a row's 64 bytes are 16 little-endian words of 8
  *           codes, the word at 4 t + j (t, j < 4) holding inputs 32 j + 8 t .. + 7, nibbles from the
  *           low end in the order 0 2 4 6 1 3 5 7 of the eight
@@ -220,11 +221,13 @@ typedef struct prism_moe_w4 {
 /*
  * y = x W^T for 4-bit weights: x [rows, in_features] and y [rows, out_features] bf16, row-major,
  * 16-byte aligned, out_features % 8 == 0; any number of rows, one (a matrix-vector product)
- * included. Sums are fp32, scales are applied to fp32 group sums, y is rounded once.
+ * included. Sums are fp32, scales are applied to fp32 group sums, y is rounded once. y must not overlap
+ * x. A row of x that holds an infinity or NaN gives outputs that are infinite or NaN, in that row only.
+ * ``device_error``: int32 device word, or NULL; a wait inside a kernel that runs out is recorded there.
  * Replaces F.linear of prism_infer/layers/linear.py:77,181 on quantised weights.
  */
 int prism_moe_linear_w4(const void* x, int64_t rows, int64_t in_features, int64_t out_features,
-                        const prism_moe_w4* weight, void* y, void* stream);
+                        const prism_moe_w4* weight, void* y, int* device_error, void* stream);
 
 /* Bytes of scratch prism_moe_expert_swiglu_w4 needs. */
 size_t prism_moe_expert_w4_workspace_size(int64_t rows_capacity, int64_t inter);
@@ -233,8 +236,9 @@ size_t prism_moe_expert_w4_workspace_size(int64_t rows_capacity, int64_t inter);
  * prism_moe_expert_swiglu on 4-bit weights (bf16 activations): w_gate_up stacks num_local_experts
  * matrices [2I, H] (gate and up rows by turns, as above), w_down as many [H, I]. hidden and inter
  * must be multiples of their matrix's group size. The gate and up sums stay in fp32; their product
- * silu(g) * u is rounded to bf16, the operand type of the second product. Rows of no segment are
- * left as they are; a segment whose seg_expert lies outside [0, num_local_experts) is skipped and
+ * silu(g) * u is rounded to bf16, the operand type of the second product. seg_offsets as there, up to
+ * 1024 segments; NULL: one segment of all rows. Any number of segments may name the same expert. y may
+ * be x_sorted. Rows of no segment are left as they are; a segment whose seg_expert lies outside [0, num_local_experts) is skipped and
  * records PRISM_MOE_ERR_ARG in ``device_error``.
  */
 int prism_moe_expert_swiglu_w4(const void* x_sorted, int64_t rows_capacity, int64_t hidden,

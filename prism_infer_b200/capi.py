@@ -59,7 +59,7 @@ _SIGNATURES = {
     "prism_moe_route_scored": (ctypes.c_int, [_vp, ctypes.c_int, _i64, _i32, _i32,
                                               ctypes.POINTER(Router), _vp, _vp, ctypes.c_int,
                                               _vp, _vp]),
-    "prism_moe_linear_w4": (ctypes.c_int, [_vp, _i64, _i64, _i64, _w4p, _vp, _vp]),
+    "prism_moe_linear_w4": (ctypes.c_int, [_vp, _i64, _i64, _i64, _w4p, _vp, _vp, _vp]),
     "prism_moe_expert_w4_workspace_size": (_sz, [_i64, _i64]),
     "prism_moe_expert_swiglu_w4": (ctypes.c_int, [_vp, _i64, _i64, _i64, _vp, _vp, _i32, _i32,
                                                   _w4p, _w4p, _vp, _vp, _sz, _vp, _vp]),
@@ -336,9 +336,10 @@ def _need_bf16(x, what: str) -> None:
         raise RuntimeError(f"{what}: 4-bit weights take bfloat16 activations, got {x.dtype}")
 
 
-def linear_w4(x, weight, out=None):
+def linear_w4(x, weight, out=None, device_error=None):
     """y = x W^T for a 4-bit ``weight`` (``quant.W4Weight``, a single matrix): ``x`` [M, K] bf16, any
-    M from 0; returns [M, N] bf16 (prism_moe_linear_w4)."""
+    M from 0; returns [M, N] bf16 (``out``, which must not overlap ``x``). ``device_error``: an int32
+    device word that a failing kernel records its status in (prism_moe_linear_w4)."""
     torch = _torch()
     _need_bf16(x, "linear_w4")
     if weight.stack is not None or weight.gate_up:
@@ -346,14 +347,16 @@ def linear_w4(x, weight, out=None):
     if x.dim() != 2 or x.shape[1] != weight.in_features:
         raise RuntimeError(f"linear_w4: x {tuple(x.shape)} does not match {weight.in_features} "
                            "inputs")
-    dev = _one_device(x, weight.qweight, out)
+    dev = _one_device(x, weight.qweight, out, device_error)
+    if device_error is not None and device_error.dtype != torch.int32:
+        raise RuntimeError("linear_w4: device_error must be int32")
     M, N = x.shape[0], weight.out_features
     if out is None:
         out = x.new_empty((M, N))
     elif tuple(out.shape) != (M, N) or out.dtype != x.dtype:
         raise RuntimeError("linear_w4: out must be [M, N] in x's dtype")
     _launch(dev, "prism_moe_linear_w4", load().prism_moe_linear_w4, x.data_ptr(), M,
-            weight.in_features, N, ctypes.byref(_w4(weight)), out.data_ptr())
+            weight.in_features, N, ctypes.byref(_w4(weight)), out.data_ptr(), ptr(device_error))
     return out
 
 
@@ -371,7 +374,7 @@ def expert_swiglu_w4(x_sorted, seg_offsets, w_gate_up, w_down, seg_expert=None, 
                      device_error=None):
     """Grouped SwiGLU experts on 4-bit weights (``quant.W4Weight`` stacks) over the segment table:
     ``expert_swiglu`` with ``w_gate_up`` [El, 2I, H] and ``w_down`` [El, H, I] in 4 bits and bf16
-    activations (prism_moe_expert_swiglu_w4)."""
+    activations (prism_moe_expert_swiglu_w4). ``seg_offsets`` None: all rows are one segment."""
     torch = _torch()
     _need_bf16(x_sorted, "expert_swiglu_w4")
     if x_sorted.dim() != 2:
@@ -380,7 +383,7 @@ def expert_swiglu_w4(x_sorted, seg_offsets, w_gate_up, w_down, seg_expert=None, 
     El, I = _expert_shapes("expert_swiglu_w4", H, w_gate_up, w_down)
     dev = _one_device(x_sorted, seg_offsets, seg_expert, w_gate_up.qweight, w_down.qweight, y,
                       device_error)
-    nseg = seg_offsets.numel() - 1
+    nseg = 1 if seg_offsets is None else seg_offsets.numel() - 1
     for name, t in (("seg_offsets", seg_offsets), ("seg_expert", seg_expert),
                     ("device_error", device_error)):
         if t is not None and t.dtype != torch.int32:
@@ -397,7 +400,7 @@ def expert_swiglu_w4(x_sorted, seg_offsets, w_gate_up, w_down, seg_expert=None, 
     ws_bytes = lib.prism_moe_expert_w4_workspace_size(R, I)
     ws = x_sorted.new_empty((max(ws_bytes, 1),), dtype=torch.uint8)
     _launch(dev, "prism_moe_expert_swiglu_w4", lib.prism_moe_expert_swiglu_w4,
-            x_sorted.data_ptr(), R, H, I, seg_offsets.data_ptr(), ptr(seg_expert), nseg, El,
+            x_sorted.data_ptr(), R, H, I, ptr(seg_offsets), ptr(seg_expert), nseg, El,
             ctypes.byref(_w4(w_gate_up)), ctypes.byref(_w4(w_down)), y.data_ptr(), ws.data_ptr(),
             ws_bytes, ptr(device_error))
     return y

@@ -336,13 +336,16 @@ int prism_moe_expert_swiglu(const void* x_sorted, int dtype, int64_t rows_capaci
 }
 
 int prism_moe_linear_w4(const void* x, int64_t rows, int64_t in_features, int64_t out_features,
-                        const prism_moe_w4* weight, void* y, void* stream) {
+                        const prism_moe_w4* weight, void* y, int* device_error, void* stream) {
   PRISM_CHECK_ARG(rows >= 0 && in_features >= 1 && out_features >= 1, "linear_w4: bad shape");
   PRISM_CHECK_ARG(rows < (int64_t(1) << 31), "linear_w4: too many rows");
   if (int r = check_w4("linear_w4", weight, in_features, out_features)) return r;
   PRISM_CHECK_ARG(rows == 0 || (x && y), "linear_w4: null pointer");
   PRISM_CHECK_ARG((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) % 16 == 0,
                   "linear_w4: buffers must be 16-byte aligned");
+  const uintptr_t x0 = reinterpret_cast<uintptr_t>(x), y0 = reinterpret_cast<uintptr_t>(y);
+  PRISM_CHECK_ARG(x0 + 2 * rows * in_features <= y0 || y0 + 2 * rows * out_features <= x0 || rows == 0,
+                  "linear_w4: y overlaps x");
   if (int r = check_device()) return r;
   if (rows == 0) return PRISM_MOE_OK;
   W4Problem p;
@@ -352,6 +355,7 @@ int prism_moe_linear_w4(const void* x, int64_t rows, int64_t in_features, int64_
   p.n_out = out_features;
   p.w = *weight;
   p.out = y;
+  p.err = device_error;
   return w4_product(p, static_cast<cudaStream_t>(stream));
 }
 
@@ -375,8 +379,11 @@ int prism_moe_expert_swiglu_w4(const void* x_sorted, int64_t rows_capacity, int6
   if (int r = check_w4("expert_swiglu_w4", w_down, inter, hidden)) return r;
   PRISM_CHECK_ARG(workspace_bytes >= w4_scratch_bytes(rows_capacity, inter),
                   "expert_swiglu_w4: workspace too small");
-  PRISM_CHECK_ARG(rows_capacity == 0 || (x_sorted && seg_offsets && y && workspace),
+  PRISM_CHECK_ARG(rows_capacity == 0 || (x_sorted && y && workspace),
                   "expert_swiglu_w4: null pointer");
+  PRISM_CHECK_ARG(seg_offsets || num_segments == 1,
+                  "expert_swiglu_w4: without seg_offsets all rows are one segment, not %d",
+                  num_segments);
   PRISM_CHECK_ARG((reinterpret_cast<uintptr_t>(x_sorted) | reinterpret_cast<uintptr_t>(y) |
                    reinterpret_cast<uintptr_t>(workspace)) % 16 == 0,
                   "expert_swiglu_w4: buffers must be 16-byte aligned");

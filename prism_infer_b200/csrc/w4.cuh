@@ -59,26 +59,6 @@ __device__ __forceinline__ void load_scales(const uint16_t* p, float (&s)[PG]) {
   }
 }
 
-// 128 + zero as a bf16 pair for each of the PG groups; 8 without zero points.
-template <int PG, bool kZeros>
-__device__ __forceinline__ void load_zeros(const uint8_t* z, int64_t at, uint32_t (&out)[PG]) {
-  if constexpr (!kZeros) {
-#pragma unroll
-    for (int i = 0; i < PG; ++i) out[i] = 0x43084308u;
-  } else {
-    uint32_t v;
-    if constexpr (PG == 1)
-      v = z[at];
-    else if constexpr (PG == 2)
-      v = *reinterpret_cast<const uint16_t*>(z + at);
-    else
-      v = *reinterpret_cast<const uint32_t*>(z + at);
-#pragma unroll
-    for (int i = 0; i < PG; ++i)
-      out[i] = (((v >> (8 * i)) & 0xfu) * 0x00010001u) | 0x43004300u;
-  }
-}
-
 // The zero point of each of the PG groups.
 template <int PG>
 __device__ __forceinline__ void load_zero_points(const uint8_t* z, float (&out)[PG]) {
@@ -112,11 +92,10 @@ __device__ __forceinline__ RowSpan segment_rows(const int32_t* seg_offsets, int 
 }
 
 // Warp-cooperative: prefix[s] = row blocks (of ``bm`` rows) before segment s, prefix[nseg] = all.
-// Only segments of more than ``min_rows`` and at most ``max_rows`` rows count.
+// Only segments of more than ``min_rows`` rows count.
 __device__ __forceinline__ void build_row_blocks(const int32_t* seg_offsets, int nseg,
                                                  int64_t rows_cap, int bm, int32_t* prefix,
-                                                 int64_t min_rows = 0,
-                                                 int64_t max_rows = int64_t(1) << 31) {
+                                                 int64_t min_rows) {
   const int lane = threadIdx.x & 31;
   int32_t carry = 0;
   for (int base = 0; base < nseg; base += 32) {
@@ -125,7 +104,7 @@ __device__ __forceinline__ void build_row_blocks(const int32_t* seg_offsets, int
     if (s < nseg) {
       const RowSpan r = segment_rows(seg_offsets, s, rows_cap);
       const int64_t len = r.end - r.begin;
-      n = len > min_rows && len <= max_rows ? static_cast<int32_t>((len + bm - 1) / bm) : 0;
+      n = len > min_rows ? static_cast<int32_t>((len + bm - 1) / bm) : 0;
     }
     int32_t incl = n;
 #pragma unroll
@@ -139,8 +118,9 @@ __device__ __forceinline__ void build_row_blocks(const int32_t* seg_offsets, int
   if (lane == 0) prefix[nseg] = carry;
 }
 
-// The same by all threads of a block (at most 1024 segments, blocks of up to 256 threads): every
-// offset is loaded at once, so the list costs one memory latency. Ends with a barrier.
+// The same by all threads of a block (at most 1024 segments, blocks of up to 256 threads), counting
+// segments of at most ``max_rows`` rows: every offset is loaded at once, so the list costs one memory
+// latency. Ends with a barrier.
 __device__ __forceinline__ void build_row_blocks_cta(const int32_t* seg_offsets, int nseg,
                                                      int64_t rows_cap, int bm, int32_t* prefix,
                                                      int64_t max_rows) {

@@ -22,9 +22,16 @@
 //   warps 4-7     decode: 16 bytes (four words) per lane and row -> K-major, swizzled bf16 A tile
 //   warps 8-15    accumulate (8-11 for narrow tiles): two warps per TMEM lane quarter, each half of the
 //                 columns; a lane owns one weight row, so a group's scale is one register
-// Stages hold 64 inputs (A 16 KB + B 32 KB, four of them); a stage is full when its copies have
-// landed and the four decoding warps have arrived. Two TMEM buffers of 256 columns take turns, one
-// group each. Registers are split per warpgroup (Shape).
+// Stages hold 64 inputs (wide tiles: A 16 KB + B 32 KB, four of them); a stage is full when its copies
+// have landed and the four decoding warps have arrived. TMEM buffers (two of 256 columns) take turns,
+// one group each. Registers are split per warpgroup (Shape).
+//
+// What bounds it: with groups of 128 a chunk of 128 inputs takes a wide tile about 1450 cycles where
+// its eight MMAs need 1024; the accumulating warps' TMEM loads and multiply-adds are nearly as long,
+// and four reads of the accumulator per chunk bound groups of 32. A tile's output adds about 5400 cycles
+// in which the MMAs stand (no third TMEM buffer fits).
+// Measured: 8192 x 4736 x 4096, groups of 128: 268 us (1184 TFLOP/s); of 64 with zero points 318 us
+// (1001); of 32 469 us (678). 8192 tokens of 32 experts, top 4, 4096 x 1024: 901 us (915).
 // Every wait is bounded; one that runs out records PRISM_MOE_ERR_TIMEOUT and the CTA drains its
 // copies and MMAs before it frees TMEM.
 #include <algorithm>
@@ -38,7 +45,10 @@ namespace prism {
 namespace {
 
 constexpr int kRowsW = 128;      // weight rows per tile
-constexpr int kNarrowRows = 64;  // average rows per segment up to which tiles are narrow
+// Average rows per segment up to which tiles are narrow. 128 experts of 2048 x 768, groups of 128,
+// both products, narrow and wide: 32 rows on average 211 and 303 us, 64 rows 297 and 322, 96 rows 373
+// and 324. One segment, 18944 x 4096: 64 rows 35.0 and 36.9 us, 96 rows 45 and 37.
+constexpr int kNarrowRows = 64;
 constexpr int kTokBox = 64;      // activation rows per copy
 constexpr int kPackStage = 8 * 1024;
 constexpr size_t kPrefixW4 = ((kMaxW4Segments + 1) * 4 + 15) / 16 * 16;
@@ -710,7 +720,6 @@ int w4_product_large(const W4Problem& pr, int min_rows, cudaStream_t st) {
   if (p.z)
     if (int r = tiles_map(&map.z, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.z, 16 * pg, 16 * pg)) return r;
   const int64_t long_segs = std::min<int64_t>(pr.nseg, pr.rows_cap / (min_rows + 1));
-  // tens of rows per segment: narrow tiles (measured: see the table at Shape)
   const bool narrow = pr.rows_cap <= kNarrowRows * static_cast<int64_t>(pr.nseg);
   const int64_t items = (pr.rows_cap / (narrow ? 64 : 256) + long_segs) * p.tiles_n;
   PRISM_CHECK_ARG(items < (int64_t(1) << 31), "4-bit product: too many tiles");

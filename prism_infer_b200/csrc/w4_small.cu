@@ -21,6 +21,11 @@
 // magnitudes at 4096 inputs where the output's rounding is 2^-8.
 //
 // What bounds it: few rows reuse nothing, so every hit weight crosses HBM once and that is the floor.
+// Decoding comes next: a tile of 2048 codes is 64 instructions a warp (shifts, logic) beside 32 of the
+// tensor cores, and they, not HBM, set the rate when every SM is busy. Measured: 18944 x 4096 for 1 row
+// 18.4 us (2.1 TB/s of codes), 16 rows 24.7 us; 64 tokens of 128 experts, top 8, 2048 x 768, both
+// products 89 us (3.4 TB/s); one token of them 17 us, where two launches and three memory latencies are
+// most of it.
 // A block's warps split the inputs (kw ways) and keep their part of x in registers while the block
 // streams its row tiles; the partial sums meet in shared memory in a fixed order. Every lane copies
 // the 16-byte pieces that it will use itself (cp.async, kDepth row tiles ahead, across the borders
@@ -443,8 +448,11 @@ int launch_small(SmallParams p, int64_t units, cudaStream_t st) {
 
 template <int G, bool kZeros, bool kSwiGLU>
 int launch_rows(const SmallParams& p, int64_t units8, int64_t units16, cudaStream_t st) {
-  // 16 rows at a time once segments average more than 5
-  if (p.rows_cap > 5 * static_cast<int64_t>(p.nseg))
+  // 8 rows at a time (two blocks share an SM) while most segments have no more, else 16. 128 experts of
+  // 2048 x 768, groups of 128, both products, 8 or 16 at a time: 4 rows on average 96 and 150 us,
+  // 6 rows 104 and 158, 8 rows 127 and 160; groups of 64: 8 rows 170 and 158; 8 experts of 4096 x 1024
+  // with 6 rows 39 and 35. One segment of 8 rows, 18944 x 4096: 20.5 and 22.5; of 9: 28.7 and 22.5.
+  if (p.rows_cap > (p.seg_offsets ? 7 * static_cast<int64_t>(p.nseg) : 8))
     return launch_small<G, kZeros, kSwiGLU, 2>(p, units16, st);
   return launch_small<G, kZeros, kSwiGLU, 1>(p, units8, st);
 }
@@ -472,6 +480,8 @@ int w4_product(const W4Problem& pr, cudaStream_t st) {
   // 17 x 18944 x 4096: 39 and 33). With one: segments of 10 rows on average (1280 rows of 128
   // experts: 169 us here, 185 with both). Else segments of at most kSmallRows rows run here and longer
   // ones on the other kernel; the host does not know the lengths and launches both.
+  // the lists of row blocks and output tiles count in 32 bits
+  PRISM_CHECK_ARG(ceil_div(pr.rows_cap, 8) * pr.nseg < (int64_t(1) << 31), "4-bit product: too many rows");
   const int64_t out_tiles = ceil_div(pr.swiglu ? 2 * pr.n_out : pr.n_out, 16);
   const bool few = pr.seg_offsets
                        ? pr.rows_cap <= std::max<int64_t>(kSmallRows, 10 * pr.nseg)

@@ -98,9 +98,10 @@ class Qwen3MLP(nn.Module):
             return torch.empty_like(x)
         if self.w4_gate_up is not None:
             gu, dn = self.w4_gate_up, self.w4_down
+            if shape[-1] != self.hidden_size:
+                raise RuntimeError(f"input has {shape[-1]} features, not {self.hidden_size}")
             y = torch.ops.prism_moe.expert_swiglu_w4(
-                x2, _one_segment(x2.shape[0], x2.device), gu.qweight, gu.scales, gu.zeros, dn.qweight,
-                dn.scales, dn.zeros, self.intermediate_size, gu.group_size, dn.group_size, None)
+                x2, None, gu.qweight, gu.scales, gu.zeros, dn.qweight, dn.scales, dn.zeros, self.intermediate_size, gu.group_size, dn.group_size, None)
             return y.view(shape)
         wgu = self.gate_up_proj.weight
         wd = self.down_proj.weight

@@ -27,10 +27,11 @@ class W4Holder(nn.Module):
         self.gate_up = weight.gate_up
 
     def _apply(self, fn, recurse=True):
+        exact = self.scales
         super()._apply(fn, recurse)
-        # a model-wide change of type leaves the scales in bf16, their only type
+        # a model-wide change of type leaves the scales in bf16, their only type, and as they were
         if self.scales.dtype != torch.bfloat16:
-            self.scales = self.scales.to(torch.bfloat16)
+            self.scales = exact.to(self.scales.device)
         return self
 
     @property
@@ -54,6 +55,8 @@ class W4Linear(W4Holder):
         return cls(quantize_w4(weight.detach(), group_size, symmetric=symmetric))
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.shape[-1] != self.in_features:
+            raise RuntimeError(f"input has {x.shape[-1]} features, not {self.in_features}")
         x2 = x.reshape(-1, x.shape[-1]).contiguous()
         y = torch.ops.prism_moe.linear_w4(x2, self.qweight, self.scales, self.zeros,
                                           self.out_features, self.group_size)

@@ -36,7 +36,7 @@ Ops (shapes: T tokens, H hidden, E experts, k top-k, W expert-parallel ranks):
 * 4-bit weights (``quant.W4Weight`` as its tensors ``q, scales, zeros`` and group size):
   ``linear_w4(x[M,K], q, scales, zeros, out_features, group_size) -> y[M,N]``,
   ``expert_swiglu_w4(x_sorted, seg_offsets, gate_up q/scales/zeros, down q/scales/zeros, inter,
-  gate_up group, down group, seg_expert) -> y``, ``block_forward_w4`` / ``block_forward_w4_norm``:
+  gate_up group, down group, seg_expert) -> y`` (no ``seg_offsets``: one segment), ``block_forward_w4`` / ``block_forward_w4_norm``:
   the routed block on such experts.
 """
 from __future__ import annotations
@@ -282,7 +282,7 @@ def _(x, q, scales, zeros, out_features, group_size):
 
 
 @custom_op("prism_moe::expert_swiglu_w4", mutates_args=())
-def expert_swiglu_w4(x_sorted: Tensor, seg_offsets: Tensor, gu_q: Tensor, gu_scales: Tensor,
+def expert_swiglu_w4(x_sorted: Tensor, seg_offsets: Tensor | None, gu_q: Tensor, gu_scales: Tensor,
                      gu_zeros: Tensor | None, dn_q: Tensor, dn_scales: Tensor,
                      dn_zeros: Tensor | None, inter: int, gu_group: int, dn_group: int,
                      seg_expert: Tensor | None) -> Tensor:

@@ -155,6 +155,7 @@ def quantize_w4(weight: torch.Tensor, group_size: int = 128, *, symmetric: bool 
     """
     if group_size not in GROUP_SIZES:
         raise RuntimeError(f"group_size {group_size} is not one of {GROUP_SIZES}")
+    weight = weight.detach()
     *lead, N, K = weight.shape
     if K % group_size:
         raise RuntimeError(f"{K} inputs are not a multiple of group_size {group_size}")

@@ -251,6 +251,39 @@ def test_experts_operator_stream_and_graph():
     assert torch.equal(gy, y)
 
 
+@pytest.mark.parametrize("R,H,I", [(1, 384, 160), (17, 384, 160), (64, 384, 160), (65, 384, 160),
+                                   (700, 384, 160), (20, 256, 5632)])
+def test_experts_one_segment_of_all_rows(R, H, I):
+    """Without a table (the last case's two products run on different kernels); y may be the input."""
+    gu = weights(1, (1,), 2 * I, H, 64, True, gate_up=True)
+    dn = weights(2, (1,), H, I, 32, True)
+    x = rows(R, R, H)
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    y = capi.expert_swiglu_w4(x, None, gu, dn, device_error=err)
+    check_experts(x, [0, R], [0], gu, dn, y)
+    same = x.clone()
+    capi.expert_swiglu_w4(same, None, gu, dn, y=same)
+    assert torch.equal(same, y) and capi.read_device_error(err) == 0
+    two = weights(3, (2,), H, I, 32, True)
+    with pytest.raises(RuntimeError):                 # two experts, one segment: which one?
+        capi.expert_swiglu_w4(x, None, weights(1, (2,), 2 * I, H, 64, True, gate_up=True), two)
+
+
+def test_linear_out_and_error_word():
+    w = weights(1, (), 256, 256, 64, False)
+    x = rows(2, 40, 256)
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    y = capi.linear_w4(x, w, device_error=err)
+    check_linear(x, w, y)
+    assert capi.read_device_error(err) == 0
+    both = torch.zeros(60, 256, device=DEV, dtype=torch.bfloat16)
+    for out in (x, both[10:50]):
+        with pytest.raises(RuntimeError):
+            capi.linear_w4(both[:40] if out is not x else x, w, out=out)
+    with pytest.raises(RuntimeError):
+        capi.linear_w4(x, w, device_error=err.long())
+
+
 def test_quantised_close_to_the_weights():
     """Round-to-nearest: every value within half a step of its group's scale (and the bf16 scale's
     own rounding of the largest code)."""

@@ -142,11 +142,13 @@ def test_c_abi_refusals_need_no_gpu(lib):
 
     def linear(M=4, K=128, N=64, G=64, q=P, s=P, z=None, x=P, w=True):
         st = capi.W4(q, s, z, G)
-        return lib.prism_moe_linear_w4(x, M, K, N, ctypes.byref(st) if w else None, P, None)
+        return lib.prism_moe_linear_w4(x, M, K, N, ctypes.byref(st) if w else None, P, None,
+                                       None)
 
     for bad in (dict(M=-1), dict(K=0), dict(N=0), dict(G=16), dict(G=96), dict(K=96), dict(N=12),
                 dict(q=None), dict(s=None), dict(w=False), dict(x=None), dict(x=P + 2), dict(q=P + 4),
-                dict(s=P + 2), dict(z=P + 1), dict(M=1 << 31), dict(K=1 << 30)):
+                dict(s=P + 2), dict(z=P + 1), dict(M=1 << 31), dict(K=1 << 30), dict(),
+                dict(x=P + 64 * 2 * 4 - 16)):   # the last two: x is y, or starts inside it
         assert linear(**bad) == capi.ERR_ARG, bad
 
     def experts(R=4, H=128, I=64, nseg=2, El=2, ws=1 << 20, seg=P, Gu=64, Gd=64, y=P, x=P, wsp=P):
@@ -154,6 +156,7 @@ def test_c_abi_refusals_need_no_gpu(lib):
         return lib.prism_moe_expert_swiglu_w4(x, R, H, I, seg, None, nseg, El, ctypes.byref(gu),
                                               ctypes.byref(dn), y, wsp, ws, None, None)
 
+    assert experts(seg=None, nseg=2) == experts(seg=None, nseg=2, El=1) == capi.ERR_ARG
     for bad in (dict(R=-1), dict(H=0), dict(I=0), dict(nseg=0), dict(nseg=1025), dict(El=0),
                 dict(ws=16), dict(seg=None), dict(Gu=48), dict(Gd=128), dict(H=96), dict(y=None),
                 dict(x=P + 8), dict(wsp=P + 4), dict(R=1 << 31)):
@@ -222,8 +225,10 @@ def test_modules_refuse_and_keep_types():
     assert (dequantize_w4(moe.w4_down.weight) - dense).abs().max() < 0.5
     with pytest.raises(RuntimeError):
         moe.quantize_experts_(32)
-    again = moe.to(torch.float32).to(torch.bfloat16)
-    assert again.w4_down.scales.dtype == torch.bfloat16
+    scales = moe.w4_down.scales.clone().mul_(1e-6)      # below the range of float16
+    moe.w4_down.scales.copy_(scales)
+    again = moe.to(torch.float32).to(torch.float16).to(torch.bfloat16)
+    assert torch.equal(again.w4_down.scales, scales)
     mlp = Qwen3MLP(128, 64)
     for q in mlp.parameters():
         q.data.normal_()
@@ -232,6 +237,13 @@ def test_modules_refuse_and_keep_types():
         mlp.quantize_(32)
     with pytest.raises(RuntimeError):
         W4Linear(moe.w4_gate_up.weight)
+    # 96 and 128 inputs have the same number of tiles: the modules know which it is
+    lin = W4Linear.from_weight(torch.nn.Parameter(torch.randn(16, 96)), 32)
+    assert not lin.scales.requires_grad
+    with pytest.raises(RuntimeError):
+        lin(torch.zeros(1, 128, dtype=torch.bfloat16))
+    with pytest.raises(RuntimeError):
+        mlp(torch.zeros(1, 96, dtype=torch.bfloat16))
 
 
 def test_quantised_scored_block_exports_as_one_graph():
