@@ -79,6 +79,15 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
   return __fdividef(g, 1.f + __expf(-g)) * u;
 }
 
+// Programmatic launches: wait for the end (and the writes) of the kernel before this one; let the
+// next one start once every block has come here or ended.
+__device__ __forceinline__ void wait_for_earlier() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void launch_dependents() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 struct RowSpan {
   int64_t begin, end;
 };

@@ -49,6 +49,11 @@ constexpr int kTps = 2;         // row tiles per step
 constexpr int kMaxRt = 4;       // row tiles per item
 constexpr int kColStride = 20;  // floats between the columns of a partial tile: no bank conflicts
 
+// How a launch follows the kernel before it: after its end; early (it may start while that one ends,
+// and waits before it reads what that one wrote); beside it (it reads nothing that one writes, and
+// only ends after it).
+enum { kAfter, kEarly, kBeside };
+
 struct SmallParams {
   const uint16_t* x;
   int64_t ld_x;              // elements; = inputs
@@ -67,7 +72,7 @@ struct SmallParams {
   int blocks_n;              // ceil(tiles / rt)
   int all_chunks;            // of all matrices
   int64_t max_rows;          // longer segments are the other kernel's
-  int early;                 // may start while the kernel before it ends (see griddepcontrol)
+  int start;                 // kAfter, kEarly or kBeside
   int* err;
 };
 
@@ -78,10 +83,6 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
       "{%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ void wait_for_earlier() {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 template <int B>
@@ -135,8 +136,10 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 2 : 1) w4_small_kernel(
   const int64_t bid = blockIdx.x, blocks = gridDim.x;
   const int item0 = static_cast<int>(total * bid / blocks);
   const int item1 = static_cast<int>(total * (bid + 1) / blocks);
+  // a grid that ended before the one ahead of it would let the next one pass both
+  const bool hold = p.start == kEarly || blockIdx.x == 0;
   if (item0 >= item1) {
-    wait_for_earlier();   // a grid that ends before the one ahead of it would let the next one pass both
+    if (hold) wait_for_earlier();
     return;
   }
 
@@ -219,8 +222,8 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 2 : 1) w4_small_kernel(
 
   // From here on this kernel reads what the one before it wrote. Everything above (the list, the
   // weights in flight) may run while that one ends; a kernel behind may start likewise.
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  wait_for_earlier();
+  launch_dependents();
+  if (p.start != kBeside) wait_for_earlier();
   uint4 xb[kCh][NT][4];
   // sums over each group, columns 2 t and 2 t + 1: of offset * x (with zero point 8 where there are
   // none), and of x
@@ -391,6 +394,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 2 : 1) w4_small_kernel(
     }
   }
   copy_wait<0>();
+  if (p.start == kBeside && hold) wait_for_earlier();
 }
 
 template <int G, bool kZeros, bool kSwiGLU, int NT>
@@ -441,7 +445,7 @@ int launch_small(SmallParams p, int64_t units, cudaStream_t st) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = p.early ? 1 : 0;
+  cfg.numAttrs = p.start != kAfter ? 1 : 0;
   PRISM_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
   return PRISM_MOE_OK;
 }
@@ -492,7 +496,10 @@ int w4_product(const W4Problem& pr, cudaStream_t st) {
     if (!pr.seg_offsets) return PRISM_MOE_OK;
     p.max_rows = kSmallRows;
   }
-  p.early = few && pr.after_product;
+  // The two kernels of a product share neither rows nor weights, so this one fills the SMs that the
+  // other's last tiles leave (333 tokens of 60 experts, top 4, 1440 x 736, both products: 117 us, one
+  // kernel after the other 125; 1024 tokens 193 and 209).
+  p.start = !few ? kBeside : pr.after_product ? kEarly : kAfter;
   p.x = static_cast<const uint16_t*>(pr.x);
   p.ld_x = pr.K;
   p.K = static_cast<int>(pr.K);
