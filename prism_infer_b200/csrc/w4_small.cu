@@ -21,11 +21,12 @@
 // magnitudes at 4096 inputs where the output's rounding is 2^-8.
 //
 // What bounds it: few rows reuse nothing, so every hit weight crosses HBM once and that is the floor.
-// Decoding comes next: a tile of 2048 codes is 64 instructions a warp (shifts, logic) beside 32 of the
-// tensor cores, and they, not HBM, set the rate when every SM is busy. Measured: 18944 x 4096 for 1 row
-// 18.4 us (2.1 TB/s of codes), 16 rows 24.7 us; 64 tokens of 128 experts, top 8, 2048 x 768, both
-// products 89 us (3.4 TB/s); one token of them 17 us, where two launches and three memory latencies are
-// most of it.
+// What keeps it from that is latency inside the warps: 16 of them an SM, as many as registers allow, each
+// with copy, wait, decoding, product and sum in line (counters of the decode call below: HBM 46%, SM 48%
+// busy). More warps with fewer registers (24 of 80) spilled and took 10% longer, smaller and deeper
+// steps as well. Measured: 1 x 18944 x 4096 17.0 us (2.3 TB/s of codes), 16 rows 24.6; 64 tokens of 128
+// experts, top 8, 2048 x 768, both products 88 us (3.5 TB/s); one token of them 17, where two
+// launches and three memory latencies are most of it.
 // A block's warps split the inputs (kw ways) and keep their part of x in registers while the block
 // streams its row tiles; the partial sums meet in shared memory in a fixed order. Every lane copies
 // the 16-byte pieces that it will use itself (cp.async, kDepth row tiles ahead, across the borders
@@ -452,11 +453,15 @@ int launch_small(SmallParams p, int64_t units, cudaStream_t st) {
 
 template <int G, bool kZeros, bool kSwiGLU>
 int launch_rows(const SmallParams& p, int64_t units8, int64_t units16, cudaStream_t st) {
-  // 8 rows at a time (two blocks share an SM) while most segments have no more, else 16. 128 experts of
-  // 2048 x 768, groups of 128, both products, 8 or 16 at a time: 4 rows on average 96 and 150 us,
-  // 6 rows 104 and 158, 8 rows 127 and 160; groups of 64: 8 rows 170 and 158; 8 experts of 4096 x 1024
-  // with 6 rows 39 and 35. One segment of 8 rows, 18944 x 4096: 20.5 and 22.5; of 9: 28.7 and 22.5.
-  if (p.rows_cap > (p.seg_offsets ? 7 * static_cast<int64_t>(p.nseg) : 8))
+  // 8 rows at a time (two blocks share an SM) while most segments have few more, else 16: a second pass
+  // over the weights comes from L2 but is decoded again, so the limit is lower where a tile has more
+  // scales and zero points. 128 experts of 2048 x 768, both products, 8 and 16 at a time: groups
+  // of 128, 6 rows on average 103 and 156 us, 9 rows 137 and 162, 10 rows 146 and 162; of 64 without
+  // zero points 9 rows 144 and 152, 10 rows 152 and 150; with zero points 7 rows 152 and 154, 8 rows 164
+  // and 156; of 32, 6 rows 144 and 156, 7 rows 162 and 156. (8 experts of 4096 x 1024 turn at 7 rows.)
+  // One segment of 8 rows, 18944 x 4096: 20.5 and 22.5; of 9: 28.7 and 22.5.
+  constexpr int kRows = G == 128 || (G == 64 && !kZeros) ? 9 : 7;
+  if (p.rows_cap > (p.seg_offsets ? kRows * static_cast<int64_t>(p.nseg) : 8))
     return launch_small<G, kZeros, kSwiGLU, 2>(p, units16, st);
   return launch_small<G, kZeros, kSwiGLU, 1>(p, units8, st);
 }
@@ -481,14 +486,14 @@ int w4_product(const W4Problem& pr, cudaStream_t st) {
   // Few rows: this kernel alone (a longer segment runs in blocks of 16 rows, its weights from L2
   // after the first). Without a table: up to 16 rows, and up to 64 while the matrix is so small that
   // the other kernel's tiles could not fill the GPU (17 x 4096 x 4096: 17 us here, 29 there;
-  // 17 x 18944 x 4096: 39 and 33). With one: segments of 10 rows on average (1280 rows of 128
-  // experts: 169 us here, 185 with both). Else segments of at most kSmallRows rows run here and longer
+  // 17 x 18944 x 4096: 39 and 33). With one: segments of 12 rows on average (128 experts of
+  // 2048 x 768, both products: 1536 rows 178 us here and 191 with both, 1792 rows 201 and 190). Else segments of at most kSmallRows rows run here and longer
   // ones on the other kernel; the host does not know the lengths and launches both.
   // the lists of row blocks and output tiles count in 32 bits
   PRISM_CHECK_ARG(ceil_div(pr.rows_cap, 8) * pr.nseg < (int64_t(1) << 31), "4-bit product: too many rows");
   const int64_t out_tiles = ceil_div(pr.swiglu ? 2 * pr.n_out : pr.n_out, 16);
   const bool few = pr.seg_offsets
-                       ? pr.rows_cap <= std::max<int64_t>(kSmallRows, 10 * pr.nseg)
+                       ? pr.rows_cap <= std::max<int64_t>(kSmallRows, 12 * pr.nseg)
                        : pr.rows_cap <= kSmallRows ||
                              (pr.rows_cap <= 64 && ceil_div(pr.rows_cap, 16) * out_tiles <= 9 * num_sms());
   if (!few) {
