@@ -197,6 +197,26 @@ def test_dense_modules(T):
     assert (out.double() - ref).abs().norm() <= HALF * ref.norm()
 
 
+@pytest.mark.parametrize("T", [3, 37, 150])
+def test_dense_mlp_captured_at_its_first_call_with_these_rows(T):
+    """Nothing that a replay needs is kept from, or made by, another call."""
+    torch.manual_seed(4)
+    mlp = Qwen3MLP(H, I).to(DEV, torch.bfloat16)
+    for p in mlp.parameters():
+        p.data.normal_(std=p.shape[1] ** -0.5)
+    mlp.quantize_(64)
+    mlp(tokens(T + 1000))
+    x = tokens(T)
+    static = torch.zeros_like(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = mlp(static)
+    eager = mlp(x)            # between capture and first replay
+    static.copy_(x)
+    graph.replay()
+    assert torch.equal(y, eager)
+
+
 def test_refusals_on_the_device():
     moe, x = block(), tokens(4)
     gu, dn = moe.w4_gate_up.weight, moe.w4_down.weight

@@ -269,6 +269,42 @@ def test_experts_one_segment_of_all_rows(R, H, I):
         capi.expert_swiglu_w4(x, None, weights(1, (2,), 2 * I, H, 64, True, gate_up=True), two)
 
 
+@pytest.mark.parametrize("counts", [[2, 0, 3, 1], [200, 3, 0, 40], [700, 16, 900, 17], [30, 40, 1, 20]])
+def test_experts_follow_each_other_and_run_side_by_side(counts):
+    """A call's kernels overlap; a call that reads what the one before it wrote, in the same buffers,
+    still sees all of it, and calls on two streams do not meet."""
+    H, I, E = 256, 192, len(counts)
+    gu, dn = weights(1, (E,), 2 * I, H, 64, True, gate_up=True), weights(2, (E,), H, I, 64, True)
+    seg = torch.tensor(bounds_of(counts), dtype=torch.int32, device=DEV)
+    xs = [rows(s, sum(counts), H) for s in (3, 4)]
+
+    def chain(x, wait):
+        y = x.clone()
+        for _ in range(6):
+            capi.expert_swiglu_w4(y, seg, gu, dn, y=y)
+            if wait:
+                torch.cuda.synchronize()
+            # a reader and writer in between, which also keeps rows at a length of sqrt(H)
+            y.copy_(torch.nn.functional.normalize(y.float(), dim=1) * 16)
+            capi.expert_swiglu_w4(y, seg, gu, dn, y=y)
+            if wait:
+                torch.cuda.synchronize()
+        return y
+
+    want = [chain(x, True) for x in xs]
+    assert all(w.abs().max() > 0 and w.isfinite().all() for w in want)
+    streams = [torch.cuda.Stream() for _ in xs]
+    for _ in range(10):
+        got = []
+        for x, s in zip(xs, streams):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append(chain(x, False))
+        for s in streams:
+            torch.cuda.current_stream().wait_stream(s)
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
 def test_linear_out_and_error_word():
     w = weights(1, (), 256, 256, 64, False)
     x = rows(2, 40, 256)
