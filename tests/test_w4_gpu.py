@@ -19,7 +19,7 @@ import pytest
 import torch
 
 from prism_infer_b200 import capi, ops  # noqa: F401
-from prism_infer_b200.quant import dequantize_w4, pack_w4, quantize_w4
+from prism_infer_b200.quant import W4Weight, dequantize_w4, pack_w4, quantize_w4
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -303,6 +303,40 @@ def test_experts_follow_each_other_and_run_side_by_side(counts):
         for s in streams:
             torch.cuda.current_stream().wait_stream(s)
         assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+def test_linear_outputs_past_32_bits():
+    M, N, K = 540_000, 4096, 128                     # 2.2e9 outputs
+    w = weights(1, (), N, K, 128, False)
+    x = rows(2, M, K)
+    y = capi.linear_w4(x, w)
+    for at in (0, M // 2, 2 ** 31 // N - 100, M - 300):
+        check_linear(x[at:at + 300], w, y[at:at + 300])
+
+
+@pytest.mark.parametrize("counts", [[3, 1], [40, 700]])
+def test_experts_of_a_stack_past_32_bits(counts):
+    """The last experts of stacks whose codes take 2.5 GB."""
+    E, H, I, G = 1200, 2048, 1024, 128
+    g = gen_of(5)
+
+    def stack(N, K, gate_up):
+        shape = (E, N // 16, K // 128, 16)
+        q = torch.randint(0, 256, (*shape, 64), generator=g, device=DEV, dtype=torch.uint8)
+        s = ((0.5 + torch.rand(*shape, 1, generator=g, device=DEV)) / (4.6 * K ** 0.5)).bfloat16()
+        return W4Weight(q, s, None, N, K, G, gate_up)
+
+    def some(w, ids):
+        return W4Weight(w.qweight[ids], w.scales[ids], None, w.out_features, w.in_features, G,
+                        w.gate_up)
+
+    gu, dn = stack(2 * I, H, True), stack(H, I, False)
+    ids = [E - 1, E - 150]
+    off = bounds_of(counts)
+    x = rows(6, off[-1], H)
+    y = capi.expert_swiglu_w4(x, torch.tensor(off, dtype=torch.int32, device=DEV), gu, dn,
+                              seg_expert=torch.tensor(ids, dtype=torch.int32, device=DEV))
+    check_experts(x, off, [0, 1], some(gu, ids), some(dn, ids), y)
 
 
 def test_linear_out_and_error_word():
