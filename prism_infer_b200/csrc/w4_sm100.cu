@@ -53,33 +53,36 @@ constexpr int kTokBox = 64;      // activation rows per copy
 constexpr int kPackStage = 8 * 1024;
 constexpr size_t kPrefixW4 = ((kMaxW4Segments + 1) * 4 + 15) / 16 * 16;
 
-// The two shapes: 256 activation rows (many rows per segment: one decoding serves them all) or 64
-// (tens of rows). With 64 a stage's work is shorter than the latency of handing it from role to role
-// (about 500 cycles each, waits and votes included), so two CTAs share an SM and take turns.
-template <bool kNarrow>
+// The shapes: 256 activation rows (many rows per segment: one decoding serves them all) or 64 (tens of
+// rows). With 64 a stage's work is shorter than the latency of handing it from role to role (about 500
+// cycles each, waits and votes included), so two CTAs share an SM and take turns; where there are no
+// more tiles than SMs, one CTA has the whole SM's shared memory for its rings instead.
+enum { kWide, kNarrow, kDeep };
+template <int kShape>
 struct Shape {
-  static constexpr int kTok = kNarrow ? 64 : 256;        // activation rows per tile, at most
+  static constexpr bool k64 = kShape != kWide;
+  static constexpr int kTok = k64 ? 64 : 256;            // activation rows per tile, at most
   static constexpr int kAStage = kRowsW * kBK * 2;
   static constexpr int kStage = kAStage + kTok * kBK * 2;
-  static constexpr int kStages = kNarrow ? 3 : 4;
-  static constexpr int kPackStages = 3;
-  static constexpr int kAccWarps = kNarrow ? 4 : 8;
+  static constexpr int kStages = kShape == kWide ? 4 : kShape == kNarrow ? 3 : 7;
+  static constexpr int kPackStages = kShape == kDeep ? 5 : 3;
+  static constexpr int kAccWarps = k64 ? 4 : 8;
   static constexpr int kThreads = 256 + 32 * kAccWarps;
-  static constexpr int kCtas = kNarrow ? 2 : 1;          // per SM
-  static constexpr int kBufs = kNarrow ? 4 : 2;          // TMEM buffers, one group each
+  static constexpr int kCtas = kShape == kNarrow ? 2 : 1;   // per SM
+  static constexpr int kBufs = k64 ? 4 : 2;              // TMEM buffers, one group each
   static constexpr uint32_t kTmem = kBufs * kTok;        // TMEM columns
-  // registers of the control, decoding and accumulating warpgroups; their sum is the launch's
-  // at most (80 x 3, 128 x 4)
+  // registers of the control, decoding and accumulating warpgroups; their sum is the launch's at
+  // most (wide 128 x 4, narrow 80 x 3, deep 168 x 3)
   static constexpr int kRegsControl = 32;
-  static constexpr int kRegsDecode = kNarrow ? 64 : 72;
-  static constexpr int kRegsAcc = kNarrow ? 144 : 200;
+  static constexpr int kRegsDecode = kShape == kNarrow ? 64 : 72;
+  static constexpr int kRegsAcc = kShape == kNarrow ? 144 : 200;
 };
 constexpr int kDecWarps = 4;
 
 // Shared memory after the stages: packed slots, zero-point slots, scale slots, barriers, prefix.
-template <int G, bool kNarrow>
+template <int G, int kShape>
 struct Smem {
-  using P = Shape<kNarrow>;
+  using P = Shape<kShape>;
   static constexpr int kPG = 128 / G;                 // groups per chunk
   static constexpr int kZeroSlot = kRowsW * kPG;      // bytes
   static constexpr int kScaleSlot = kRowsW * kPG * 2;
@@ -91,7 +94,7 @@ struct Smem {
   static constexpr int kNumBars = 2 * (P::kStages + P::kPackStages + kScaleSlots + P::kBufs) + 1;
   static constexpr int kPrefix = kBars + (kNumBars * 8 + 8 + 15) / 16 * 16;
   static constexpr int kBytes = 1024 + kPrefix + static_cast<int>(kPrefixW4);
-  static_assert(kBytes <= (kNarrow ? 115712 : 232448), "shared memory budget");
+  static_assert(kBytes <= (kShape == kNarrow ? 115712 : 232448), "shared memory budget");
 };
 
 struct LargeParams {
@@ -293,14 +296,14 @@ struct Ring {
   }
 };
 
-template <int G, bool kZeros, bool kSwiGLU, bool kNarrow>
-__global__ void __launch_bounds__(Shape<kNarrow>::kThreads, Shape<kNarrow>::kCtas)
+template <int G, bool kZeros, bool kSwiGLU, int kShape>
+__global__ void __launch_bounds__(Shape<kShape>::kThreads, Shape<kShape>::kCtas)
     w4_large_kernel(const __grid_constant__ CUtensorMap map_x,
                     const __grid_constant__ CUtensorMap map_q,
                     const __grid_constant__ CUtensorMap map_s,
                     const __grid_constant__ CUtensorMap map_z, const LargeParams p) {
-  using P = Shape<kNarrow>;
-  using S = Smem<G, kNarrow>;
+  using P = Shape<kShape>;
+  using S = Smem<G, kShape>;
   constexpr int PG = S::kPG;
   constexpr int kTok = P::kTok, kStage = P::kStage, kAStage = P::kAStage;
   extern __shared__ uint8_t smem_raw[];
@@ -547,13 +550,13 @@ __global__ void __launch_bounds__(Shape<kNarrow>::kThreads, Shape<kNarrow>::kCta
     // ------------------------------------------------------------------ accumulate
     reg_alloc<P::kRegsAcc>();
     const int q = warp & 3, side = (warp - 8) >> 2;   // narrow: one side, all columns
-    constexpr int kPairs = kNarrow ? 32 : 64;          // pairs of columns held, at most
+    constexpr int kPairs = P::k64 ? 32 : 64;          // pairs of columns held, at most
     Ring<P::kBufs> buf;
     Ring<S::kScaleSlots> sl;
     int held = -1;
     const int row = q * 32 + lane;                     // weight row in the tile
     const bool ok = for_tiles([&](const Tile& t) {
-      const int left = kNarrow ? t.cols : (t.cols / 16 + 1) / 2 * 16;   // columns of side 0
+      const int left = P::k64 ? t.cols : (t.cols / 16 + 1) / 2 * 16;   // columns of side 0
       const int col0 = side ? left : 0, ncols = side ? t.cols - left : left;
       float2 acc[kPairs];
 #pragma unroll
@@ -591,8 +594,8 @@ __global__ void __launch_bounds__(Shape<kNarrow>::kThreads, Shape<kNarrow>::kCta
         case 0: done = add_chunks(std::integral_constant<int, 0>{}); break;
         case 1: done = add_chunks(std::integral_constant<int, 1>{}); break;
         case 2: done = add_chunks(std::integral_constant<int, 2>{}); break;
-        case 3: done = add_chunks(std::integral_constant<int, kNarrow ? 2 : 3>{}); break;
-        default: done = add_chunks(std::integral_constant<int, kNarrow ? 2 : 4>{}); break;
+        case 3: done = add_chunks(std::integral_constant<int, P::k64 ? 2 : 3>{}); break;
+        default: done = add_chunks(std::integral_constant<int, P::k64 ? 2 : 4>{}); break;
       }
       if (!done) return false;
       // ---- output: a lane is one output of every activation row, so 32 lanes store 64 bytes of a row
@@ -650,33 +653,33 @@ struct Maps {
   CUtensorMap x, q, s, z;
 };
 
-template <int G, bool kZeros, bool kSwiGLU, bool kNarrow>
+template <int G, bool kZeros, bool kSwiGLU, int kShape>
 int launch_shape(const Maps& map, const LargeParams& p, int grid, cudaStream_t st) {
-  auto kern = w4_large_kernel<G, kZeros, kSwiGLU, kNarrow>;
-  if (int r = ensure_smem_attr(reinterpret_cast<const void*>(kern), Smem<G, kNarrow>::kBytes))
+  auto kern = w4_large_kernel<G, kZeros, kSwiGLU, kShape>;
+  if (int r = ensure_smem_attr(reinterpret_cast<const void*>(kern), Smem<G, kShape>::kBytes))
     return r;
   // a plain launch, after the end of the kernel before it: started while gate_up ended, the down product
   // of a skewed batch (4096 tokens of 128 experts) made both 690 us instead of 620
-  kern<<<grid, Shape<kNarrow>::kThreads, Smem<G, kNarrow>::kBytes, st>>>(map.x, map.q, map.s, map.z, p);
+  kern<<<grid, Shape<kShape>::kThreads, Smem<G, kShape>::kBytes, st>>>(map.x, map.q, map.s, map.z, p);
   PRISM_LAUNCH_CHECK("w4_large_kernel launch");
   return PRISM_MOE_OK;
 }
 
 template <int G, bool kZeros, bool kSwiGLU>
-int launch_large(const Maps& map, const LargeParams& p, bool narrow, int grid,
-                 cudaStream_t st) {
-  return narrow ? launch_shape<G, kZeros, kSwiGLU, true>(map, p, grid, st)
-                : launch_shape<G, kZeros, kSwiGLU, false>(map, p, grid, st);
+int launch_large(const Maps& map, const LargeParams& p, int shape, int grid, cudaStream_t st) {
+  if (shape == kDeep) return launch_shape<G, kZeros, kSwiGLU, kDeep>(map, p, grid, st);
+  return shape == kNarrow ? launch_shape<G, kZeros, kSwiGLU, kNarrow>(map, p, grid, st)
+                          : launch_shape<G, kZeros, kSwiGLU, kWide>(map, p, grid, st);
 }
 
 template <int G>
-int launch_group(const Maps& map, const LargeParams& p, bool swiglu, bool narrow, int grid,
+int launch_group(const Maps& map, const LargeParams& p, bool swiglu, int shape, int grid,
                  cudaStream_t st) {
   if (p.z)
-    return swiglu ? launch_large<G, true, true>(map, p, narrow, grid, st)
-                  : launch_large<G, true, false>(map, p, narrow, grid, st);
-  return swiglu ? launch_large<G, false, true>(map, p, narrow, grid, st)
-                : launch_large<G, false, false>(map, p, narrow, grid, st);
+    return swiglu ? launch_large<G, true, true>(map, p, shape, grid, st)
+                  : launch_large<G, true, false>(map, p, shape, grid, st);
+  return swiglu ? launch_large<G, false, true>(map, p, shape, grid, st)
+                : launch_large<G, false, false>(map, p, shape, grid, st);
 }
 
 }  // namespace
@@ -724,14 +727,22 @@ int w4_product_large(const W4Problem& pr, int min_rows, cudaStream_t st) {
   if (p.z)
     if (int r = tiles_map(&map.z, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.z, 16 * pg, 16 * pg)) return r;
   const int64_t long_segs = std::min<int64_t>(pr.nseg, pr.rows_cap / (min_rows + 1));
-  const bool narrow = pr.rows_cap <= kNarrowRows * static_cast<int64_t>(pr.nseg);
-  const int64_t items = (pr.rows_cap / (narrow ? 64 : 256) + long_segs) * p.tiles_n;
+  // most tiles there can be, of 64 rows or of 256
+  auto tiles_of = [&](int rows) {
+    return (pr.seg_offsets ? pr.rows_cap / rows + long_segs : ceil_div(pr.rows_cap, rows)) * p.tiles_n;
+  };
+  const int sms = num_sms();
+  const int shape = tiles_of(64) <= sms                                                ? kDeep
+                    : pr.rows_cap <= kNarrowRows * static_cast<int64_t>(pr.nseg) ? kNarrow
+                                                                                 : kWide;
+  const int64_t items = tiles_of(shape == kWide ? 256 : 64);
   PRISM_CHECK_ARG(items < (int64_t(1) << 31), "4-bit product: too many tiles");
-  const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(items, num_sms() * (narrow ? 2 : 1))));
+  const int grid = static_cast<int>(
+      std::max<int64_t>(1, std::min<int64_t>(items, sms * (shape == kNarrow ? 2 : 1))));
   switch (pr.w.group_size) {
-    case 32: return launch_group<32>(map, p, pr.swiglu, narrow, grid, st);
-    case 64: return launch_group<64>(map, p, pr.swiglu, narrow, grid, st);
-    default: return launch_group<128>(map, p, pr.swiglu, narrow, grid, st);
+    case 32: return launch_group<32>(map, p, pr.swiglu, shape, grid, st);
+    case 64: return launch_group<64>(map, p, pr.swiglu, shape, grid, st);
+    default: return launch_group<128>(map, p, pr.swiglu, shape, grid, st);
   }
 }
 

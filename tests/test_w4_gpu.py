@@ -93,7 +93,10 @@ LINEAR = [(1, 8, 32, 32), (1, 4096, 4096, 128), (2, 24, 96, 32), (3, 2056, 1440,
           (8, 136, 192, 64), (9, 1000, 128, 64), (16, 264, 2176, 128), (17, 512, 640, 128),
           (33, 72, 352, 32), (64, 520, 4224, 64), (100, 1536, 2048, 128), (127, 40, 256, 128),
           (128, 128, 1024, 32), (129, 136, 1088, 64), (255, 96, 32, 32), (256, 384, 512, 64),
-          (257, 392, 576, 64), (700, 1032, 1152, 128), (2048, 256, 768, 32), (5, 640, 9216, 128)]
+          (257, 392, 576, 64), (700, 1032, 1152, 128), (2048, 256, 768, 32), (5, 640, 9216, 128),
+          # more tiles than SMs, of 64 and of 256 rows; exactly as many of 64; deep sums on few tiles
+          (40, 19208, 96, 32), (64, 20000, 704, 64), (33, 19000, 1152, 128), (300, 19208, 192, 64),
+          (64, 18944, 256, 128), (128, 9472, 320, 32), (250, 4096, 8192, 128), (190, 776, 5120, 64)]
 
 
 @pytest.mark.parametrize("M,N,K,G", LINEAR)
@@ -165,6 +168,8 @@ EXPERTS = [
     (1440, 736, 32, 32, [22, 0, 150, 7, 64]), (320, 192, 64, 32, [129, 64, 15]),
     (512, 256, 128, 64, [130, 0, 255, 256, 257, 3]), (256, 1024, 64, 128, [600, 2, 0, 1]),
     (32, 32, 32, 32, [0, 1, 0, 300]), (128, 128, 128, 128, [0, 0, 0]),
+    (512, 512, 128, 64, [30, 17, 64, 0, 65, 16, 100, 2] * 5), (320, 1088, 32, 64, [40, 33, 20] * 12),
+    (1024, 768, 128, 128, [200, 300, 16, 17, 90, 500] * 2),
 ]
 
 
