@@ -17,7 +17,8 @@
 // are the logits themselves (both scores increase with the logit), exactly; with one they are
 // fp32 scores + bias, whose error is bounded. Any two neighbours in the order of the k + 1 best (and
 // any two groups at the cut) that are closer than their errors, and not the same logit and bias,
-// are looked at in 64 bits: sigmoid keys with a bias among a few more candidates, all else (NaN,
+// are looked at in 64 bits, and so is a tie at the cut with another key that close behind it: sigmoid
+// keys with a bias among a few more candidates, all else (NaN,
 // infinities and scores that saturate too) by choose_exact, on 64-bit keys of the whole row. On
 // normal logits with a random bias about 1 row in 500 looks again, and nearly none goes on.
 //
@@ -334,7 +335,9 @@ __global__ void __launch_bounds__(32 * kScoredWarps) route_scored_kernel(const _
     const bool exact = !p.bias && !two;   // logits: equal ones are ties, distinct ones decided
     unsure |= !(low > high || (exact && low == high)) || !(gs == gs);
     if (exact)
+      // (a tie at the cut: no other group may be that close to it)
       unsure |= (low - high > 0.f && low - high < 0x1p-40f) ||
+                (low == high && grp < p.groups && gs != low && fabsf(gs - low) < 0x1p-40f) ||
                 (p.sigmoid ? fabsf(low) > 16.f || fabsf(high) > 16.f : !(top - low <= 600.f));
     if (!kept) {
 #pragma unroll
@@ -399,17 +402,39 @@ __global__ void __launch_bounds__(32 * kScoredWarps) route_scored_kernel(const _
     nl = next_key ? load_logit<kBf16>(p.logits, t * p.E + next_id) : 0.f;
     nb = next_key && p.bias ? p.bias[next_id] : 0.f;
   }
+  auto reach = [&](float x, float y) {   // two keys closer than this may be in the wrong order
+    return 2.f * score_err + 0x1p-22f * (fabsf(x) + fabsf(y));
+  };
   bool close = false;   // in the wrong order, perhaps
+  bool tie = false;     // equal in 64 bits too, and others may be close
   if (lane < p.k) {
     const bool next = lane + 1 < p.k || next_key != 0;
     if (p.bias) {
-      const float err = 2.f * score_err + 0x1p-22f * (fabsf(v) + fabsf(nv));
-      if (next) close = !(v - nv > err) && !(my.logit == nl && mb == nb);
+      tie = next && my.logit == nl && mb == nb;
+      if (next) close = !(v - nv > reach(v, nv)) && !tie;
       unsure |= !(fabsf(v) <= 3.4028235e38f);
     } else {
       // where 64-bit scores could merge distinct logits: next to 0 or 1, or next to each other
+      tie = next && v == nv && fabsf(v) < 0x1p-16f;   // larger ones lie 2^-40 apart or more
       if (next) unsure |= v - nv > 0.f && v - nv < 0x1p-40f;
       unsure |= p.sigmoid ? !(fabsf(v) <= 16.f) : !(top - v <= 600.f);
+    }
+  }
+  if (__shfl_sync(kFull, tie, p.k - 1)) {
+    // A tie at the cut says nothing of the keys behind it: one of another logit or bias that is in
+    // reach of the tied ones may belong before them.
+    const float cut = __shfl_sync(kFull, v, p.k - 1), cut_logit = __shfl_sync(kFull, my.logit, p.k - 1);
+    const float cut_bias = __shfl_sync(kFull, mb, p.k - 1);
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) {
+      const float o = key_value32(key[i]);
+      if (key[i] == 0 || o == -__int_as_float(0x7f800000)) continue;   // far from a finite cut
+      if (!p.bias) {
+        unsure |= o < cut && cut - o < 0x1p-40f;
+      } else if (!(cut - o > reach(cut, o))) {
+        const int id = first + at[i];
+        close |= !(load_logit<kBf16>(p.logits, t * p.E + id) == cut_logit && p.bias[id] == cut_bias);
+      }
     }
   }
   unsure = __any_sync(kFull, unsure);

@@ -1,0 +1,81 @@
+"""Scored routing where 32-bit keys do not decide: the choice is that of 64-bit keys, exactly."""
+import pytest
+import torch
+
+from prism_infer_b200 import capi
+from oracle.scored_routing import route_scored_ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def gen_of(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def check_ids(logits, k, **kw):
+    ids, w, _ = capi.route_scored(logits, k, **kw)
+    r_ids, r_w = route_scored_ref(logits, k, **kw)
+    wrong = (ids != r_ids).any(-1)
+    assert not wrong.any(), (int(wrong.sum()), ids[wrong][:3].tolist(), r_ids[wrong][:3].tolist())
+    return w, r_w
+
+
+# ------------------------------------------------------------------------------ ties at the cut
+
+def test_tie_at_the_cut_with_a_better_third():
+    """Two equal keys meet at the cut; a third, equal in 32 bits, is larger in 64."""
+    for dtype in (torch.bfloat16, torch.float32):
+        logits = torch.tensor([[14, 14, 14.0625], [14, 14.0625, 14], [14.0625, 14, 14]],
+                              device=DEV, dtype=dtype)
+        check_ids(logits, 1, scoring="sigmoid", bias=torch.zeros(3, device=DEV))
+
+
+@pytest.mark.parametrize("k", [1, 3, 8, 29, 32])
+@pytest.mark.parametrize("scoring", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("ties", [2, 3, 9])
+def test_tie_at_the_cut_among_biased_keys(k, scoring, ties):
+    """k - 1 certain choices, then ``ties`` equal keys and one 2^-24 of a key above them."""
+    E, T, g = 160, 40, gen_of(k)
+    order = torch.rand(T, E, generator=g, device=DEV).argsort(-1)
+    logits = torch.full((T, E), -3.0, device=DEV)
+    where = order[:, :ties + 1]
+    logits.scatter_(1, where, 2.0)
+    logits.scatter_(1, where[:, :1], 2.0 + 2.0 ** -22)
+    bias = torch.full((E,), 0.5, device=DEV)
+    for row in range(T):                 # a bias belongs to an expert: rows one by one
+        b = bias.clone()
+        b[order[row, ties + 1:ties + k]] = 1.5 + 0.01 * torch.arange(k - 1, device=DEV)
+        check_ids(logits[row:row + 1], k, scoring=scoring, bias=b)
+
+
+@pytest.mark.parametrize("k", [1, 2, 5, 8, 27, 29, 32])
+@pytest.mark.parametrize("groups,keep", [(1, 1), (4, 3), (3, 2)])
+@pytest.mark.parametrize("scoring", ["sigmoid", "softmax"])
+def test_ties_and_close_keys_together(k, groups, keep, scoring):
+    """bf16 logits of few values and biases in fixed steps: many equal keys, many within a rounding."""
+    g = gen_of(100 * k + groups)
+    steps = torch.randint(0, 24, (600, 96), generator=g, device=DEV)
+    high = 12 if scoring == "sigmoid" else 0
+    logits = (high + 0.0625 * steps).to(torch.bfloat16)
+    if scoring == "softmax":   # all scores small beside the biases
+        logits[:, 7] = 14
+    bias = 0.5 + 0.001 * torch.randint(-2, 3, (96,), generator=g, device=DEV)
+    for b in (torch.zeros(96, device=DEV), bias):
+        for score in ("max", "top2"):
+            check_ids(logits, k, scoring=scoring, bias=b, num_groups=groups, topk_groups=keep,
+                      group_score=score)
+
+
+@pytest.mark.parametrize("scoring", ["sigmoid", "softmax"])
+def test_logits_that_only_32_bits_tell_apart(scoring):
+    """Logits so small that their 64-bit scores are equal: ties, which go to the lowest index."""
+    logits = torch.full((4, 16), -5.0, device=DEV)
+    logits[0, :3] = torch.tensor([0.0, 1e-20, 1e-20])
+    logits[1, 4:8] = torch.tensor([1e-20, 1e-20, 0.0, 2e-20])
+    logits[2, 1:16:4] = torch.tensor([0.0, 1e-20, 1e-20, 1e-20], device=DEV)
+    logits[3, 1:16:4] = torch.tensor([1e-20, 1e-20, 2e-20, -1e-20], device=DEV)
+    for k in (1, 2, 3):
+        check_ids(logits, k, scoring=scoring)
+        for keep in (1, 2, 3):
+            check_ids(logits, k, scoring=scoring, num_groups=4, topk_groups=keep)
