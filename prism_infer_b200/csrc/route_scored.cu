@@ -35,6 +35,7 @@ namespace {
 constexpr int kScoredWarps = 4;
 constexpr int kSpare = 4;   // candidates beyond the k that a close order looks at
 constexpr unsigned kFull = 0xffffffffu;
+constexpr float kFloor = 0x1p-120f;   // absolute error that any fp32 score is allowed, however small it is
 
 template <bool kBf16>
 __device__ __forceinline__ float load_logit(const void* p, int64_t i) {
@@ -291,7 +292,8 @@ __global__ void __launch_bounds__(32 * kScoredWarps) route_scored_kernel(const _
   // Error of any fp32 score of this row. Sigmoid: expf (2 ulp), a sum and a division (2 ulp), 2^-20
   // of the score. Softmax: expf, its argument (|l - top| 2^-24, but e^-x x < 0.4), a division and a sum
   // whose 2^6 lane terms and 32 lanes meet in a tree (11 roundings): 2^-19 of the largest.
-  const float score_err = p.bias ? (p.sigmoid ? 0x1p-20f : 0x1p-19f) * score(top) : 0.f;
+  // Scores under 2^-126 come out as 0 (expf(-l) above 2^126 makes the division 0): kFloor covers them.
+  const float score_err = p.bias ? fmaf(p.sigmoid ? 0x1p-20f : 0x1p-19f, score(top), kFloor) : 0.f;
   if constexpr (kSorted && EPT > 1) sort_lane(key, at);
 
   // ---- groups: the keep best, equal scores by ascending group
@@ -317,7 +319,7 @@ __global__ void __launch_bounds__(32 * kScoredWarps) route_scored_kernel(const _
       err = 2.f * score_err + 0x1p-22f * (fabsf(va) + fabsf(vb));
     } else if (two) {   // keys are logits: their scores, up to the softmax's common factor
       gs = p.sigmoid ? score(va) + score(vb) : expf(va - top) + expf(vb - top);
-      err = p.sigmoid ? 0x1p-20f * gs : 0x1p-20f;
+      err = p.sigmoid ? fmaf(0x1p-20f, gs, kFloor) : 0x1p-20f;
     }
     int rank = 0;
     for (int g = 0; g < p.groups; ++g) {

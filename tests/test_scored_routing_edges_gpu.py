@@ -79,3 +79,18 @@ def test_logits_that_only_32_bits_tell_apart(scoring):
         check_ids(logits, k, scoring=scoring)
         for keep in (1, 2, 3):
             check_ids(logits, k, scoring=scoring, num_groups=4, topk_groups=keep)
+
+
+# ------------------------------------------------------------------------------ the bottom of the range
+
+@pytest.mark.parametrize("score", ["max", "top2"])
+def test_keys_at_the_bottom_of_the_range(score):
+    """Sigmoid scores around the smallest normal fp32 number, which 32 bits round to 0 or nearly so."""
+    logits = torch.tensor([[-87.3, -200.0, -87.4, -87.4]], device=DEV)
+    check_ids(logits, 2, scoring="sigmoid", num_groups=2, group_score=score)
+    logits = -104 + 18 * torch.rand(300, 64, generator=gen_of(1), device=DEV)
+    tiny = 1e-38 * torch.randn(64, generator=gen_of(2), device=DEV)
+    for bias in (None, torch.zeros(64, device=DEV), tiny):
+        for groups, keep in ((1, 1), (8, 3), (8, 8)):
+            check_ids(logits, 6, scoring="sigmoid", bias=bias, num_groups=groups, topk_groups=keep,
+                      group_score=score)
