@@ -177,7 +177,7 @@ __device__ __noinline__ Choice choose_exact(const ScoredParams& p, int64_t t) {
       key[i] = order_key(s + (p.bias ? static_cast<double>(p.bias[expert(i)]) : 0.0));
     }
   }
-  if (p.groups > 1) {
+  if (p.keep < p.groups) {
     uint64_t a = 0, b = 0;
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(32 * kScoredWarps) route_scored_kernel(const _
   if constexpr (kSorted && EPT > 1) sort_lane(key, at);
 
   // ---- groups: the keep best, equal scores by ascending group
-  if (p.groups > 1) {
+  if (p.keep < p.groups) {   // else there is no cut, and nothing to be unsure of
     uint32_t a = 0, b = 0;
     if constexpr (kSorted) {
       a = key[0];
@@ -335,12 +335,13 @@ __global__ void __launch_bounds__(32 * kScoredWarps) route_scored_kernel(const _
       high = fmaxf(high, __shfl_xor_sync(kFull, high, off));
     }
     const bool exact = !p.bias && !two;   // logits: equal ones are ties, distinct ones decided
-    unsure |= !(low > high || (exact && low == high)) || !(gs == gs);
+    // (lanes of no group hold no score)
+    unsure |= !(low > high || (exact && low == high)) || (grp < p.groups && !(gs == gs));
     if (exact)
       // (a tie at the cut: no other group may be that close to it)
       unsure |= (low - high > 0.f && low - high < 0x1p-40f) ||
                 (low == high && grp < p.groups && gs != low && fabsf(gs - low) < 0x1p-40f) ||
-                (p.sigmoid ? fabsf(low) > 16.f || fabsf(high) > 16.f : !(top - low <= 600.f));
+                (p.sigmoid ? fabsf(low) > 16.f : !(top - low <= 600.f));   // saturated
     if (!kept) {
 #pragma unroll
       for (int i = 0; i < EPT; ++i) key[i] = 0;

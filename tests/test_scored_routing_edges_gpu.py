@@ -94,3 +94,59 @@ def test_keys_at_the_bottom_of_the_range(score):
         for groups, keep in ((1, 1), (8, 3), (8, 8)):
             check_ids(logits, 6, scoring="sigmoid", bias=bias, num_groups=groups, topk_groups=keep,
                       group_score=score)
+
+
+# ------------------------------------------------------------------------------ who looks again
+
+SWEEP = [(300, 33, 8, 3, 2), (300, 60, 6, 5, 3), (300, 60, 6, 6, 4), (200, 384, 8, 3, 2),
+         (200, 102, 29, 17, 9), (200, 40, 32, 5, 4), (200, 9, 6, 3, 2), (200, 64, 8, 8, 8),
+         (200, 512, 8, 1, 1), (100, 1008, 16, 18, 5)]
+
+
+@pytest.mark.parametrize("T,E,k,groups,keep", SWEEP)
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_near_ties_at_every_count(T, E, k, groups, keep, scoring):
+    """Keys a few ulp apart, at group counts of no power of two, all groups kept, k + 4 above 32 or
+    above the experts that stay."""
+    g = gen_of(E + k)
+    row = torch.randn(1, E, generator=g, device=DEV).expand(T, E).clone()
+    logits = (row.view(torch.int32) +
+              torch.randint(-3, 4, (T, E), generator=g, device=DEV, dtype=torch.int32)).view(torch.float32)
+    score = torch.sigmoid(row[0].double()) if scoring == "sigmoid" else \
+        torch.softmax(row[0].double(), -1)
+    level = (0.75 - score).float() + 2.0 ** -26 * (torch.arange(E, device=DEV) % 5 - 2)
+    bf16 = row.to(torch.bfloat16)
+    for l, bias in ((logits, None), (logits, level), (bf16, None), (bf16, level)):
+        for group_score in ("max", "top2"):
+            check_ids(l, k, scoring=scoring, bias=bias, num_groups=groups, topk_groups=keep,
+                      group_score=group_score)
+
+
+def time_of(logits, **kw):
+    """Shortest of some graph replays of ten calls."""
+    capi.route_scored(logits, 8, **kw)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(10):
+            capi.route_scored(logits, 8, **kw)
+    best = float("inf")
+    for _ in range(20):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        graph.replay()
+        b.record()
+        b.synchronize()
+        best = min(best, a.elapsed_time(b))
+    return best
+
+
+def test_ordinary_rows_are_decided_in_32_bits():
+    """Three groups, or all groups kept, cost no more than their neighbours: when every row of them
+    took the 64-bit path the times were 3.4 and 4.1 apart."""
+    logits = torch.randn(8192, 384, generator=gen_of(3), device=DEV)
+    kw = dict(scoring="sigmoid", group_score="top2", bias=0.1 * torch.randn(384, generator=gen_of(4), device=DEV))
+    assert time_of(logits, num_groups=3, topk_groups=2, **kw) < \
+        2 * time_of(logits, num_groups=4, topk_groups=2, **kw)
+    logits = logits[:, :256].contiguous()
+    assert time_of(logits, scoring="sigmoid", num_groups=8, topk_groups=8) < \
+        2 * time_of(logits, scoring="sigmoid")
