@@ -487,7 +487,8 @@ __global__ void __launch_bounds__(32 * kScoredWarps) route_scored_kernel(const _
   float s = 0.f;
   if (lane < p.k) {
     if (p.sigmoid) {
-      s = 1.f / (1.f + expf(-my.logit));
+      // far down the sum is e^-l itself, which overflows before its inverse is 0
+      s = my.logit < -80.f ? expf(my.logit) : 1.f / (1.f + expf(-my.logit));
     } else {
       const float d = my.logit - top, z = d - my.logit;
       const float lost = (my.logit - (d - z)) - (top + z);

@@ -96,6 +96,28 @@ def test_keys_at_the_bottom_of_the_range(score):
                       group_score=score)
 
 
+@pytest.mark.parametrize("renorm", [False, True])
+def test_weights_of_scores_that_underflow(renorm):
+    """A subnormal score is within 2^-148 (expf's 2 ulp); the sum of 8 of them is within 2^-145, and
+    renormalising divides either by 1e-20 at least: 9 * 2^-148 / 1e-20 for a weight."""
+    k = 8
+    logits = -104 + 16 * torch.rand(300, 64, generator=gen_of(5), device=DEV)
+    w, ref = check_ids(logits, k, scoring="sigmoid", renorm=renorm)
+    atol = 9 * 2.0 ** -148 / 1e-20 if renorm else 2.0 ** -148
+    torch.testing.assert_close(w.double(), ref, rtol=2.0 ** -18, atol=atol)
+    assert (ref > 1e3 * atol).any()
+
+
+@pytest.mark.parametrize("scoring,renorm", [("softmax", False), ("softmax", True), ("sigmoid", False),
+                                            ("sigmoid", True)])
+def test_which_weights_a_nan_logit_reaches(scoring, renorm):
+    logits = torch.randn(4, 32, generator=gen_of(6), device=DEV)
+    logits[1, 9] = float("nan")
+    w, ref = check_ids(logits, 4, scoring=scoring, renorm=renorm)
+    assert torch.equal(w.isnan(), ref.isnan())
+    assert w[1].isnan().sum() == (1 if scoring == "sigmoid" and not renorm else 4)
+
+
 # ------------------------------------------------------------------------------ who looks again
 
 SWEEP = [(300, 33, 8, 3, 2), (300, 60, 6, 5, 3), (300, 60, 6, 6, 4), (200, 384, 8, 3, 2),
