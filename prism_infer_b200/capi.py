@@ -449,12 +449,32 @@ def block_error_word(device):
 
 def norm_epilogue(residual, norm_weight, eps: float, residual_out):
     """A ``prism_moe_norm_epilogue`` for the *_norm entry points (None when ``norm_weight`` is
-    None). The tensors must stay alive for the call."""
+    None): ``residual`` and ``residual_out`` [T,H] and ``norm_weight`` [H], of the hidden states' dtype
+    and device. It holds the tensors."""
     if norm_weight is None:
         return None
-    _need_cuda(residual, norm_weight, residual_out)
-    return NormEpilogue(residual.data_ptr(), norm_weight.data_ptr(), float(eps),
-                        residual_out.data_ptr())
+    if residual.dim() != 2 or residual_out.shape != residual.shape or \
+            norm_weight.shape != residual.shape[1:]:
+        raise RuntimeError("norm epilogue: residual and residual_out must be [T, H], the weight [H]")
+    if not residual.dtype == norm_weight.dtype == residual_out.dtype:
+        raise RuntimeError("norm epilogue: residual, weight and residual_out differ in dtype")
+    _one_device(residual, norm_weight, residual_out)
+    epilogue = NormEpilogue(residual.data_ptr(), norm_weight.data_ptr(), float(eps),
+                            residual_out.data_ptr())
+    epilogue.held = (residual, norm_weight, residual_out)
+    return epilogue
+
+
+def _check_block_outputs(what: str, x, out, epilogue) -> None:
+    """What a block call writes beside its workspace looks like ``x``."""
+    if out is not None and (out.shape != x.shape or out.dtype != x.dtype):
+        raise RuntimeError(f"{what}: out must be {tuple(x.shape)} in {x.dtype}, got "
+                           f"{tuple(out.shape)} in {out.dtype}")
+    held = getattr(epilogue, "held", None)   # None: the caller filled the struct
+    if held is not None and (held[0].shape != x.shape or held[0].dtype != x.dtype or
+                             held[0].device != x.device):
+        raise RuntimeError(f"{what}: the norm epilogue's residual must be {tuple(x.shape)} in "
+                           f"{x.dtype} on {x.device}")
 
 
 def rmsnorm(x, weight, eps: float, residual=None):
@@ -490,6 +510,8 @@ def block_forward(x, router_logits, w_gate_up, w_down, top_k: int, renorm: bool,
     for t in (router_logits, w_gate_up, w_down):
         if t.dtype != x.dtype:
             raise RuntimeError(f"block_forward: dtype {t.dtype} != hidden dtype {x.dtype}")
+    _check_block_outputs("block_forward", x, out, epilogue)
+    _need_cuda(out)
     if out is None:
         out = torch.empty_like(x)
     if T == 0:
@@ -541,6 +563,7 @@ def block_forward_routed(x, topk_ids, topk_weights, w_gate_up, w_down, out=None,
         if w_gate_up.dtype != x.dtype or w_down.dtype != x.dtype:
             raise RuntimeError("block_forward_routed: weights must have the hidden dtype")
         held = (w_gate_up, w_down)
+    _check_block_outputs("block_forward_routed", x, out, epilogue)
     dev = _one_device(x, topk_ids, topk_weights, out, *held)
     if topk_ids.dtype != torch.int64 or topk_weights.dtype != x.dtype or \
             tuple(topk_ids.shape) != (T, k) or tuple(topk_weights.shape) != (T, k):

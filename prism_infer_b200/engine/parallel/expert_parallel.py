@@ -183,6 +183,7 @@ class ExpertParallelMoE(ExpertBank):
         res_out = torch.empty_like(x) if norm_weight is not None else None
         epi = capi.norm_epilogue(None if residual is None else residual.contiguous(),
                                  norm_weight, eps, res_out)
+        capi._check_block_outputs("ep_forward", x, None, epi)
         lib = capi.load()
         capi.check(lib.prism_moe_ep_forward_norm(
             x.data_ptr(), capi.ptr(lg), capi.ptr(ids), capi.ptr(w), capi.BF16, T,
