@@ -129,6 +129,18 @@ int check_w4(const char* what, const prism_moe_w4* w, int64_t k, int64_t n) {
   return PRISM_MOE_OK;
 }
 
+// The block's kernels read and write rows in 16-byte pieces.
+int check_block_buffers(const char* what, const void* x, const void* out, const void* workspace,
+                        const prism_moe_norm_epilogue* e) {
+  uintptr_t all = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out) |
+                  reinterpret_cast<uintptr_t>(workspace);
+  if (e)
+    all |= reinterpret_cast<uintptr_t>(e->residual) | reinterpret_cast<uintptr_t>(e->norm_weight) |
+           reinterpret_cast<uintptr_t>(e->residual_out);
+  PRISM_CHECK_ARG(all % 16 == 0, "%s: buffers must be 16-byte aligned", what);
+  return PRISM_MOE_OK;
+}
+
 size_t w4_scratch_bytes(int64_t rows, int64_t inter) {
   return align_up(static_cast<size_t>(2 * rows * inter), 256);
 }
@@ -435,6 +447,7 @@ int prism_moe_block_forward_norm(const void* x, const void* router_logits, int d
   PRISM_CHECK_ARG(!epilogue || (epilogue->residual && epilogue->norm_weight &&
                                 epilogue->residual_out && epilogue->eps >= 0.f),
                   "block_forward: incomplete norm epilogue");
+  if (int r = check_block_buffers("block_forward", x, out, workspace, epilogue)) return r;
   if (int r = check_device()) return r;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (num_tokens == 0) return PRISM_MOE_OK;
@@ -478,6 +491,7 @@ int prism_moe_block_forward_routed(const void* x, const int64_t* topk_ids,
   PRISM_CHECK_ARG(!epilogue || (epilogue->residual && epilogue->norm_weight &&
                                 epilogue->residual_out && epilogue->eps >= 0.f),
                   "block_forward_routed: incomplete norm epilogue");
+  if (int r = check_block_buffers("block_forward_routed", x, out, workspace, epilogue)) return r;
   if (int r = check_device()) return r;
   if (num_tokens == 0) return PRISM_MOE_OK;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -1,8 +1,10 @@
 """What the block entry points refuse before anything is launched, without a GPU."""
+import ctypes
+
 import pytest
 import torch
 
-from prism_infer_b200 import capi
+from prism_infer_b200 import build, capi
 from prism_infer_b200.quant import quantize_w4
 
 H, I, E, K, T = 64, 32, 4, 2, 5
@@ -50,3 +52,36 @@ def test_norm_epilogue_of_tensors_that_do_not_match():
             capi.norm_epilogue(bad[0], bad[1], 1e-6, bad[2])
     with pytest.raises(RuntimeError, match="CUDA"):
         capi.norm_epilogue(res, w, 1e-6, res)
+
+
+# ------------------------------------------------------------------------------ the C ABI
+
+P = 1 << 20   # an aligned address that no refused call looks at
+
+
+@pytest.fixture(scope="module")
+def lib():
+    build.build()
+    return capi.load()
+
+
+def block(lib, x=P, out=P, ws=P, res=P, w=P, res_out=2 * P, dense=False, norm=True):
+    q = ctypes.byref(capi.W4(P, P, None, 64))
+    epi = capi.NormEpilogue(res, w, 1e-6, res_out)
+    experts = (P, P, None, None) if dense else (None, None, q, q)
+    return lib.prism_moe_block_forward_routed(x, P, P, capi.BF16, 2, 128, 64, 4, 2, *experts, out, ws,
+                                              1 << 30, None, ctypes.byref(epi) if norm else None)
+
+
+@pytest.mark.parametrize("dense", [False, True])
+def test_buffers_that_are_not_16_byte_aligned(lib, dense):
+    """A view that starts inside a row: the kernels read 16 bytes at a time."""
+    for bad in (dict(x=P + 8), dict(x=P + 2), dict(out=P + 8), dict(ws=P + 4), dict(res=P + 2),
+                dict(w=P + 8), dict(res_out=2 * P + 4), dict(x=P + 8, norm=False)):
+        assert block(lib, dense=dense, **bad) == capi.ERR_ARG, bad
+        assert b"16-byte aligned" in lib.prism_moe_last_error()
+    for bad in (dict(x=P + 8), dict(out=P + 2)):
+        kw = dict(x=P, out=P) | bad
+        assert lib.prism_moe_block_forward(kw["x"], P, capi.BF16, 2, 128, 64, 4, 2, 1, P, P, kw["out"],
+                                           None, None, P, 1 << 30, None) == capi.ERR_ARG
+        assert b"16-byte aligned" in lib.prism_moe_last_error()
