@@ -284,7 +284,7 @@ int prism_moe_rmsnorm(const void* x, const void* residual, const void* weight, f
  *   out          = RMSNorm(that sum) with norm_weight and eps
  * instead of the block output, bit for bit what the plain entry point followed by
  * prism_moe_rmsnorm(out, residual, ...) gives, without the block output's round trip through
- * HBM. ``residual_out`` may alias neither ``residual`` nor ``out``.
+ * HBM. ``residual``, ``residual_out`` and ``out`` are three buffers: none may be another.
  */
 typedef struct prism_moe_norm_epilogue {
   const void* residual;      /* [T, H] dtype */

@@ -138,6 +138,9 @@ int check_block_buffers(const char* what, const void* x, const void* out, const 
     all |= reinterpret_cast<uintptr_t>(e->residual) | reinterpret_cast<uintptr_t>(e->norm_weight) |
            reinterpret_cast<uintptr_t>(e->residual_out);
   PRISM_CHECK_ARG(all % 16 == 0, "%s: buffers must be 16-byte aligned", what);
+  // the residual is read again after ``out`` and ``residual_out`` have been written
+  PRISM_CHECK_ARG(!e || (e->residual != out && e->residual != e->residual_out && e->residual_out != out),
+                  "%s: residual, residual_out and out must be three buffers", what);
   return PRISM_MOE_OK;
 }
 

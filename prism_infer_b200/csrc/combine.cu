@@ -166,8 +166,9 @@ int combine(const void* y, int dtype, const int32_t* entry_row, const void* w, i
   PRISM_CHECK_ARG(!src || !src->norm_weight || (src->residual && src->residual_out),
                   "combine: the norm epilogue needs residual and residual_out");
   PRISM_CHECK_ARG(!src || !src->norm_weight ||
-                      (src->residual_out != src->residual && src->residual_out != out),
-                  "combine: residual_out must not alias residual or out");
+                      (src->residual_out != src->residual && src->residual_out != out &&
+                       src->residual != out),
+                  "combine: residual, residual_out and out must be three buffers");
   if (T == 0) return PRISM_MOE_OK;
   const int64_t vpr = hidden * el / 16;
   CombineSource s = src ? *src : CombineSource{};

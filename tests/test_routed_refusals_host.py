@@ -65,7 +65,7 @@ def lib():
     return capi.load()
 
 
-def block(lib, x=P, out=P, ws=P, res=P, w=P, res_out=2 * P, dense=False, norm=True):
+def block(lib, x=P, out=P, ws=P, res=3 * P, w=P, res_out=2 * P, dense=False, norm=True):
     q = ctypes.byref(capi.W4(P, P, None, 64))
     epi = capi.NormEpilogue(res, w, 1e-6, res_out)
     experts = (P, P, None, None) if dense else (None, None, q, q)
@@ -76,7 +76,7 @@ def block(lib, x=P, out=P, ws=P, res=P, w=P, res_out=2 * P, dense=False, norm=Tr
 @pytest.mark.parametrize("dense", [False, True])
 def test_buffers_that_are_not_16_byte_aligned(lib, dense):
     """A view that starts inside a row: the kernels read 16 bytes at a time."""
-    for bad in (dict(x=P + 8), dict(x=P + 2), dict(out=P + 8), dict(ws=P + 4), dict(res=P + 2),
+    for bad in (dict(x=P + 8), dict(x=P + 2), dict(out=P + 8), dict(ws=P + 4), dict(res=3 * P + 2),
                 dict(w=P + 8), dict(res_out=2 * P + 4), dict(x=P + 8, norm=False)):
         assert block(lib, dense=dense, **bad) == capi.ERR_ARG, bad
         assert b"16-byte aligned" in lib.prism_moe_last_error()
@@ -85,3 +85,11 @@ def test_buffers_that_are_not_16_byte_aligned(lib, dense):
         assert lib.prism_moe_block_forward(kw["x"], P, capi.BF16, 2, 128, 64, 4, 2, 1, P, P, kw["out"],
                                            None, None, P, 1 << 30, None) == capi.ERR_ARG
         assert b"16-byte aligned" in lib.prism_moe_last_error()
+
+
+@pytest.mark.parametrize("dense", [False, True])
+def test_norm_epilogue_on_one_buffer_twice(lib, dense):
+    """The residual is read again for the second pass, after the outputs have been written."""
+    for bad in (dict(out=P, res=P), dict(res=P, res_out=P, out=3 * P), dict(out=P, res_out=P)):
+        assert block(lib, dense=dense, **bad) == capi.ERR_ARG, bad
+        assert b"three buffers" in lib.prism_moe_last_error()
