@@ -121,7 +121,8 @@ def _unpack_groups(v: torch.Tensor, N: int, n_groups: int) -> torch.Tensor:
 def pack_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None, *,
             group_size: int, gate_up: bool = False) -> W4Weight:
     """Lay out ``codes`` [.., N, K] (integers 0..15), ``scales`` and ``zeros`` [.., N, K/G] (any
-    quantiser's result). With ``gate_up`` the N rows are the I gate rows, then the I up rows."""
+    quantiser's result); scales are rounded to bf16 and must be finite there. With ``gate_up`` the N
+    rows are the I gate rows, then the I up rows."""
     N, K = codes.shape[-2:]
     if group_size not in GROUP_SIZES:
         raise RuntimeError(f"group_size {group_size} is not one of {GROUP_SIZES}")
@@ -136,7 +137,10 @@ def pack_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | Non
         if t is not None and t.numel() and (t.is_floating_point() or int(t.min()) < 0
                                             or int(t.max()) > 15):
             raise RuntimeError(f"{name} must be integers in 0..15")
-    parts = [codes.to(torch.uint8), scales.to(torch.bfloat16),
+    scales = scales.to(torch.bfloat16)
+    if not bool(scales.isfinite().all()):
+        raise RuntimeError("scales must be finite in bfloat16")
+    parts = [codes.to(torch.uint8), scales,
              None if zeros is None else zeros.to(torch.uint8)]
     if gate_up:
         parts = [None if t is None else _turns(t) for t in parts]
@@ -151,7 +155,8 @@ def quantize_w4(weight: torch.Tensor, group_size: int = 128, *, symmetric: bool 
 
     ``symmetric``: codes 1..15 around zero point 8, scale = largest magnitude / 7. Otherwise a zero
     point per group, scale = (max - min) / 15 over the group and zero, so that zero stays exact.
-    The scale is rounded to bf16 before the codes are chosen. A group of zeros gets scale 1.
+    The scale is rounded to bf16 before the codes are chosen. A group of zeros gets scale 1. Weights
+    that are not finite, or whose scale is not, are refused.
     """
     if group_size not in GROUP_SIZES:
         raise RuntimeError(f"group_size {group_size} is not one of {GROUP_SIZES}")
@@ -167,6 +172,8 @@ def quantize_w4(weight: torch.Tensor, group_size: int = 128, *, symmetric: bool 
         else:
             lo, hi = w.amin(-1).clamp_max(0), w.amax(-1).clamp_min(0)
             s = (hi - lo) / 15
+        if not bool(s.to(torch.bfloat16).isfinite().all()):   # a NaN weight makes its scale NaN
+            raise RuntimeError("quantize_w4: weights and their scales must be finite")
         s = torch.where(s > 0, s, torch.ones_like(s)).to(torch.bfloat16)
         s = s.clamp_min(torch.finfo(torch.bfloat16).tiny)
         sf = s.float().unsqueeze(-1)
