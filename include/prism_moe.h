@@ -330,7 +330,8 @@ int prism_moe_block_forward_norm(const void* x, const void* router_logits, int d
  * the optional norm epilogue. Experts are ``w_gate_up`` / ``w_down`` in dtype, or, where those are
  * NULL, the 4-bit ``q_gate_up`` / ``q_down`` (bf16 activations). Workspace: that of
  * prism_moe_block_forward. Ids outside [0, E) add nothing to ``out`` and record PRISM_MOE_ERR_ARG in
- * the workspace's first word.
+ * the workspace's first word, or, with ``_reporting``, in ``device_error`` (NULL: the workspace's
+ * first word; else that need not be zero).
  */
 int prism_moe_block_forward_routed(const void* x, const int64_t* topk_ids,
                                    const void* topk_weights, int dtype, int64_t num_tokens,
@@ -339,6 +340,12 @@ int prism_moe_block_forward_routed(const void* x, const int64_t* topk_ids,
                                    const prism_moe_w4* q_gate_up, const prism_moe_w4* q_down,
                                    void* out, void* workspace, size_t workspace_bytes,
                                    void* stream, const prism_moe_norm_epilogue* epilogue);
+int prism_moe_block_forward_routed_reporting(
+    const void* x, const int64_t* topk_ids, const void* topk_weights, int dtype, int64_t num_tokens,
+    int64_t hidden, int64_t inter, int32_t num_experts, int32_t top_k, const void* w_gate_up,
+    const void* w_down, const prism_moe_w4* q_gate_up, const prism_moe_w4* q_down, void* out,
+    void* workspace, size_t workspace_bytes, int* device_error, void* stream,
+    const prism_moe_norm_epilogue* epilogue);
 
 /* ---------------------------------------------------------------------------------------------
  * Expert parallelism over NVLink peer memory (one process per GPU).
@@ -456,6 +463,10 @@ int prism_moe_profile_events(void* const* events, int32_t count);
  * prism_moe_expert_swiglu, or the start of a prism_moe_block_forward workspace.
  */
 int prism_moe_read_device_error(int* device_error, void* stream);
+
+/* The library's own error word on the current device, for calls without a better place: it exists as
+ * long as the process does, so captured graphs can name it, and all its users share it. */
+int prism_moe_device_error_word(int** word);
 
 #ifdef __cplusplus
 }

@@ -66,6 +66,10 @@ _SIGNATURES = {
     "prism_moe_block_forward_routed": (ctypes.c_int, [_vp, _vp, _vp, ctypes.c_int, _i64, _i64,
                                                       _i64, _i32, _i32, _vp, _vp, _w4p, _w4p, _vp,
                                                       _vp, _sz, _vp, _ep]),
+    "prism_moe_block_forward_routed_reporting": (
+        ctypes.c_int, [_vp, _vp, _vp, ctypes.c_int, _i64, _i64, _i64, _i32, _i32, _vp, _vp, _w4p,
+                       _w4p, _vp, _vp, _sz, _vp, _vp, _ep]),
+    "prism_moe_device_error_word": (ctypes.c_int, [ctypes.POINTER(_vp)]),
     "prism_moe_dispatch_workspace_size": (_sz, [_i64, _i32, _i32, _i32]),
     "prism_moe_build_dispatch_plan": (ctypes.c_int, [_vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp,
                                                      _vp, _vp, _vp, _vp, _sz, _vp]),
@@ -214,6 +218,33 @@ def _one_device(first, *others) -> int:
     return index
 
 
+_error_words: dict = {}
+
+
+def device_error_word(index: int) -> int:
+    """Address of the library's error word on device ``index``, where calls that are given none record
+    a failing kernel's status, captured ones included (prism_moe_device_error_word)."""
+    at = _error_words.get(index)
+    if at is None:
+        word = ctypes.c_void_p()
+        with _torch().cuda.device(index):
+            check(load().prism_moe_device_error_word(ctypes.byref(word)),
+                  "prism_moe_device_error_word")
+        at = _error_words[index] = word.value
+    return at
+
+
+def check_device_error(device=None) -> None:
+    """Synchronise the current stream of ``device`` and raise (once) if a kernel recorded a failure in
+    its ``device_error_word``: any call's on that device, so what ran on other streams too, as far as
+    it has ended."""
+    torch = _torch()
+    index = torch.cuda.current_device() if device is None else torch.device(device).index
+    with torch.cuda.device(index):
+        check(load().prism_moe_read_device_error(device_error_word(torch.cuda.current_device()),
+                                                 stream_of(None)), "kernels on this device")
+
+
 def _launch(index: int, what: str, fn, *args) -> None:
     """``fn(*args, stream)`` with device ``index`` current, on its current torch stream (the raw
     handle: a Stream object costs more host time than the launch)."""
@@ -303,7 +334,8 @@ def permute_rows(x, top_k: int, entry_row, out=None):
 
 def expert_swiglu(x_sorted, seg_offsets, w_gate_up, w_down, seg_expert=None, y=None,
                   device_error=None):
-    """Kernel 4: grouped SwiGLU experts over the segment table (int32 device tensors)."""
+    """Kernel 4: grouped SwiGLU experts over the segment table (int32 device tensors).
+    ``device_error`` None: errors go to ``device_error_word``'s word."""
     torch = _torch()
     _need_cuda(x_sorted, seg_offsets, w_gate_up, w_down, seg_expert)
     R, H = x_sorted.shape
@@ -322,7 +354,9 @@ def expert_swiglu(x_sorted, seg_offsets, w_gate_up, w_down, seg_expert=None, y=N
     nseg = seg_offsets.numel() - 1
     check(lib.prism_moe_expert_swiglu(ptr(x_sorted), dt, R, H, I, ptr(seg_offsets),
                                       ptr(seg_expert), nseg, El, ptr(w_gate_up), ptr(w_down),
-                                      ptr(y), ptr(ws), ws_bytes, ptr(device_error),
+                                      ptr(y), ptr(ws), ws_bytes,
+                                      device_error_word(x_sorted.get_device())
+                                      if device_error is None else ptr(device_error),
                                       stream_of(x_sorted.device)), "prism_moe_expert_swiglu")
     return y
 
@@ -339,7 +373,8 @@ def _need_bf16(x, what: str) -> None:
 def linear_w4(x, weight, out=None, device_error=None):
     """y = x W^T for a 4-bit ``weight`` (``quant.W4Weight``, a single matrix): ``x`` [M, K] bf16, any
     M from 0; returns [M, N] bf16 (``out``, which must not overlap ``x``). ``device_error``: an int32
-    device word that a failing kernel records its status in (prism_moe_linear_w4)."""
+    device word that a failing kernel records its status in (None: ``device_error_word``'s;
+    prism_moe_linear_w4)."""
     torch = _torch()
     _need_bf16(x, "linear_w4")
     if weight.stack is not None or weight.gate_up:
@@ -356,7 +391,8 @@ def linear_w4(x, weight, out=None, device_error=None):
     elif tuple(out.shape) != (M, N) or out.dtype != x.dtype:
         raise RuntimeError("linear_w4: out must be [M, N] in x's dtype")
     _launch(dev, "prism_moe_linear_w4", load().prism_moe_linear_w4, x.data_ptr(), M,
-            weight.in_features, N, ctypes.byref(_w4(weight)), out.data_ptr(), ptr(device_error))
+            weight.in_features, N, ctypes.byref(_w4(weight)), out.data_ptr(),
+            device_error_word(dev) if device_error is None else ptr(device_error))
     return out
 
 
@@ -374,7 +410,8 @@ def expert_swiglu_w4(x_sorted, seg_offsets, w_gate_up, w_down, seg_expert=None, 
                      device_error=None):
     """Grouped SwiGLU experts on 4-bit weights (``quant.W4Weight`` stacks) over the segment table:
     ``expert_swiglu`` with ``w_gate_up`` [El, 2I, H] and ``w_down`` [El, H, I] in 4 bits and bf16
-    activations (prism_moe_expert_swiglu_w4). ``seg_offsets`` None: all rows are one segment."""
+    activations (prism_moe_expert_swiglu_w4). ``seg_offsets`` None: all rows are one segment.
+    ``device_error`` None: errors go to ``device_error_word``'s word."""
     torch = _torch()
     _need_bf16(x_sorted, "expert_swiglu_w4")
     if x_sorted.dim() != 2:
@@ -402,7 +439,7 @@ def expert_swiglu_w4(x_sorted, seg_offsets, w_gate_up, w_down, seg_expert=None, 
     _launch(dev, "prism_moe_expert_swiglu_w4", lib.prism_moe_expert_swiglu_w4,
             x_sorted.data_ptr(), R, H, I, ptr(seg_offsets), ptr(seg_expert), nseg, El,
             ctypes.byref(_w4(w_gate_up)), ctypes.byref(_w4(w_down)), y.data_ptr(), ws.data_ptr(),
-            ws_bytes, ptr(device_error))
+            ws_bytes, device_error_word(dev) if device_error is None else ptr(device_error))
     return y
 
 
@@ -529,15 +566,13 @@ def block_forward(x, router_logits, w_gate_up, w_down, top_k: int, renorm: bool,
 
 
 def _routed_workspace(device, nbytes: int):
-    """The block's scratch: the (device, stream) workspace, or, while a CUDA graph is captured,
-    memory of that graph's own (two graphs never share it; its error word starts zero at every
-    replay and is not the one ``block_error_word`` returns)."""
+    """The block's scratch and the address of its error word: the (device, stream) workspace and its own
+    (None), or, while a CUDA graph is captured, memory of that graph's own (two graphs never share
+    it) and ``device_error_word``'s."""
     torch = _torch()
     if torch.cuda.is_current_stream_capturing():
-        ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
-        ws[:256].zero_()
-        return ws
-    return block_workspace(device, nbytes)
+        return torch.empty(nbytes, dtype=torch.uint8, device=device), device_error_word(device.index)
+    return block_workspace(device, nbytes), None
 
 
 def block_forward_routed(x, topk_ids, topk_weights, w_gate_up, w_down, out=None, epilogue=None):
@@ -579,10 +614,10 @@ def block_forward_routed(x, topk_ids, topk_weights, w_gate_up, w_down, out=None,
     quant = (ctypes.byref(_w4(w_gate_up)), ctypes.byref(_w4(w_down))) if w4 else (None, None)
     with torch.cuda.device(dev):
         nbytes = lib.prism_moe_block_workspace_size(T, H, I, E, k, dt)
-        ws = _routed_workspace(x.device, nbytes)
-        check(lib.prism_moe_block_forward_routed(
+        ws, word = _routed_workspace(x.device, nbytes)
+        check(lib.prism_moe_block_forward_routed_reporting(
             ptr(x), ptr(topk_ids), ptr(topk_weights), dt, T, H, I, E, k, *dense, *quant, ptr(out),
-            ptr(ws), ws.numel(), stream_of(x.device),
+            ptr(ws), ws.numel(), word, stream_of(x.device),
             ctypes.byref(epilogue) if epilogue is not None else None),
             "prism_moe_block_forward_routed")
     return out

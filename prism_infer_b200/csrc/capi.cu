@@ -40,6 +40,7 @@ std::atomic<uint64_t> g_wait_ns{2000000000ull};        // 2 s: far above any leg
 std::atomic<uint64_t> g_peer_wait_ns{10000000000ull};  // 10 s: peers may start a step late
 std::mutex g_attr_mu;
 std::set<std::pair<const void*, int>> g_attr_done;
+__device__ int g_device_error;   // one on each device (prism_moe_device_error_word)
 }  // namespace
 
 int expert_engine_setting() { return g_engine.load(std::memory_order_relaxed); }
@@ -181,13 +182,14 @@ int expert_swiglu_w4(const void* xs, int64_t rows, int64_t H, int64_t I,
   return r;
 }
 
-// Plan, gather, experts (dense, or 4-bit where ``q_gu`` is given) and combine for routed tokens.
+// Plan, gather, experts (dense, or 4-bit where ``q_gu`` is given) and combine for routed tokens. Errors
+// go to ``err``, or to the workspace's first word where that is NULL.
 int block_after_router(const void* x, const int64_t* ids, const void* w, int dtype, int64_t T,
                        int64_t H, int64_t I, int E, int k, const void* w_gate_up,
                        const void* w_down, const prism_moe_w4* q_gu, const prism_moe_w4* q_dn,
-                       void* out, char* ws, const BlockLayout& L,
+                       void* out, char* ws, const BlockLayout& L, int* err,
                        const prism_moe_norm_epilogue* epilogue, cudaStream_t st) {
-  int* err = reinterpret_cast<int*>(ws + L.err);
+  if (!err) err = reinterpret_cast<int*>(ws + L.err);
   int32_t* counts = reinterpret_cast<int32_t*>(ws + L.counts);
   int32_t* offsets = reinterpret_cast<int32_t*>(ws + L.offsets);
   int32_t* entry_row = reinterpret_cast<int32_t*>(ws + L.entry_row);
@@ -461,7 +463,7 @@ int prism_moe_block_forward_norm(const void* x, const void* router_logits, int d
   int r = route_topk(router_logits, dtype, num_tokens, num_experts, top_k, renorm, ids, w, nullptr, st);
   if (r) return r;
   return block_after_router(x, ids, w, dtype, num_tokens, hidden, inter, num_experts, top_k,
-                            w_gate_up, w_down, nullptr, nullptr, out, ws, L, epilogue, st);
+                            w_gate_up, w_down, nullptr, nullptr, out, ws, L, nullptr, epilogue, st);
 }
 
 int prism_moe_block_forward_routed(const void* x, const int64_t* topk_ids,
@@ -471,6 +473,18 @@ int prism_moe_block_forward_routed(const void* x, const int64_t* topk_ids,
                                    const prism_moe_w4* q_gate_up, const prism_moe_w4* q_down,
                                    void* out, void* workspace, size_t workspace_bytes,
                                    void* stream, const prism_moe_norm_epilogue* epilogue) {
+  return prism_moe_block_forward_routed_reporting(x, topk_ids, topk_weights, dtype, num_tokens, hidden,
+                                                  inter, num_experts, top_k, w_gate_up, w_down,
+                                                  q_gate_up, q_down, out, workspace, workspace_bytes,
+                                                  nullptr, stream, epilogue);
+}
+
+int prism_moe_block_forward_routed_reporting(
+    const void* x, const int64_t* topk_ids, const void* topk_weights, int dtype, int64_t num_tokens,
+    int64_t hidden, int64_t inter, int32_t num_experts, int32_t top_k, const void* w_gate_up,
+    const void* w_down, const prism_moe_w4* q_gate_up, const prism_moe_w4* q_down, void* out,
+    void* workspace, size_t workspace_bytes, int* device_error, void* stream,
+    const prism_moe_norm_epilogue* epilogue) {
   PRISM_CHECK_ARG(dtype_ok(dtype), "block_forward_routed: unknown dtype %d", dtype);
   PRISM_CHECK_ARG(num_tokens >= 0 && hidden >= 1 && inter >= 1, "block_forward_routed: bad shape");
   PRISM_CHECK_ARG(num_experts >= 1 && num_experts <= 1024,
@@ -501,7 +515,7 @@ int prism_moe_block_forward_routed(const void* x, const int64_t* topk_ids,
   record_stage(0, st);
   return block_after_router(x, topk_ids, topk_weights, dtype, num_tokens, hidden, inter,
                             num_experts, top_k, w_gate_up, w_down, q_gate_up, q_down, out,
-                            static_cast<char*>(workspace), L, epilogue, st);
+                            static_cast<char*>(workspace), L, device_error, epilogue, st);
 }
 
 int prism_moe_block_forward(const void* x, const void* router_logits, int dtype,
@@ -557,6 +571,15 @@ int prism_moe_set_wait_limits(int64_t wait_ns, int64_t peer_wait_ns) {
                   std::memory_order_relaxed);
   g_peer_wait_ns.store(peer_wait_ns > 0 ? static_cast<uint64_t>(peer_wait_ns) : 10000000000ull,
                        std::memory_order_relaxed);
+  return PRISM_MOE_OK;
+}
+
+int prism_moe_device_error_word(int** word) {
+  PRISM_CHECK_ARG(word != nullptr, "device_error_word: null pointer");
+  if (int r = check_device()) return r;
+  void* at = nullptr;
+  PRISM_CUDA(cudaGetSymbolAddress(&at, g_device_error));
+  *word = static_cast<int*>(at);
   return PRISM_MOE_OK;
 }
 

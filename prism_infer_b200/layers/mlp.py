@@ -16,7 +16,7 @@ from __future__ import annotations
 import torch
 from torch import nn
 
-from prism_infer_b200 import ops  # noqa: F401  (registers torch.ops.prism_moe)
+from prism_infer_b200 import capi, ops  # noqa: F401  (registers torch.ops.prism_moe)
 from prism_infer_b200.layers.w4 import W4Holder
 from prism_infer_b200.quant import quantize_w4
 
@@ -89,6 +89,11 @@ class Qwen3MLP(nn.Module):
         self.gate_up_proj = self.down_proj = None
         return self
 
+    def check_device_error(self) -> None:
+        """Synchronise and raise if a kernel recorded an error (``capi.check_device_error``)."""
+        held = self.gate_up_proj.weight if self.w4_gate_up is None else self.w4_gate_up.qweight
+        capi.check_device_error(held.device)
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         shape = x.shape
         x2 = x.reshape(-1, shape[-1])
@@ -101,7 +106,8 @@ class Qwen3MLP(nn.Module):
             if shape[-1] != self.hidden_size:
                 raise RuntimeError(f"input has {shape[-1]} features, not {self.hidden_size}")
             y = torch.ops.prism_moe.expert_swiglu_w4(
-                x2, None, gu.qweight, gu.scales, gu.zeros, dn.qweight, dn.scales, dn.zeros, self.intermediate_size, gu.group_size, dn.group_size, None)
+                x2, None, gu.qweight, gu.scales, gu.zeros, dn.qweight, dn.scales, dn.zeros,
+                self.intermediate_size, gu.group_size, dn.group_size, None)
             return y.view(shape)
         wgu = self.gate_up_proj.weight
         wd = self.down_proj.weight

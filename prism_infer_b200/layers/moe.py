@@ -221,7 +221,8 @@ class MoE(ExpertBank):
         return out.view(orig_shape)
 
     def check_device_error(self, device=None) -> None:
-        """Synchronise and raise if a kernel of the last forward recorded an error."""
+        """Synchronise and raise if a kernel of the last forward recorded an error. A replayed graph's
+        show up here too, as do other modules' that share ``capi.device_error_word``."""
         if self.ep_moe is not None:
             self.ep_moe.check_device_error()
             return
@@ -229,3 +230,4 @@ class MoE(ExpertBank):
         word = capi.block_error_word(dev)
         if word is not None:
             capi.check(capi.read_device_error(word, dev), "MoE kernels")
+        capi.check_device_error(dev)

@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 from torch import nn
 
-from prism_infer_b200 import ops  # noqa: F401  (registers torch.ops.prism_moe)
+from prism_infer_b200 import capi, ops  # noqa: F401  (registers torch.ops.prism_moe)
 from prism_infer_b200.quant import W4Weight, quantize_w4
 
 
@@ -53,6 +53,10 @@ class W4Linear(W4Holder):
                     symmetric: bool = True) -> "W4Linear":
         """Quantise a [out_features, in_features] weight (round to nearest)."""
         return cls(quantize_w4(weight.detach(), group_size, symmetric=symmetric))
+
+    def check_device_error(self) -> None:
+        """Synchronise and raise if a kernel recorded an error (``capi.check_device_error``)."""
+        capi.check_device_error(self.qweight.device)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if x.shape[-1] != self.in_features:
