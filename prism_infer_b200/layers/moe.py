@@ -202,6 +202,13 @@ class MoE(ExpertBank):
                                                      self.top_k, renorm, bank.op_id)
                 return out.view(orig_shape)
             ids, w = self._choose(logits, x.dtype)
+            if bank.use_p2p(x):
+                args = (x, ids, w, bank.w_gate_up, bank.w_down, bank.op_id)
+                if fuse:
+                    out, res = torch.ops.prism_moe.ep_forward_routed_norm(
+                        *args, residual.reshape(x.shape), norm.weight, float(norm.eps))
+                    return out.view(orig_shape), res.view(orig_shape)
+                return torch.ops.prism_moe.ep_forward_routed(*args).view(orig_shape)
             out = bank(x, ids, w)
             if fuse:
                 out, res = norm(out, residual.reshape(x.shape))

@@ -32,7 +32,9 @@ Ops (shapes: T tokens, H hidden, E experts, k top-k, W expert-parallel ranks):
   scale, out_dtype) -> (topk_ids[T,k] int64, topk_weights[T,k])``: routing by softmax or sigmoid
   scores with a selection bias and expert groups (no counterpart in the reference).
 * ``block_forward_routed(x, topk_ids, topk_weights, w_gate_up, w_down) -> out[T,H]``: the block after
-  a router of the caller's choice; ``block_forward_routed_norm`` with the norm fused.
+  a router of the caller's choice; ``block_forward_routed_norm`` with the norm fused;
+  ``ep_forward_routed(x, topk_ids, topk_weights, w_gate_up, w_down, bank)`` and its ``_norm`` the
+  expert-parallel step for such a choice.
 * 4-bit weights (``quant.W4Weight`` as its tensors ``q, scales, zeros`` and group size):
   ``linear_w4(x[M,K], q, scales, zeros, out_features, group_size) -> y[M,N]``,
   ``expert_swiglu_w4(x_sorted, seg_offsets, gate_up q/scales/zeros, down q/scales/zeros, inter,
@@ -141,15 +143,20 @@ def _(x, router_logits, w_gate_up, w_down, top_k, renorm):
     return torch.empty_like(x)
 
 
+def _ep_bank(what: str, bank: int, w_gate_up: Tensor, w_down: Tensor):
+    owner = _EP_BANKS.get(bank)
+    if owner is None:
+        raise RuntimeError(f"prism_moe::{what}: unknown expert-parallel bank id")
+    if owner.w_gate_up.data_ptr() != w_gate_up.data_ptr() or \
+            owner.w_down.data_ptr() != w_down.data_ptr():
+        raise RuntimeError(f"prism_moe::{what}: weights are not the bank's")
+    return owner
+
+
 @custom_op("prism_moe::ep_forward", mutates_args=())
 def ep_forward(x: Tensor, router_logits: Tensor, w_gate_up: Tensor, w_down: Tensor, top_k: int,
                renorm: bool, bank: int) -> Tensor:
-    owner = _EP_BANKS.get(bank)
-    if owner is None:
-        raise RuntimeError("prism_moe::ep_forward: unknown expert-parallel bank id")
-    if owner.w_gate_up.data_ptr() != w_gate_up.data_ptr() or \
-            owner.w_down.data_ptr() != w_down.data_ptr():
-        raise RuntimeError("prism_moe::ep_forward: weights are not the bank's")
+    owner = _ep_bank("ep_forward", bank, w_gate_up, w_down)
     return owner.forward_p2p(x, router_logits=router_logits, top_k=top_k, renorm=renorm)
 
 
@@ -252,6 +259,32 @@ def block_forward_routed_norm(x: Tensor, topk_ids: Tensor, topk_weights: Tensor,
 
 @block_forward_routed_norm.register_fake
 def _(x, topk_ids, topk_weights, w_gate_up, w_down, residual, norm_weight, eps):
+    return torch.empty_like(x), torch.empty_like(x)
+
+
+@custom_op("prism_moe::ep_forward_routed", mutates_args=())
+def ep_forward_routed(x: Tensor, topk_ids: Tensor, topk_weights: Tensor, w_gate_up: Tensor,
+                      w_down: Tensor, bank: int) -> Tensor:
+    owner = _ep_bank("ep_forward_routed", bank, w_gate_up, w_down)
+    return owner.forward_p2p(x, topk_ids=topk_ids, topk_weights=topk_weights)
+
+
+@ep_forward_routed.register_fake
+def _(x, topk_ids, topk_weights, w_gate_up, w_down, bank):
+    return torch.empty_like(x)
+
+
+@custom_op("prism_moe::ep_forward_routed_norm", mutates_args=())
+def ep_forward_routed_norm(x: Tensor, topk_ids: Tensor, topk_weights: Tensor, w_gate_up: Tensor,
+                           w_down: Tensor, bank: int, residual: Tensor, norm_weight: Tensor,
+                           eps: float) -> tuple[Tensor, Tensor]:
+    owner = _ep_bank("ep_forward_routed_norm", bank, w_gate_up, w_down)
+    return owner.forward_p2p(x, topk_ids=topk_ids, topk_weights=topk_weights, residual=residual,
+                             norm_weight=norm_weight, eps=eps)
+
+
+@ep_forward_routed_norm.register_fake
+def _(x, topk_ids, topk_weights, w_gate_up, w_down, bank, residual, norm_weight, eps):
     return torch.empty_like(x), torch.empty_like(x)
 
 

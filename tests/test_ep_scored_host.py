@@ -1,0 +1,44 @@
+"""The scored router under expert parallelism as operators, traced without a GPU."""
+import pytest
+import torch
+
+from prism_infer_b200 import ops  # noqa: F401
+from prism_infer_b200.engine.parallel import set_expert_parallel_size
+from prism_infer_b200.engine.parallel.expert_parallel import ExpertParallelMoE
+from prism_infer_b200.layers.layernorm import RMSNorm
+from prism_infer_b200.layers.moe import MoE
+
+H, I, E, K = 128, 64, 8, 2
+
+
+class Step(torch.nn.Module):
+    def __init__(self, fuse):
+        super().__init__()
+        set_expert_parallel_size(1)
+        self.moe = MoE(H, I, E, K, scoring="sigmoid", num_groups=4, topk_groups=2)
+        # what rank 0 of two builds
+        self.moe.ep_size, self.moe.experts = 2, None
+        self.moe.ep_moe = ExpertParallelMoE(H, I, E, 2, 0, transport="p2p")
+        self.norm = RMSNorm(H) if fuse else None
+
+    def forward(self, x, residual):
+        return self.moe(x, residual=residual, norm=self.norm) if self.norm is not None else self.moe(x)
+
+
+@pytest.mark.parametrize("fuse", [False, True])
+def test_scored_expert_parallel_step_is_one_graph(fuse):
+    step = Step(fuse).to("meta", torch.bfloat16)
+    x = torch.empty(2, 5, H, device="meta", dtype=torch.bfloat16)
+    out = step(x, x)
+    assert all(o.shape == x.shape and o.dtype == x.dtype for o in (out if fuse else (out,)))
+    called = [str(n.target) for n in torch.export.export(step, (x, x)).graph.nodes
+              if n.op == "call_function"]
+    assert "prism_moe.route_scored.default" in called
+    assert f"prism_moe.ep_forward_routed{'_norm' if fuse else ''}.default" in called
+
+
+def test_a_bank_that_is_not_there():
+    x = torch.zeros(2, H, dtype=torch.bfloat16)
+    ids, w = torch.zeros(2, K, dtype=torch.int64), torch.zeros(2, K, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="unknown expert-parallel bank"):
+        torch.ops.prism_moe.ep_forward_routed(x, ids, w, x, x, -1)
