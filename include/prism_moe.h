@@ -224,7 +224,9 @@ typedef struct prism_moe_w4 {
  * y = x W^T for 4-bit weights: x [rows, in_features] and y [rows, out_features] bf16, row-major,
  * 16-byte aligned, out_features % 8 == 0; any number of rows, one (a matrix-vector product)
  * included. Sums are fp32, scales are applied to fp32 group sums, y is rounded once. y must not overlap
- * x. A row of x that holds an infinity or NaN gives outputs that are infinite or NaN, in that row only.
+ * x. Activations may be up to 2^113 (1e34) in magnitude: beyond, a group's fp32 sum can overflow before
+ * its scale is applied. A row of x that holds an infinity or NaN, or such a sum, gives outputs that
+ * are infinite or NaN, in that row only.
  * ``device_error``: int32 device word, or NULL; a wait inside a kernel that runs out is recorded there.
  * Replaces F.linear of prism_infer/layers/linear.py:77,181 on quantised weights.
  */
@@ -240,8 +242,8 @@ size_t prism_moe_expert_w4_workspace_size(int64_t rows_capacity, int64_t inter);
  * must be multiples of their matrix's group size. The gate and up sums stay in fp32; their product
  * silu(g) * u is rounded to bf16, the operand type of the second product. seg_offsets as there, up to
  * 1024 segments; NULL: one segment of all rows. Any number of segments may name the same expert. y may
- * be x_sorted. Rows of no segment are left as they are; a segment whose seg_expert lies outside [0, num_local_experts) is skipped and
- * records PRISM_MOE_ERR_ARG in ``device_error``.
+ * be x_sorted. Rows of no segment are left as they are; a segment whose seg_expert lies outside
+ * [0, num_local_experts) is skipped and records PRISM_MOE_ERR_ARG in ``device_error``.
  */
 int prism_moe_expert_swiglu_w4(const void* x_sorted, int64_t rows_capacity, int64_t hidden,
                                int64_t inter, const int32_t* seg_offsets,

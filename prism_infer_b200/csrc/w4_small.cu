@@ -18,7 +18,8 @@
 // 16 where one bit's shift puts it under a smaller exponent (w4.cuh), which makes three shifts per
 // word: shifts and logic share a half-rate pipe and are what the loop has most of. The price is
 // cancellation: the sums carry up to 143 per input instead of 8, at most 2^-17 of their terms'
-// magnitudes at 4096 inputs where the output's rounding is 2^-8.
+// magnitudes at 4096 inputs where the output's rounding is 2^-8; and range: 143 * 128 * |x| stays in
+// fp32 up to |x| = 2^113.
 //
 // What bounds it: few rows reuse nothing, so every hit weight crosses HBM once and that is the floor.
 // What keeps it from that is latency inside the warps: 16 of them an SM, as many as registers allow, each
