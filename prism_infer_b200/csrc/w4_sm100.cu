@@ -31,7 +31,8 @@
 // and four reads of the accumulator per chunk bound groups of 32. A tile's output adds about 5400 cycles
 // in which the MMAs stand (no third TMEM buffer fits).
 // Measured: 8192 x 4736 x 4096, groups of 128: 268 us (1184 TFLOP/s); of 64 with zero points 318 us
-// (1001); of 32 469 us (678). 8192 tokens of 32 experts, top 4, 4096 x 1024: 901 us (915).
+// (1001); of 32 469 us (678). 8192 tokens of 32 experts, top 4, 4096 x 1024: 907 us (909) one at a
+// time, 1045 (789) one after the other, where the power limit lowers the clock.
 // Every wait is bounded; one that runs out records PRISM_MOE_ERR_TIMEOUT and the CTA drains its
 // copies and MMAs before it frees TMEM.
 #include <algorithm>
@@ -45,9 +46,11 @@ namespace prism {
 namespace {
 
 constexpr int kRowsW = 128;      // weight rows per tile
-// Average rows per segment up to which tiles are narrow. 128 experts of 2048 x 768, groups of 128,
-// both products, narrow and wide: 32 rows on average 211 and 303 us, 64 rows 297 and 322, 96 rows 373
-// and 324. One segment, 18944 x 4096: 64 rows 35.0 and 36.9 us, 96 rows 45 and 37.
+// Average rows per segment up to which tiles are narrow, for every group size. 128 experts of
+// 2048 x 768, both products, narrow and wide, 32, 64 and 80 rows on average: groups of 128 195 and
+// 289 us, 285 and 304, 369 and 311; of 64 with zero points 241 and 315, 356 and 358, 440 and 374; of 32
+// 361 and 425, 534 and 580, 662 and 601; with zero points 377 and 406, 533 and 560, 709 and 580. One
+// segment, 18944 x 4096, groups of 128: 64 rows 35.0 and 36.9 us, 96 rows 45 and 37.
 constexpr int kNarrowRows = 64;
 constexpr int kTokBox = 64;      // activation rows per copy
 constexpr int kPackStage = 8 * 1024;

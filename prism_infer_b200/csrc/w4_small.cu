@@ -29,7 +29,7 @@
 // experts, top 8, 2048 x 768, both products 88 us (3.5 TB/s); one token of them 17, where two
 // launches and three memory latencies are most of it.
 // A block's warps split the inputs (kw ways) and keep their part of x in registers while the block
-// streams its row tiles; the partial sums meet in shared memory in a fixed order. Every lane copies
+// streams its row tiles (up to 2048 inputs; of longer rows every item loads x again, part by part); the partial sums meet in shared memory in a fixed order. Every lane copies
 // the 16-byte pieces that it will use itself (cp.async, kDepth row tiles ahead, across the borders
 // of blocks of rows), so no barrier stands between a copy and its use. Blocks take equal runs of a
 // device-side list of (segment's rows, output tiles), so the host needs no counts.
@@ -487,9 +487,12 @@ int w4_product(const W4Problem& pr, cudaStream_t st) {
   // Few rows: this kernel alone (a longer segment runs in blocks of 16 rows, its weights from L2
   // after the first). Without a table: up to 16 rows, and up to 64 while the matrix is so small that
   // the other kernel's tiles could not fill the GPU (17 x 4096 x 4096: 17 us here, 29 there;
-  // 17 x 18944 x 4096: 39 and 33). With one: segments of 12 rows on average (128 experts of
-  // 2048 x 768, both products: 1536 rows 178 us here and 191 with both, 1792 rows 201 and 190). Else segments of at most kSmallRows rows run here and longer
-  // ones on the other kernel; the host does not know the lengths and launches both.
+  // 17 x 18944 x 4096: 39 and 33). With one: segments of 12 rows on average, for every group size
+  // (128 experts of 2048 x 768, both products, here and with both kernels, 12 and 16 rows on average:
+  // groups of 128 169 and 189 us, 222 and 175; of 64 with zero points 167 and 184, 214 and 194; of 32
+  // 174 and 188, 223 and 213; with zero points 186 and 200, 239 and 222). Else segments of at most
+  // kSmallRows rows run here and longer ones on the other kernel; the host does not know the lengths
+  // and launches both.
   // the lists of row blocks and output tiles count in 32 bits
   PRISM_CHECK_ARG(ceil_div(pr.rows_cap, 8) * pr.nseg < (int64_t(1) << 31), "4-bit product: too many rows");
   const int64_t out_tiles = ceil_div(pr.swiglu ? 2 * pr.n_out : pr.n_out, 16);
@@ -503,8 +506,9 @@ int w4_product(const W4Problem& pr, cudaStream_t st) {
     p.max_rows = kSmallRows;
   }
   // The two kernels of a product share neither rows nor weights, so this one fills the SMs that the
-  // other's last tiles leave (333 tokens of 60 experts, top 4, 1440 x 736, both products: 88 us, one
-  // kernel after the other 102; 4096 tokens of 128 experts, skewed: 617 and 629).
+  // other's last tiles leave (333 tokens of 60 experts, top 4, 1440 x 736, groups of 32 with zero points,
+  // both products: 96 us, one kernel after the other 107; 4096 tokens of 128 experts, skewed: 607
+  // and 634).
   p.start = !few ? kBeside : pr.after_product ? kEarly : kAfter;
   p.x = static_cast<const uint16_t*>(pr.x);
   p.ld_x = pr.K;
