@@ -29,10 +29,11 @@
 // experts, top 8, 2048 x 768, both products 88 us (3.5 TB/s); one token of them 17, where two
 // launches and three memory latencies are most of it.
 // A block's warps split the inputs (kw ways) and keep their part of x in registers while the block
-// streams its row tiles (up to 2048 inputs; of longer rows every item loads x again, part by part); the partial sums meet in shared memory in a fixed order. Every lane copies
-// the 16-byte pieces that it will use itself (cp.async, kDepth row tiles ahead, across the borders
-// of blocks of rows), so no barrier stands between a copy and its use. Blocks take equal runs of a
-// device-side list of (segment's rows, output tiles), so the host needs no counts.
+// streams its row tiles (up to 2048 inputs; of longer rows every item loads x again, part by part); the
+// partial sums meet in shared memory in a fixed order. Every lane copies the 16-byte pieces that it will
+// use itself (cp.async, kDepth row tiles ahead, across the borders of blocks of rows), so no barrier
+// stands between a copy and its use. Blocks take equal runs of a device-side list of (segment's rows,
+// output tiles), so the host needs no counts.
 #include <algorithm>
 
 #include "internal.h"

@@ -81,6 +81,29 @@ def test_logits_that_only_32_bits_tell_apart(scoring):
             check_ids(logits, k, scoring=scoring, num_groups=4, topk_groups=keep)
 
 
+@pytest.mark.parametrize("value", [float("-inf"), torch.finfo(torch.float32).min, -100.0, -17.0])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("groups,keep", [(8, 3), (6, 4), (5, 2)])
+def test_groups_that_are_masked(value, scoring, groups, keep):
+    """Whole groups at a masking value, more of them than go, and by rows also less."""
+    E = 240
+    g = gen_of(groups)
+    logits = torch.randn(200, E, generator=g, device=DEV)
+    masked = torch.rand(200, groups, generator=g, device=DEV) < 0.5
+    logits[masked.repeat_interleave(E // groups, 1)] = value
+    logits[0] = value
+    bias = 0.1 * torch.randn(E, generator=g, device=DEV)
+    for b in (None, bias, torch.zeros(E, device=DEV)):
+        for score in ("max", "top2"):
+            ids, w, _ = capi.route_scored(logits, 8, scoring=scoring, bias=b, num_groups=groups,
+                                          topk_groups=keep, group_score=score)
+            r_ids, r_w = route_scored_ref(logits, 8, scoring=scoring, bias=b, num_groups=groups,
+                                          topk_groups=keep, group_score=score)
+            assert torch.equal(ids, r_ids)
+            torch.testing.assert_close(w.double(), r_w, rtol=2.0 ** -18, atol=9 * 2.0 ** -148 / 1e-20,
+                                       equal_nan=True)
+
+
 # ------------------------------------------------------------------------------ the bottom of the range
 
 @pytest.mark.parametrize("score", ["max", "top2"])
