@@ -167,8 +167,26 @@ class ExpertParallelMoE(ExpertBank):
 
         With ``residual`` and ``norm_weight`` the final combine also applies the decoder layer's
         next residual add + RMSNorm and the call returns (normalised, residual_out)."""
+        if x.dim() != 2 or x.shape[1] != self.hidden_size or x.dtype != torch.bfloat16:
+            raise RuntimeError(f"ep_forward: x must be bfloat16 [T, {self.hidden_size}], got "
+                               f"{tuple(x.shape)} in {x.dtype}")
         T = x.shape[0]
-        k = top_k if top_k is not None else topk_ids.shape[1]
+        if topk_ids is None:
+            if router_logits is None or top_k is None or router_logits.dtype != x.dtype or \
+                    tuple(router_logits.shape) != (T, self.num_experts):
+                raise RuntimeError("ep_forward: needs router logits [T, num_experts] in x's dtype and "
+                                   "top_k, or a choice")
+            k = top_k
+        else:
+            k = topk_ids.shape[-1] if top_k is None else top_k
+            if topk_ids.dtype != torch.int64 or topk_weights is None or \
+                    not tuple(topk_ids.shape) == tuple(topk_weights.shape) == (T, k):
+                raise RuntimeError("ep_forward: topk_ids must be int64 [T, k] with topk_weights [T, k]")
+        for t in (router_logits, topk_ids, topk_weights, self.w_gate_up):
+            if t is not None and t.device != x.device:
+                raise RuntimeError(f"ep_forward: tensors are on {t.device} and {x.device}")
+        if not x.is_cuda:
+            raise RuntimeError("ep_forward: prism MoE kernels run on CUDA tensors only")
         if self._p2p is None or self._p2p["top_k"] != k:
             self.reserve(T, k)
         st = self._p2p

@@ -37,6 +37,29 @@ def test_scored_expert_parallel_step_is_one_graph(fuse):
     assert f"prism_moe.ep_forward_routed{'_norm' if fuse else ''}.default" in called
 
 
+def test_choices_that_do_not_fit_the_step():
+    """The step's kernels read [T, k] int64 ids and [T, E] logits, whatever they are given."""
+    bank = ExpertParallelMoE(H, I, E, 2, 0, transport="p2p").to(torch.bfloat16)
+    bf16 = torch.bfloat16
+    x = torch.zeros(5, H, dtype=bf16)
+    ids, w = torch.zeros(5, K, dtype=torch.int64), torch.zeros(5, K, dtype=bf16)
+    choice = dict(topk_ids=ids, topk_weights=w)
+    for bad in (dict(choice, topk_ids=ids.int()), dict(choice, topk_ids=ids[:4]),
+                dict(choice, topk_weights=w[:, :1]), dict(choice, topk_weights=None),
+                dict(choice, topk_ids=ids[0]), dict(choice, top_k=K + 1),
+                dict(choice, topk_ids=ids.to("meta")),
+                dict(router_logits=torch.zeros(5, E, dtype=bf16)), dict(top_k=K),
+                dict(router_logits=torch.zeros(5, E), top_k=K),
+                dict(router_logits=torch.zeros(5, E - 1, dtype=bf16), top_k=K)):
+        with pytest.raises(RuntimeError, match="ep_forward"):
+            bank.forward_p2p(x, **bad)
+    for bad in (x.float(), x[:, :-1], x[0]):
+        with pytest.raises(RuntimeError, match="ep_forward: x must be"):
+            bank.forward_p2p(bad, **choice)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        bank.forward_p2p(x, **choice)
+
+
 def test_a_bank_that_is_not_there():
     x = torch.zeros(2, H, dtype=torch.bfloat16)
     ids, w = torch.zeros(2, K, dtype=torch.int64), torch.zeros(2, K, dtype=torch.bfloat16)
