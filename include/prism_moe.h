@@ -92,10 +92,11 @@ typedef struct prism_moe_router {
  *   ids   = the k experts with the largest keys, in descending order; equal keys (and equal group
  *           scores) go to the lowest index
  *   w     = s[ids] (without the bias), / (their sum + 1e-20) with renorm, * scale
- * The choice is that of 64-bit keys. Weights are computed in fp32, within 2^-18 of their value, and
- * rounded to weights_dtype; a score under 2^-126 keeps what an fp32 subnormal holds (2^-148). NaN
- * keys rank above all numbers, as torch.topk ranks them. A NaN logit makes its token's weights NaN:
- * all of them with softmax or renorm, else its own. Experts of groups that do not stay are never
+ * The choice is that of 64-bit keys (a softmax's sum rounds in an order of its own: keys of a row that
+ * differ by one such rounding may come either way). Weights are computed in fp32, within 2^-18 of
+ * their value, and rounded to weights_dtype; a score under 2^-126 keeps what an fp32 subnormal holds
+ * (2^-148). NaN keys rank above all numbers, as torch.topk ranks them. A NaN logit makes its token's
+ * weights NaN: all of them with softmax or renorm, else its own. Experts of groups that do not stay are never
  * chosen, whatever the others hold.
  *   logits [T, E] dtype; topk_ids [T, k] int64 out; topk_weights [T, k] weights_dtype out;
  *   expert_counts [E] int32 out, or NULL.
